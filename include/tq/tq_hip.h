@@ -221,6 +221,34 @@ int tq_hip_decode_step_norm_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq, 
                                   const float *d_q_norm, const float *d_k_norm, float rms_eps,
                                   const float *d_cos, const float *d_sin, float *d_out, void *stream);
 
+/* ---- a cache of bounded size: eviction by gathered attention weight -------
+ * No counterpart in the reference.  Each (sequence, kv head) has a row of
+ * `stride` totals and of text positions, one per cache slot, kept by the caller:
+ * total[(s*n_kv_heads + h)*stride + slot].  Of the d_len[i] tokens of sequence
+ * d_seq[i] (NULL: sequence i) each kv head keeps `keep`: those whose text
+ * position is below `sinks` or at least d_next[i] - `recent` (d_next: the
+ * position of the sequence's next token, NULL: d_len) rank first, the others by
+ * their total, NaN last; equal ranks go to the lower slot.  The i-th kept token
+ * in a slot at or past `keep` moves into the i-th slot below it whose token is
+ * dropped, its K and V rows, its total and its position; every other kept token
+ * stays where it is.  Then each head's kept tokens are slots [0, min(len, keep)),
+ * in an order that attention does not depend on: the next token is appended at
+ * that slot, with its own text position's cos/sin, and pages past it may be
+ * unmapped.  Slots at or past `keep` keep what they held.
+ *
+ * d_total_out and d_where_out are the inputs themselves (in place: only moved
+ * entries are written) or two other arrays of that shape, which receive the kept
+ * slots' entries; nothing else of them is written.  Lengths are cut to max_len
+ * and sequences outside the cache are skipped; a sequence appears at most once
+ * per call, and its tokens' pages are mapped and its own.  sinks + recent at most
+ * keep; n at most 65535.  d_ws: tq_hip_kv_evict_ws_bytes, 16-byte aligned,
+ * nothing is kept in it between calls. */
+size_t tq_hip_kv_evict_ws_bytes(const tq_hip_kv *kv, int n, int max_len, int keep);
+int tq_hip_kv_evict_async(tq_hip_kv *kv, int n, const int32_t *d_seq, const int32_t *d_len, int max_len,
+                          const int32_t *d_next, int keep, int sinks, int recent, const float *d_total,
+                          const int32_t *d_where, float *d_total_out, int32_t *d_where_out, size_t stride, void *d_ws,
+                          size_t ws_bytes, void *stream);
+
 /* ---- prefill: the attention loop of attention_layer_batch
  * (model/attention_layer.c:203-204,221-236): tokens pos0..pos0+n-1 of `seq`,
  * each stored then attending causally to [0, pos0+i].  q [n][nq*hd], k/v
@@ -364,6 +392,43 @@ int tq_hip_embed_lookup_q4_batch(const void *embed, int rows, int cols, const in
  * logits (strict >, so NaN never wins and ties keep the lower index), written
  * to out[0] on the device. */
 int tq_hip_sample_greedy(const float *logits, int n, int32_t *out, void *stream);
+
+/* Rules on the logits of a batch, before a token is chosen (no counterpart in
+ * the reference).  Every pointer is device memory, 4-byte aligned; a NULL array
+ * leaves its rule out.  Lists have a row of `*_stride` entries per logits row,
+ * of which the first *_len[row] count (a longer length is cut to the stride);
+ * ids outside [0, vocab) are ignored. */
+typedef struct {
+    const int32_t *tokens;    /* the row's text so far: prompt, then answer     */
+    size_t tok_stride;
+    const int32_t *tok_len;
+    const int32_t *prompt_len; /* tokens of it that are the prompt (NULL: none)  */
+    const float *repetition;  /* [rows], > 0: divides a positive logit of a     */
+                              /*   token in the text, multiplies another (1)    */
+    const float *presence;    /* [rows]: taken off once if in the answer (0)    */
+    const float *frequency;   /* [rows]: taken off per time in the answer (0)   */
+    const int32_t *bias_ids;  /* token ids; the last entry of an id counts      */
+    const float *bias_vals;
+    size_t bias_stride;
+    const int32_t *bias_len;
+    const uint32_t *mask;     /* bit t % 32 of word t / 32 allows token t       */
+    size_t mask_stride;       /* words per row, or 0: one mask for every row    */
+} tq_hip_logits_rules;
+
+/* Device workspace of tq_hip_logits_process with a d_token, or 0 for a bad shape. */
+size_t tq_hip_logits_ws_bytes(int rows, int vocab);
+/* Row r of vocab logits at logits + r*stride through the rules (NULL: none) into
+ * out + r*out_stride (in place where out == logits and the strides agree; NULL:
+ * not written).  In this order, each step rounded to fp32: repetition, frequency
+ * times the count, presence, bias, and -inf for a token that the mask does not
+ * allow.  d_token[r] (NULL: not wanted) is the first index of the row's largest
+ * result, as sample_greedy (model/sampler.c:3-13) takes it, but -1 for a row
+ * whose results are all -inf or NaN, such as one whose mask leaves nothing.
+ * rows at most 65535; d_ws (tq_hip_logits_ws_bytes, 16-byte aligned) is needed
+ * with a d_token only and holds nothing between calls.  Asynchronous on
+ * `stream`, on the current device. */
+int tq_hip_logits_process(const float *logits, size_t stride, int rows, int vocab, const tq_hip_logits_rules *rules,
+                          float *out, size_t out_stride, int32_t *d_token, void *d_ws, size_t ws_bytes, void *stream);
 
 /* ---- the whole attention layer on the device --------------------------- */
 

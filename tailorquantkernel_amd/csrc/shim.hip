@@ -50,6 +50,24 @@ int herr(hipError_t e) { return e == hipSuccess ? TQ_HIP_OK : TQ_HIP_EHIP_BASE -
         if (e_ != hipSuccess) return herr(e_); \
     } while (0)
 
+// The cache's device as the current one while a call runs, the caller's after it.
+struct OnDevice {
+    int was = -1;
+    int rc = TQ_HIP_OK;
+    explicit OnDevice(int device) {
+        int now = device;
+        rc = herr(hipGetDevice(&now));
+        if (rc != TQ_HIP_OK || now == device) return;
+        rc = herr(hipSetDevice(device));
+        if (rc == TQ_HIP_OK) was = now;
+    }
+    ~OnDevice() {
+        if (was >= 0) (void)hipSetDevice(was);
+    }
+    OnDevice(const OnDevice &) = delete;
+    OnDevice &operator=(const OnDevice &) = delete;
+};
+
 hipStream_t pick(tq_hip_kv *kv, void *stream) {
     return stream ? static_cast<hipStream_t>(stream) : kv->stream;
 }
@@ -989,6 +1007,51 @@ int tq_hip_attend(tq_hip_kv *kv, int seq, int pos, const float *q, const float *
                        nullptr, nullptr, out_slot(kv, oo, qb), s, seq, nullptr, nullptr, 0.0f, nullptr, &done);
     if (rc != TQ_HIP_OK) return rc;
     return copy_out_sync(kv, out, oo, qb, &done);
+}
+
+// ---- eviction --------------------------------------------------------------------
+
+size_t tq_hip_kv_evict_ws_bytes(const tq_hip_kv *kv, int n, int max_len, int keep) {
+    if (!kv || n <= 0 || max_len <= 0 || keep <= 0) return 0;
+    return (size_t)n * kv->desc.n_kv_heads * tq_evict_list_ints(max_len, keep) * sizeof(int32_t);
+}
+
+int tq_hip_kv_evict_async(tq_hip_kv *kv, int n, const int32_t *d_seq, const int32_t *d_len, int max_len,
+                          const int32_t *d_next, int keep, int sinks, int recent, const float *d_total,
+                          const int32_t *d_where, float *d_total_out, int32_t *d_where_out, size_t stride, void *d_ws,
+                          size_t ws_bytes, void *stream) {
+    if (!kv || n < 0 || keep <= 0 || sinks < 0 || recent < 0 || sinks > keep || recent > keep - sinks)
+        return TQ_HIP_EINVAL;
+    if (n == 0) return TQ_HIP_OK;
+    if (n > 65535 || kv->desc.n_kv_heads > 65535) return TQ_HIP_EINVAL;   // grid dimensions
+    if (max_len <= 0 || stride < (size_t)max_len) return TQ_HIP_EINVAL;
+    if (max_len > (long)kv->desc.max_pages_per_seq * TQ_HIP_PAGE_TOKENS) return TQ_HIP_EINVAL;
+    if (!d_len || !d_total || !d_where || !d_total_out || !d_where_out || !d_ws) return TQ_HIP_EINVAL;
+    if ((d_total_out == d_total) != (d_where_out == d_where)) return TQ_HIP_EINVAL;
+    if (((uintptr_t)d_len | (uintptr_t)d_seq | (uintptr_t)d_next | (uintptr_t)d_total | (uintptr_t)d_where |
+         (uintptr_t)d_total_out | (uintptr_t)d_where_out) & 3)
+        return TQ_HIP_EINVAL;
+    if (((uintptr_t)d_ws & 15) || ws_bytes < tq_hip_kv_evict_ws_bytes(kv, n, max_len, keep)) return TQ_HIP_EINVAL;
+    if (!d_seq && n > kv->desc.max_seqs) return TQ_HIP_EINVAL;
+    const OnDevice on(kv->device);
+    if (on.rc != TQ_HIP_OK) return on.rc;
+    TqEvictArgs a;
+    a.view = kv->view;
+    a.n = n;
+    a.seq_of = d_seq;
+    a.len_of = d_len;
+    a.next_of = d_next;
+    a.max_len = max_len;
+    a.keep = keep;
+    a.sinks = sinks;
+    a.recent = recent;
+    a.total = d_total;
+    a.where = d_where;
+    a.total_out = d_total_out;
+    a.where_out = d_where_out;
+    a.stride = stride;
+    a.list = static_cast<int32_t *>(d_ws);
+    return herr(tq_launch_evict(a, pick(kv, stream)));
 }
 
 // ---- prefill ---------------------------------------------------------------------

@@ -360,3 +360,22 @@ void tq_prefill_scratch(int head_dim, int group, int n_kv_heads, int pos0, int n
 bool tq_prefill_mfma_supported(int head_dim, int group, int kend);
 size_t tq_prefill_image_bytes(int head_dim, int group, int n_kv_heads, int pos0, int n);
 hipError_t tq_launch_prefill(const TqPrefillArgs &a, hipStream_t s);
+
+// tq_hip_kv_evict_async (evict.hip): n sequences' tokens chosen and moved.
+struct TqEvictArgs {
+    tq::PagedView view;
+    int n;
+    const int32_t *seq_of;   // [n], or null: sequence i
+    const int32_t *len_of;   // [n]
+    const int32_t *next_of;  // [n], or null: the lengths
+    int max_len;
+    int keep, sinks, recent;
+    const float *total;      // [max_seqs][n_kv_heads][stride]
+    const int32_t *where;
+    float *total_out;        // both or neither equal to the inputs
+    int32_t *where_out;
+    size_t stride;
+    int32_t *list;           // [n][n_kv_heads][tq_evict_list_ints]
+};
+size_t tq_evict_list_ints(int max_len, int keep);
+hipError_t tq_launch_evict(const TqEvictArgs &a, hipStream_t s);

@@ -100,6 +100,10 @@ _PROTOS = {
     "tq_hip_project_output_q4": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _vp]),
     "tq_hip_embed_lookup_q4": (_i, [_vp, _i, _i, _i, _vp, _vp]),
     "tq_hip_embed_lookup_q4_batch": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp]),
+    "tq_hip_kv_evict_ws_bytes": (_sz, [_vp, _i, _i, _i]),
+    "tq_hip_kv_evict_async": (_i, [_vp, _i, _vp, _vp, _i, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp]),
+    "tq_hip_logits_ws_bytes": (_sz, [_i, _i]),
+    "tq_hip_logits_process": (_i, [_vp, _sz, _i, _i, _vp, _vp, _sz, _vp, _vp, _sz, _vp]),
 }
 
 EXPORTS = tuple(_PROTOS)
@@ -167,6 +171,15 @@ class AttnWeights(C.Structure):
     _fields_ = [("wq", C.c_void_p), ("wk", C.c_void_p), ("wv", C.c_void_p), ("wo", C.c_void_p),
                 ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("hidden", C.c_int), ("rms_eps", C.c_float),
                 ("format", C.c_int)]
+
+
+class LogitsRules(C.Structure):
+    """tq_hip_logits_rules: device arrays of a batch's penalties, biases and masks."""
+    _fields_ = [("tokens", C.c_void_p), ("tok_stride", C.c_size_t), ("tok_len", C.c_void_p),
+                ("prompt_len", C.c_void_p), ("repetition", C.c_void_p), ("presence", C.c_void_p),
+                ("frequency", C.c_void_p), ("bias_ids", C.c_void_p), ("bias_vals", C.c_void_p),
+                ("bias_stride", C.c_size_t), ("bias_len", C.c_void_p), ("mask", C.c_void_p),
+                ("mask_stride", C.c_size_t)]
 
 
 class DeviceBuffer:
