@@ -221,6 +221,25 @@ int tq_hip_decode_step_norm_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq, 
                                   const float *d_q_norm, const float *d_k_norm, float rms_eps,
                                   const float *d_cos, const float *d_sin, float *d_out, void *stream);
 
+/* The same step, which also gathers what attention gives each cached token (no
+ * counterpart in the reference; what tq_hip_kv_evict_async goes by).  For the
+ * token of query i at slot p = d_pos[i] of sequence s, every kv head h and every
+ * slot t <= p, with the softmax weights w of the group's query heads:
+ *   total[(s*n_kv_heads + h)*stride + t]  = (t < p ? its value : 0) + sum w[t]
+ *   where[(s*n_kv_heads + h)*stride + p]  = d_at[i] (NULL: p)
+ * so a slot's total begins with the token that takes it.  d_at is the token's
+ * position in its text, which after an eviction is past its slot; d_where may be
+ * NULL.  Slots past p are not touched, nor anything for a negative d_pos[i].
+ * Head dims 32/64/128 with groups 1..8, TQ_HIP_ETYPE otherwise; fp32 arrays
+ * 16-byte aligned (the totals 4), d_pos at most max_pos < stride.  d_ws:
+ * tq_hip_decode_step_weights_ws_bytes (0: a shape that is not served), 16-byte
+ * aligned, nothing is kept in it between calls. */
+size_t tq_hip_decode_step_weights_ws_bytes(const tq_hip_kv *kv, int n_q, int max_pos);
+int tq_hip_decode_step_weights_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq, const int32_t *d_pos, int max_pos,
+                                     const float *d_q, const float *d_k, const float *d_v, const float *d_cos,
+                                     const float *d_sin, float *d_out, const int32_t *d_at, float *d_total,
+                                     int32_t *d_where, size_t stride, void *d_ws, size_t ws_bytes, void *stream);
+
 /* ---- a cache of bounded size: eviction by gathered attention weight -------
  * No counterpart in the reference.  Each (sequence, kv head) has a row of
  * `stride` totals and of text positions, one per cache slot, kept by the caller:

@@ -231,8 +231,28 @@ __device__ __forceinline__ void norm8(float (&x)[8], float inv, const float *w) 
     for (int i = 0; i < 8; i++) x[i] = norm1(x[i], inv, ww[i]);
 }
 
+// x = hi + mid + lo, each the bf16 of what the ones before it leave: x to 2^-25.
+__device__ __forceinline__ void split3_bf16(const float (&x)[8], v8bf &hi, v8bf &mid, v8bf &lo) {
+    float rest[8];
+    u32x4 h;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t w = bf16_pair(x[2 * i], x[2 * i + 1]);
+        h[i] = w;
+        rest[2 * i] = x[2 * i] - __uint_as_float(w << 16);
+        rest[2 * i + 1] = x[2 * i + 1] - __uint_as_float(w & 0xFFFF0000u);
+    }
+    hi = __builtin_bit_cast(v8bf, h);
+    split_bf16(rest, mid, lo);
+}
+
 // W waves per work-group (4, or 8 when each wave has only a tile or two).
-template <int HD, int G, int W>
+// SC (the step that gathers weights): every score goes to a.scores, always as a
+// partial of its split, and the combine is left to decode_weights_kernel, which
+// follows; W is split in three parts instead of two, so that out is as exact as
+// the weights beside it (2^-25 instead of 2^-18 per term; the third product
+// and its split take no time beside the stream: 64 sequences of 512-8,192).
+template <int HD, int G, int W, bool SC>
 __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
     using L = L3<HD, G>;
     constexpr int kWaves = W;
@@ -667,8 +687,27 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
             }
         }
 
+        if constexpr (SC) {
+            // the tile's scores [key][head]: the NB lanes of a head hold the
+            // same 8 keys' scores and store 8 / NB of them each, whole runs of
+            // heads (G = 4, hd 128: two stores of 256 contiguous bytes)
+            float *dst = a.scores + (((size_t)qi * a.n_kv_heads + kvh) * a.score_stride + k0) * G;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                const int h = (16 * nt + l16) / NB;
+#pragma unroll
+                for (int i0 = 0; i0 < 8; i0 += NB) {
+                    float v = sc[nt][i0];
+#pragma unroll
+                    for (int j = 1; j < NB; j++) v = bl == j ? sc[nt][i0 + j] : v;
+                    if (h < G) dst[(slot_key(lg, i0) + bl) * G + h] = v + moff[nt];
+                }
+            }
+        }
+
         // W = exp2(S - moff) * vd <= 2^kLazy * vd, split into bf16 hi | lo
         v8bf whi[NT], wlo[NT];
+        [[maybe_unused]] v8bf wmid[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             float w[8];
@@ -686,7 +725,10 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
                 for (int i = 0; i < 8; i++) w[i] = k0 + slot_key(lg, i) < t_end ? w[i] : 0.0f;
             }
             l_part[nt] += ps;
-            split_bf16(w, whi[nt], wlo[nt]);
+            if constexpr (SC)
+                split3_bf16(w, whi[nt], wmid[nt], wlo[nt]);
+            else
+                split_bf16(w, whi[nt], wlo[nt]);
         }
 
         // P.V: A = V codes of 16 columns x the 32 keys in slot order
@@ -704,6 +746,7 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 o[c][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, whi[nt], o[c][nt], 0, 0, 0);
+                if constexpr (SC) o[c][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, wmid[nt], o[c][nt], 0, 0, 0);
                 o[c][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, wlo[nt], o[c][nt], 0, 0, 0);
             }
         }
@@ -784,7 +827,7 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
 
     const size_t out_row = (size_t)qi * a.n_q_heads + (size_t)kvh * G;
     const size_t pbase = ((size_t)qi * a.n_kv_heads + kvh) * a.n_splits;
-    const bool single = a.n_splits == 1;
+    const bool single = !SC && a.n_splits == 1;
     // Float4 f4 / 4 of this (query, kv head)'s G output rows.  With completion
     // flags the rows are stored through to system scope, every wave waits for
     // its acknowledgements, and then one lane raises the flag: a host that sees
@@ -842,6 +885,7 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
             }
         }
     }
+    if constexpr (SC) return;
     if (single) {
         if (a.done) signal_done();
         return;
@@ -931,26 +975,27 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
     if (a.done) signal_done();
 }
 
-template <int HD, int G>
+template <int HD, int G, bool SC>
 hipError_t launch3_hd_g(const TqDecodeArgs &a, int waves, hipStream_t s) {
+    const dim3 grid(a.n_splits, a.n_kv_heads, a.n_q);
     if (waves == 8)
-        hipLaunchKernelGGL((decode3_kernel<HD, G, 8>), dim3(a.n_splits, a.n_kv_heads, a.n_q), dim3(512), 0, s, a);
+        hipLaunchKernelGGL((decode3_kernel<HD, G, 8, SC>), grid, dim3(512), 0, s, a);
     else
-        hipLaunchKernelGGL((decode3_kernel<HD, G, 4>), dim3(a.n_splits, a.n_kv_heads, a.n_q), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((decode3_kernel<HD, G, 4, SC>), grid, dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
-template <int HD>
+template <int HD, bool SC>
 hipError_t launch3_hd(const TqDecodeArgs &a, int g, int waves, hipStream_t s) {
     switch (g) {
-        case 1: return launch3_hd_g<HD, 1>(a, waves, s);
-        case 2: return launch3_hd_g<HD, 2>(a, waves, s);
-        case 3: return launch3_hd_g<HD, 3>(a, waves, s);
-        case 4: return launch3_hd_g<HD, 4>(a, waves, s);
-        case 5: return launch3_hd_g<HD, 5>(a, waves, s);
-        case 6: return launch3_hd_g<HD, 6>(a, waves, s);
-        case 7: return launch3_hd_g<HD, 7>(a, waves, s);
-        case 8: return launch3_hd_g<HD, 8>(a, waves, s);
+        case 1: return launch3_hd_g<HD, 1, SC>(a, waves, s);
+        case 2: return launch3_hd_g<HD, 2, SC>(a, waves, s);
+        case 3: return launch3_hd_g<HD, 3, SC>(a, waves, s);
+        case 4: return launch3_hd_g<HD, 4, SC>(a, waves, s);
+        case 5: return launch3_hd_g<HD, 5, SC>(a, waves, s);
+        case 6: return launch3_hd_g<HD, 6, SC>(a, waves, s);
+        case 7: return launch3_hd_g<HD, 7, SC>(a, waves, s);
+        case 8: return launch3_hd_g<HD, 8, SC>(a, waves, s);
         default: return hipErrorInvalidValue;
     }
 }
@@ -972,13 +1017,15 @@ hipError_t tq_launch_decode3(const TqDecodeArgs &a, int waves, hipStream_t s) {
     if (a.n_splits < 1 || a.n_splits > kMaxSplits3 || a.split_tokens <= 0 || a.split_tokens % kTK != 0 ||
         a.split_tokens > kMaxSplitPages3 * kPage)
         return hipErrorInvalidValue;
-    if (a.n_splits > 1 && (a.partials == nullptr || a.counters == nullptr)) return hipErrorInvalidValue;
+    if (a.scores ? !a.partials || a.score_stride < (long)a.n_splits * a.split_tokens
+                 : a.n_splits > 1 && (a.partials == nullptr || a.counters == nullptr))
+        return hipErrorInvalidValue;
     const int g = a.n_q_heads / a.n_kv_heads;
     if (!tq_decode3_supported(a.head_dim, g)) return hipErrorInvalidValue;
     switch (a.head_dim) {
-        case 32: return launch3_hd<32>(a, g, waves, s);
-        case 64: return launch3_hd<64>(a, g, waves, s);
-        case 128: return launch3_hd<128>(a, g, waves, s);
+        case 32: return a.scores ? launch3_hd<32, true>(a, g, waves, s) : launch3_hd<32, false>(a, g, waves, s);
+        case 64: return a.scores ? launch3_hd<64, true>(a, g, waves, s) : launch3_hd<64, false>(a, g, waves, s);
+        case 128: return a.scores ? launch3_hd<128, true>(a, g, waves, s) : launch3_hd<128, false>(a, g, waves, s);
         default: return hipErrorInvalidValue;
     }
 }

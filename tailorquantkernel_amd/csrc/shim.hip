@@ -180,6 +180,26 @@ void plan_splits3(const tq_hip_kv *kv, int n_q, int max_len, int waves, int *spl
     *n_splits = (int)((units + per - 1) / per);
 }
 
+// Waves per work-group, and the splits, of the MFMA decode.
+//
+// four waves per work-group: for a single 4k-token sequence at the 8B
+// shape this spreads one 32-key tile per wave over all 256 CUs, which beats
+// eight waves on half of them (8.7 against 9.1 us per step).  A batch at
+// G <= 4 takes eight: two resident work-groups per CU then stream 16 tiles
+// at once (the 64-sequence batch: 117 against 129 us); at G = 8 four waves
+// stay ahead (234 against 240 us at 16 x 32k tokens).
+int plan_decode3(const tq_hip_kv *kv, int n_q, int max_len, int *split_tokens, int *n_splits) {
+    int waves = n_q > 1 && kv->desc.n_q_heads / kv->desc.n_kv_heads <= 4 ? 8 : 4;
+    // one query over at most 256 keys: eight waves of one 32-key tile each in
+    // one work-group per kv head, with no split-K combine (its store, counter
+    // and pull cost more than the tiles: 8B shape at 256 keys 7.1 -> 6.2 us,
+    // 8q/2kv/hd64 6.6 -> 5.3 us; from 384 keys on the splits win)
+    if (n_q == 1 && max_len <= 8 * 32) waves = 8;
+    if (decode3_waves_env()) waves = decode3_waves_env();
+    plan_splits3(kv, n_q, max_len, waves, split_tokens, n_splits);
+    return waves;
+}
+
 // Longest context one decode call serves for this cache's shape.
 long max_context(const tq_hip_kv *kv) {
     const int g = kv->desc.n_q_heads / kv->desc.n_kv_heads;
@@ -437,17 +457,27 @@ struct CallScratch {
     size_t counter_ints;
 };
 
+// Where a step that gathers weights leaves its splits' partials and its scores;
+// decode_common fills in the splits.
+struct ScoreScratch {
+    float *partials;
+    float *scores;
+    int split_tokens;
+    int n_splits;
+};
+
 // contig_seq: the one sequence every query of this call reads, or -1.
 // q_norm non-null: q (and the new K) are raw projections, RMSNorm'd in the
 // kernel with q_norm / k_norm and eps (MFMA kernel only).
 // scratch non-null: the split-K partials and counters come from it (a call
 // that needs more returns TQ_HIP_ESCRATCH) and nothing is allocated.
+// ss non-null: the first half of a step that gathers weights (MFMA kernel only).
 int decode_common(tq_hip_kv *kv, int n_q, const int32_t *d_seq, const int32_t *d_len, int len_plus,
                   int seq_const, int seq_stride, int pos0, int max_len, const float *d_q, const float *d_cos,
                   const float *d_sin, const float *d_k, const float *d_v, float *d_out,
                   hipStream_t s, int contig_seq, const float *q_norm = nullptr,
                   const float *k_norm = nullptr, float rms_eps = 0.0f, const CallScratch *scratch = nullptr,
-                  DoneFlags *done = nullptr) {
+                  DoneFlags *done = nullptr, ScoreScratch *ss = nullptr) {
     if (n_q <= 0) return TQ_HIP_OK;
     // queries and kv heads are grid dimensions y/z (at most 65535 each)
     if (n_q > 65535 || kv->desc.n_kv_heads > 65535) return TQ_HIP_EINVAL;
@@ -498,24 +528,22 @@ int decode_common(tq_hip_kv *kv, int n_q, const int32_t *d_seq, const int32_t *d
         if (((uintptr_t)q_norm | (uintptr_t)k_norm) & 15) return TQ_HIP_EINVAL;
         if (!v3) return TQ_HIP_ETYPE;
     }
-    // four waves per work-group: for a single 4k-token sequence at the 8B
-    // shape this spreads one 32-key tile per wave over all 256 CUs, which beats
-    // eight waves on half of them (8.7 against 9.1 us per step).  A batch at
-    // G <= 4 takes eight: two resident work-groups per CU then stream 16 tiles
-    // at once (the 64-sequence batch: 117 against 129 us); at G = 8 four waves
-    // stay ahead (234 against 240 us at 16 x 32k tokens).
     const int g = D.n_q_heads / D.n_kv_heads;
-    int waves = n_q > 1 && g <= 4 ? 8 : 4;
-    // one query over at most 256 keys: eight waves of one 32-key tile each in
-    // one work-group per kv head, with no split-K combine (its store, counter
-    // and pull cost more than the tiles: 8B shape at 256 keys 7.1 -> 6.2 us,
-    // 8q/2kv/hd64 6.6 -> 5.3 us; from 384 keys on the splits win)
-    if (n_q == 1 && max_len <= 8 * 32) waves = 8;
-    if (decode3_waves_env()) waves = decode3_waves_env();
+    int waves = 0;
     if (v3)
-        plan_splits3(kv, n_q, max_len, waves, &a.split_tokens, &a.n_splits);
+        waves = plan_decode3(kv, n_q, max_len, &a.split_tokens, &a.n_splits);
     else
         plan_splits(kv, n_q, max_len, &a.split_tokens, &a.n_splits);
+    if (ss) {
+        // scores and partials go where the caller planned them (plan_decode3 again)
+        if (!v3) return TQ_HIP_ETYPE;
+        a.partials = ss->partials;
+        a.scores = ss->scores;
+        a.score_stride = a.n_splits * a.split_tokens;
+        ss->split_tokens = a.split_tokens;
+        ss->n_splits = a.n_splits;
+        return herr(tq_launch_decode3(a, waves, s));
+    }
     if (a.n_splits > 1) {
         const size_t row = v3 ? (size_t)tq_decode3_partial_floats(D.head_dim, g) : (size_t)g * (D.head_dim + 2);
         const size_t bytes = (size_t)n_q * D.n_kv_heads * a.n_splits * row * sizeof(float);
@@ -979,6 +1007,72 @@ int tq_hip_decode_step_norm_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq, 
     if (!d_seq && n_q > kv->desc.max_seqs) return TQ_HIP_EINVAL;
     return decode_common(kv, n_q, d_seq, d_pos, 1, 0, 1, 0, max_pos + 1, d_q, d_cos, d_sin, d_k, d_v, d_out,
                          pick(kv, stream), (!d_seq && n_q == 1) ? 0 : -1, d_q_norm, d_k_norm, rms_eps);
+}
+
+// The workspace of a step that gathers weights: partials, then scores.
+static size_t weights_ws(const tq_hip_kv *kv, int n_q, int max_len, size_t *scores_at) {
+    const tq_hip_kv_desc &D = kv->desc;
+    int split_tokens = 0, n_splits = 0;
+    plan_decode3(kv, n_q, max_len, &split_tokens, &n_splits);
+    const int g = D.n_q_heads / D.n_kv_heads;
+    const size_t pairs = (size_t)n_q * D.n_kv_heads;
+    const size_t partials = pairs * n_splits * tq_decode3_partial_floats(D.head_dim, g) * sizeof(float);
+    *scores_at = (partials + 255) & ~(size_t)255;
+    return *scores_at + pairs * n_splits * split_tokens * g * sizeof(float);
+}
+
+size_t tq_hip_decode_step_weights_ws_bytes(const tq_hip_kv *kv, int n_q, int max_pos) {
+    if (!kv || n_q <= 0 || n_q > 65535 || max_pos < 0 || max_pos >= max_context(kv) || !use_decode3(kv)) return 0;
+    size_t scores_at;
+    return weights_ws(kv, n_q, max_pos + 1, &scores_at);
+}
+
+int tq_hip_decode_step_weights_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq, const int32_t *d_pos, int max_pos,
+                                     const float *d_q, const float *d_k, const float *d_v, const float *d_cos,
+                                     const float *d_sin, float *d_out, const int32_t *d_at, float *d_total,
+                                     int32_t *d_where, size_t stride, void *d_ws, size_t ws_bytes, void *stream) {
+    if (!kv || n_q < 0 || max_pos < 0) return TQ_HIP_EINVAL;
+    if (n_q == 0) return TQ_HIP_OK;
+    if (n_q > 65535 || kv->desc.n_kv_heads > 65535 || max_pos >= max_context(kv)) return TQ_HIP_EINVAL;
+    if (!d_pos || !d_q || !d_k || !d_v || !d_out || !d_total || !d_ws) return TQ_HIP_EINVAL;
+    if ((d_cos == nullptr) != (d_sin == nullptr) || stride < (size_t)max_pos + 1) return TQ_HIP_EINVAL;
+    if (!d_seq && n_q > kv->desc.max_seqs) return TQ_HIP_EINVAL;
+    if (((uintptr_t)d_q | (uintptr_t)d_k | (uintptr_t)d_v | (uintptr_t)d_cos | (uintptr_t)d_sin | (uintptr_t)d_out |
+         (uintptr_t)d_ws) & 15)
+        return TQ_HIP_EINVAL;
+    if (((uintptr_t)d_seq | (uintptr_t)d_pos | (uintptr_t)d_at | (uintptr_t)d_total | (uintptr_t)d_where) & 3)
+        return TQ_HIP_EINVAL;
+    if (!use_decode3(kv)) return TQ_HIP_ETYPE;
+    size_t scores_at;
+    if (ws_bytes < weights_ws(kv, n_q, max_pos + 1, &scores_at)) return TQ_HIP_EINVAL;
+    const OnDevice on(kv->device);
+    if (on.rc != TQ_HIP_OK) return on.rc;
+    unsigned char *ws = static_cast<unsigned char *>(d_ws);
+    ScoreScratch ss{reinterpret_cast<float *>(ws), reinterpret_cast<float *>(ws + scores_at), 0, 0};
+    const hipStream_t s = pick(kv, stream);
+    const int rc = decode_common(kv, n_q, d_seq, d_pos, 1, 0, 1, 0, max_pos + 1, d_q, d_cos, d_sin, d_k, d_v, d_out, s,
+                                 (!d_seq && n_q == 1) ? 0 : -1, nullptr, nullptr, 0.0f, nullptr, nullptr, &ss);
+    if (rc != TQ_HIP_OK) return rc;
+    TqWeightsArgs a;
+    a.seq_of = d_seq;
+    a.pos_of = d_pos;
+    a.at_of = d_at;
+    a.max_len = max_pos + 1;
+    a.max_seqs = kv->desc.max_seqs;
+    a.n_q = n_q;
+    a.n_q_heads = kv->desc.n_q_heads;
+    a.n_kv_heads = kv->desc.n_kv_heads;
+    a.head_dim = kv->desc.head_dim;
+    a.partials = ss.partials;
+    a.scores = ss.scores;
+    a.score_stride = ss.n_splits * ss.split_tokens;
+    a.split_tokens = ss.split_tokens;
+    a.n_splits = ss.n_splits;
+    a.out = d_out;
+    a.total = d_total;
+    a.where = d_where;
+    a.stride = stride;
+    return herr(tq_launch_decode_weights(a, s));
 }
 
 int tq_hip_attend(tq_hip_kv *kv, int seq, int pos, const float *q, const float *cos_t, const float *sin_t,

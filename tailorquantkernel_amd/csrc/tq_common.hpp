@@ -249,6 +249,11 @@ struct TqDecodeArgs {
     // at system scope and acknowledged, then done[i * n_kv_heads + h] = done_seq.
     unsigned *done;
     unsigned done_seq;
+    // The step that gathers weights (MFMA kernel only), or null: every score
+    // (exp2 domain) goes to scores[query][kv head][score_stride][group], every
+    // split leaves a partial, and tq_launch_decode_weights finishes the call.
+    float *scores;
+    int score_stride;        // >= n_splits * split_tokens
 };
 
 hipError_t tq_launch_quantize(const float *x, block_q8 *out, int n, hipStream_t s);
@@ -318,6 +323,27 @@ int tq_decode3_partial_floats(int head_dim, int group);
 // waves: 4 or 8 per work-group; split_tokens a multiple of 32*waves keeps the
 // waves' tile counts equal.
 hipError_t tq_launch_decode3(const TqDecodeArgs &a, int waves, hipStream_t s);
+
+// After tq_launch_decode3 with scores on the same stream: out from the splits'
+// partials, and each token's softmax weight, summed over the group's heads,
+// added to its total.
+struct TqWeightsArgs {
+    const int32_t *seq_of;   // or null: query i is sequence i
+    const int32_t *pos_of;   // the new token's slot; the totals' tokens are [0, pos]
+    const int32_t *at_of;    // its text position, or null: pos_of
+    int max_len;
+    int max_seqs;
+    int n_q, n_q_heads, n_kv_heads, head_dim;
+    const float *partials;   // tq_launch_decode3's
+    const float *scores;
+    int score_stride;
+    int split_tokens, n_splits;
+    float *out;              // [n_q][n_q_heads][hd]
+    float *total;            // [max_seqs][n_kv_heads][stride]
+    int32_t *where;          // the same shape, or null
+    size_t stride;
+};
+hipError_t tq_launch_decode_weights(const TqWeightsArgs &a, hipStream_t s);
 
 struct TqPrefillArgs {
     tq::PagedView view;

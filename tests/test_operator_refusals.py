@@ -57,3 +57,10 @@ def test_evict_without_a_cache(nat):
     assert lib.tq_hip_kv_evict_ws_bytes(None, 1, 64, 32) == 0
     assert lib.tq_hip_kv_evict_async(None, 1, None, P, 64, None, 32, 0, 0, P, P, P, P, 64, P, 1 << 20,
                                      None) == nat.EINVAL
+
+
+def test_step_weights_without_a_cache(nat):
+    lib = nat.load()
+    assert lib.tq_hip_decode_step_weights_ws_bytes(None, 1, 64) == 0
+    assert lib.tq_hip_decode_step_weights_async(None, 1, None, P, 64, P, P, P, P, P, P, None, P, P, 65, P, 1 << 20,
+                                                None) == nat.EINVAL
