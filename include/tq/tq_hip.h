@@ -278,6 +278,25 @@ int tq_hip_prefill_async(tq_hip_kv *kv, int seq, int pos0, int n, const float *d
                          const float *d_k, const float *d_v, const float *d_cos,
                          const float *d_sin, float *d_out, void *stream);
 
+/* The same for n_seqs sequences at once, their rows one behind the other: sequence
+ * seq[i] (NULL: i) has rows start[i] .. start[i+1]-1 of q, k, v, cos/sin and out,
+ * its tokens pos0[i] (NULL: 0) .. pos0[i] + start[i+1] - start[i] - 1.  Rows
+ * before start[0] and from start[n_seqs] on are neither read nor written; a
+ * sequence may have no rows.  seq, pos0 and start (n_seqs + 1 entries, none less
+ * than the one before) are HOST arrays, read during the call.  TQ_HIP_EINVAL,
+ * before any launch, for a sequence that appears twice or that has no page for one
+ * of its tokens; a page that takes a token of one sequence is no other's.  Head
+ * dims 64/128 with groups 1..8 and up to 65,536 tokens a sequence take the dense
+ * kernel (arrays 16-byte aligned), which keeps P and V to 2^-22 where
+ * tq_hip_prefill_async keeps 2^-16 (and no term below 2^-29 of the largest V scale
+ * so far); other shapes attend row by row as decode steps do.  d_ws: tq_hip_prefill_packed_ws_bytes for the same pos0 and
+ * start (0: a call that is refused), 16-byte aligned; nothing is kept in it. */
+size_t tq_hip_prefill_packed_ws_bytes(const tq_hip_kv *kv, int n_seqs, const int32_t *pos0, const int32_t *start);
+int tq_hip_prefill_packed_async(tq_hip_kv *kv, int n_seqs, const int32_t *seq, const int32_t *pos0,
+                                const int32_t *start, const float *d_q, const float *d_k, const float *d_v,
+                                const float *d_cos, const float *d_sin, float *d_out, void *d_ws, size_t ws_bytes,
+                                void *stream);
+
 /* ---- the weight side: Q8 weight matrices and the projections -----------
  *
  * A weight matrix lives on the device in the "tiled Q8" layout, the same

@@ -148,7 +148,25 @@ __global__ __launch_bounds__(kThreads) void append_run_kernel(PagedView view, in
     }
 }
 
+// Sequence and position of every row of the packed sequences: grid (rows of the
+// longest / 256, sequence).
+__global__ __launch_bounds__(256) void pack_rows_kernel(TqPackTable t, int row0, int32_t *seq_of, int32_t *pos_of) {
+    const int i = blockIdx.y, r = (int)blockIdx.x * 256 + (int)threadIdx.x;
+    if (r >= t.n[i]) return;
+    seq_of[t.start[i] - row0 + r] = t.seq[i];
+    pos_of[t.start[i] - row0 + r] = t.pos0[i] + r;
+}
+
 }  // namespace
+
+hipError_t tq_launch_pack_rows(const TqPackTable &t, int row0, int32_t *seq_of, int32_t *pos_of, hipStream_t s) {
+    int longest = 0;
+    for (int i = 0; i < t.n_seqs; i++) longest = t.n[i] > longest ? t.n[i] : longest;
+    if (longest == 0) return hipSuccess;
+    hipLaunchKernelGGL(pack_rows_kernel, dim3((unsigned)((longest - 1) / 256 + 1), (unsigned)t.n_seqs), dim3(256), 0, s,
+                       t, row0, seq_of, pos_of);
+    return hipGetLastError();
+}
 
 hipError_t tq_launch_append(const PagedView &view, int n_rows, const int32_t *seq,
                             const int32_t *pos, int seq_const, int pos0, const float *k,

@@ -8,6 +8,7 @@
 #include <time.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <mutex>
 #include <new>
 #include <vector>
@@ -90,6 +91,8 @@ int decode_wg_target(int n_q) {
 
 // Fewest new tokens for which a prefill call uses the dense kernel.
 constexpr int kPrefillDenseMin = 32;
+// Longest sequence the packed prefill's dense form serves.
+constexpr int kMaxPackKeys = 65536;
 
 // The dense MFMA prefill kernel (default) or, with TQ_HIP_PREFILL_DENSE=0,
 // the decode kernel run once per token with causal lengths.
@@ -1287,6 +1290,211 @@ int tq_hip_prefill(tq_hip_kv *kv, int seq, int pos0, int n, const float *q, cons
     return copy_out_sync(kv, out, oo, qb, &done);
 }
 
+// ---- prefill of several sequences ----------------------------------------
+
+namespace {
+
+// Rows per decode launch of the row form: bounds its split-K partials.
+constexpr int kPackRows = 2048;
+
+// Walk the sequences of a packed call that have rows, longest first, in tables
+// of up to TQ_MAX_PACK.
+struct PackWalk {
+    std::vector<int> order;
+    const int32_t *seq, *pos0, *start;
+    PackWalk(int n_seqs, const int32_t *seq_, const int32_t *pos0_, const int32_t *start_)
+        : seq(seq_), pos0(pos0_), start(start_) {
+        order.reserve((size_t)n_seqs);
+        for (int i = 0; i < n_seqs; i++)
+            if (start[i + 1] > start[i]) order.push_back(i);
+        std::stable_sort(order.begin(), order.end(), [this](int a, int b) { return end(a) > end(b); });
+    }
+    int first(int i) const { return pos0 ? pos0[i] : 0; }
+    int end(int i) const { return first(i) + start[i + 1] - start[i]; }
+    size_t tables() const { return (order.size() + TQ_MAX_PACK - 1) / TQ_MAX_PACK; }
+    void fill(size_t table, TqPackTable &t) const {
+        const size_t at = table * TQ_MAX_PACK;
+        t = TqPackTable{};
+        t.n_seqs = (int)std::min<size_t>(TQ_MAX_PACK, order.size() - at);
+        for (int j = 0; j < t.n_seqs; j++) {
+            const int i = order[at + j];
+            t.seq[j] = seq ? seq[i] : i;
+            t.pos0[j] = first(i);
+            t.start[j] = start[i];
+            t.n[j] = start[i + 1] - start[i];
+        }
+    }
+    int longest() const { return order.empty() ? 0 : end(order[0]); }
+};
+
+// Whether a packed call's arrays are in order; `rows` and `longest` of it.
+bool pack_ok(int n_seqs, const int32_t *pos0, const int32_t *start) {
+    if (start[0] < 0) return false;
+    for (int i = 0; i < n_seqs; i++) {
+        if (start[i + 1] < start[i] || (pos0 && pos0[i] < 0)) return false;
+        if ((long)(pos0 ? pos0[i] : 0) + start[i + 1] - start[i] > INT32_MAX - TQ_HIP_PAGE_TOKENS) return false;
+    }
+    return true;
+}
+
+bool pack_dense(const tq_hip_kv *kv, int longest, uintptr_t addresses) {
+    const tq_hip_kv_desc &D = kv->desc;
+    return prefill_dense() && (addresses & 15) == 0 && tq_pack_supported(D.head_dim, D.n_q_heads / D.n_kv_heads) &&
+           longest <= kMaxPackKeys;
+}
+
+// The row form's workspace: sequence and position of each row, the decode
+// launches' counters and partials, whichever decode kernel runs them.
+struct PackRows {
+    size_t pos, counters, partials, bytes, counter_ints, partial_bytes;
+};
+PackRows pack_rows_space(const tq_hip_kv *kv, int rows, int longest) {
+    auto al = [](size_t x) { return (x + 255) & ~(size_t)255; };
+    const tq_hip_kv_desc &D = kv->desc;
+    const int g = D.n_q_heads / D.n_kv_heads;
+    PackRows w{};
+    for (const int n : {std::min(rows, kPackRows), rows % kPackRows}) {
+        if (n <= 0) continue;
+        int per = 0, splits = 0;
+        size_t row = 0;
+        if (use_decode3(kv)) {
+            plan_decode3(kv, n, longest, &per, &splits);
+            row = splits > 1 ? (size_t)splits * tq_decode3_partial_floats(D.head_dim, g) : 0;
+        }
+        plan_splits(kv, n, longest, &per, &splits);
+        row = std::max(row, splits > 1 ? (size_t)splits * g * (D.head_dim + 2) : 0);
+        w.partial_bytes = std::max(w.partial_bytes, (size_t)n * D.n_kv_heads * row * sizeof(float));
+    }
+    w.counter_ints = (size_t)std::min(rows, kPackRows) * D.n_kv_heads * TQ_DECODE_COUNTER_STRIDE;
+    w.pos = al((size_t)rows * sizeof(int32_t));
+    w.counters = 2 * w.pos;
+    w.partials = w.counters + al(w.counter_ints * sizeof(int));
+    w.bytes = w.partials + w.partial_bytes;
+    return w;
+}
+
+int pack_by_rows(tq_hip_kv *kv, const PackWalk &walk, int row0, int rows, const float *d_q, const float *d_k,
+                 const float *d_v, const float *d_cos, const float *d_sin, float *d_out, unsigned char *ws,
+                 hipStream_t s) {
+    const tq_hip_kv_desc &D = kv->desc;
+    const PackRows w = pack_rows_space(kv, rows, walk.longest());
+    int32_t *seq_of = reinterpret_cast<int32_t *>(ws), *pos_of = reinterpret_cast<int32_t *>(ws + w.pos);
+    TqPackTable t;
+    for (size_t i = 0; i < walk.tables(); i++) {
+        walk.fill(i, t);
+        TQ_TRY(tq_launch_pack_rows(t, row0, seq_of, pos_of, s));
+    }
+    hipLaunchKernelGGL(zero_words_kernel, dim3(64), dim3(256), 0, s, reinterpret_cast<uint32_t *>(ws + w.counters),
+                       w.counter_ints);
+    TQ_TRY(hipGetLastError());
+    const size_t qd = (size_t)D.n_q_heads * D.head_dim, kd = (size_t)D.n_kv_heads * D.head_dim, half = D.head_dim / 2;
+    const float *cos0 = d_cos ? d_cos + (size_t)row0 * half : nullptr, *sin0 = d_sin ? d_sin + (size_t)row0 * half : nullptr;
+    TQ_TRY(tq_launch_append(kv->view, rows, seq_of, pos_of, 0, 0, d_k + (size_t)row0 * kd, d_v + (size_t)row0 * kd, cos0,
+                            sin0, D.head_dim, s));
+    const CallScratch sc{reinterpret_cast<float *>(ws + w.partials), w.partial_bytes,
+                         reinterpret_cast<int *>(ws + w.counters), w.counter_ints};
+    for (int r = 0; r < rows; r += kPackRows) {
+        const size_t at = (size_t)row0 + r;
+        const int rc = decode_common(kv, std::min(kPackRows, rows - r), seq_of + r, pos_of + r, 1, 0, 1, 0, walk.longest(),
+                                     d_q + at * qd, d_cos ? d_cos + at * half : nullptr,
+                                     d_sin ? d_sin + at * half : nullptr, nullptr, nullptr, d_out + at * qd, s, -1,
+                                     nullptr, nullptr, 0.0f, &sc);
+        if (rc != TQ_HIP_OK) return rc;
+    }
+    return TQ_HIP_OK;
+}
+
+// The larger of the two forms' workspaces: which one runs also depends on the
+// call's addresses.
+size_t pack_bytes(const tq_hip_kv *kv, const PackWalk &walk, int rows) {
+    const tq_hip_kv_desc &D = kv->desc;
+    const int g = D.n_q_heads / D.n_kv_heads;
+    size_t bytes = pack_rows_space(kv, rows, walk.longest()).bytes;
+    if (pack_dense(kv, walk.longest(), 0)) {
+        TqPackTable t;
+        for (size_t i = 0; i < walk.tables(); i++) {
+            walk.fill(i, t);
+            bytes = std::max(bytes, tq_pack_bytes(D.head_dim, g, D.n_kv_heads, t));
+        }
+    }
+    return bytes;
+}
+
+}  // namespace
+
+size_t tq_hip_prefill_packed_ws_bytes(const tq_hip_kv *kv, int n_seqs, const int32_t *pos0, const int32_t *start) {
+    if (!kv || n_seqs <= 0 || !start || !pack_ok(n_seqs, pos0, start)) return 0;
+    try {
+        const PackWalk walk(n_seqs, nullptr, pos0, start);
+        if (walk.longest() > max_context(kv)) return 0;
+        return std::max<size_t>(16, pack_bytes(kv, walk, start[n_seqs] - start[0]));
+    } catch (...) {
+        return 0;
+    }
+}
+
+int tq_hip_prefill_packed_async(tq_hip_kv *kv, int n_seqs, const int32_t *seq, const int32_t *pos0,
+                                const int32_t *start, const float *d_q, const float *d_k, const float *d_v,
+                                const float *d_cos, const float *d_sin, float *d_out, void *d_ws, size_t ws_bytes,
+                                void *stream) {
+    if (!kv || n_seqs < 0) return TQ_HIP_EINVAL;
+    if (n_seqs == 0) return TQ_HIP_OK;
+    if (!start || !pack_ok(n_seqs, pos0, start) || n_seqs > kv->desc.max_seqs || kv->desc.n_kv_heads > 65535)
+        return TQ_HIP_EINVAL;
+    const int row0 = start[0], rows = start[n_seqs] - row0;
+    if (rows == 0) return TQ_HIP_OK;
+    if (!d_q || !d_k || !d_v || !d_out || !d_ws || ((d_cos == nullptr) != (d_sin == nullptr))) return TQ_HIP_EINVAL;
+    const uintptr_t addresses = (uintptr_t)d_q | (uintptr_t)d_k | (uintptr_t)d_v | (uintptr_t)d_cos | (uintptr_t)d_sin |
+                                (uintptr_t)d_out;
+    if ((addresses & 3) || ((uintptr_t)d_ws & 15)) return TQ_HIP_EINVAL;
+    try {
+        // every sequence of the cache, at most once, with pages for all its tokens
+        std::vector<char> taken((size_t)kv->desc.max_seqs, 0);
+        for (int i = 0; i < n_seqs; i++) {
+            const int q = seq ? seq[i] : i;
+            if (!seq_ok(kv, q) || taken[(size_t)q]) return TQ_HIP_EINVAL;
+            taken[(size_t)q] = 1;
+            const int n = start[i + 1] - start[i];
+            if (n == 0) continue;
+            const long pages = ((long)(pos0 ? pos0[i] : 0) + n - 1) / TQ_HIP_PAGE_TOKENS + 1;
+            if (pages > kv->desc.max_pages_per_seq) return TQ_HIP_EINVAL;
+            const int32_t *row = kv->h_page_table.data() + (size_t)q * kv->desc.max_pages_per_seq;
+            for (long p = 0; p < pages; p++)
+                if (row[p] < 0) return TQ_HIP_EINVAL;
+        }
+        const PackWalk walk(n_seqs, seq, pos0, start);
+        if (walk.longest() > max_context(kv)) return TQ_HIP_EINVAL;
+        if (ws_bytes < pack_bytes(kv, walk, rows)) return TQ_HIP_EINVAL;
+        const OnDevice on(kv->device);
+        if (on.rc != TQ_HIP_OK) return on.rc;
+        const hipStream_t s = pick(kv, stream);
+        unsigned char *ws = static_cast<unsigned char *>(d_ws);
+        const tq_hip_kv_desc &D = kv->desc;
+        if (!pack_dense(kv, walk.longest(), addresses))
+            return pack_by_rows(kv, walk, row0, rows, d_q, d_k, d_v, d_cos, d_sin, d_out, ws, s);
+        TqPackTable t;
+        TqPackArgs a;
+        a.view = kv->view;
+        a.table = &t;
+        a.q = d_q;
+        a.k = d_k;
+        a.v = d_v;
+        a.cos_t = d_cos;
+        a.sin_t = d_sin;
+        a.out = d_out;
+        a.n_q_heads = D.n_q_heads;
+        a.head_dim = D.head_dim;
+        a.scale = 1.0f / sqrtf((float)D.head_dim);
+        a.ws = ws;
+        for (size_t i = 0; i < walk.tables(); i++) {
+            walk.fill(i, t);
+            TQ_TRY(tq_launch_pack(a, s));
+        }
+        return TQ_HIP_OK;
+    } catch (...) {
+        return TQ_HIP_ENOMEM;
+    }
+}
 
 // ---- the whole attention layer -------------------------------------------
 

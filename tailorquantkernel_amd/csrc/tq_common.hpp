@@ -405,3 +405,34 @@ struct TqEvictArgs {
 };
 size_t tq_evict_list_ints(int max_len, int keep);
 hipError_t tq_launch_evict(const TqEvictArgs &a, hipStream_t s);
+
+// tq_hip_prefill_packed_async's dense form (prefill.hip): the sequences of one
+// launch, none of them empty, longest first.
+#define TQ_MAX_PACK 64
+struct TqPackTable {
+    int n_seqs;
+    int chunk;                      // the plan's: key tiles per run, or 0
+    int seq[TQ_MAX_PACK];
+    int pos0[TQ_MAX_PACK];
+    int start[TQ_MAX_PACK];         // first row
+    int n[TQ_MAX_PACK];             // rows
+    int tile0[TQ_MAX_PACK + 1];     // the plan's: first key tile, query block
+    int blk0[TQ_MAX_PACK + 1];      //   and run of each
+    int run0[TQ_MAX_PACK + 1];
+};
+struct TqPackArgs {
+    tq::PagedView view;
+    const TqPackTable *table;
+    const float *q, *k, *v;         // rows of all sequences, 16-byte aligned
+    const float *cos_t, *sin_t;     // or null
+    float *out;
+    int n_q_heads;
+    int head_dim;
+    float scale;
+    unsigned char *ws;              // tq_pack_bytes
+};
+bool tq_pack_supported(int head_dim, int group);
+size_t tq_pack_bytes(int head_dim, int group, int n_kv_heads, TqPackTable &t);
+hipError_t tq_launch_pack(const TqPackArgs &a, hipStream_t s);
+// The row form's tables: seq_of[r - row0] and pos_of[r - row0] of every row of the table's sequences.
+hipError_t tq_launch_pack_rows(const TqPackTable &t, int row0, int32_t *seq_of, int32_t *pos_of, hipStream_t s);

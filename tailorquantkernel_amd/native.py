@@ -100,6 +100,8 @@ _PROTOS = {
     "tq_hip_project_output_q4": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _vp]),
     "tq_hip_embed_lookup_q4": (_i, [_vp, _i, _i, _i, _vp, _vp]),
     "tq_hip_embed_lookup_q4_batch": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp]),
+    "tq_hip_prefill_packed_ws_bytes": (_sz, [_vp, _i, _vp, _vp]),
+    "tq_hip_prefill_packed_async": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "tq_hip_decode_step_weights_ws_bytes": (_sz, [_vp, _i, _i]),
     "tq_hip_decode_step_weights_async": (_i, [_vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
                                              _vp, _sz, _vp]),

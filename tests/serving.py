@@ -88,7 +88,7 @@ class Cache:
         self.nat.check(self.lib.tq_hip_device_synchronize(), "sync")
 
 
-def attention(cache, q_blocks, rows, last):
+def attention(cache, q_blocks, rows, last, term=2.0 ** -17):
     """Query rows q_blocks [m][nq][nb], row r over keys rows[0..last[r]] ([n][nkv][2][nb]): outputs [m][nq][hd], their
     error bound in fp32, weights [m][nq][n] and theirs (relative).
 
@@ -97,7 +97,7 @@ def attention(cache, q_blocks, rows, last):
     row, so it is off by (3 nb + 6) 2^-24 S and the weight by ln 2 times that; exp2 and its argument's subtraction add
     2^-23 and ln 2 * 126 * 2^-24 (beyond 126 the weight is nothing).  A sum of n non-negative terms in any order of
     partial sums is off by at most n 2^-24 of itself.  A weight is such a term over such a sum.  An output is such a
-    sum of weights times values, each product kept to 2^-17 where weights and values are split in two bf16 parts.
+    sum of weights times values, each product kept to `term` (2^-17 where they are split in two bf16 parts).
     """
     nq, nkv, hd, nb = cache.nq, cache.nkv, cache.hd, cache.nb
     group, n, m = nq // nkv, rows.shape[0], q_blocks.shape[0]
@@ -117,5 +117,5 @@ def attention(cache, q_blocks, rows, last):
         one = 2.0 ** -24 * (2 * np.log(2) * ((3 * nb + 6) * size + 126) + 4 + n)
         weights[:, h], loose[:, h] = w, one
         out[:, h] = w @ vh
-        bound[:, h] = (w @ np.abs(vh)) * (one + 2.0 ** -24 * n + 2.0 ** -17)[:, None]
+        bound[:, h] = (w @ np.abs(vh)) * (one + 2.0 ** -24 * n + term)[:, None]
     return out, bound, weights, loose

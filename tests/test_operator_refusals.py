@@ -64,3 +64,10 @@ def test_step_weights_without_a_cache(nat):
     assert lib.tq_hip_decode_step_weights_ws_bytes(None, 1, 64) == 0
     assert lib.tq_hip_decode_step_weights_async(None, 1, None, P, 64, P, P, P, P, P, P, None, P, P, 65, P, 1 << 20,
                                                 None) == nat.EINVAL
+
+
+def test_prefill_packed_without_a_cache(nat):
+    lib, start = nat.load(), (C.c_int32 * 2)(0, 4)
+    assert lib.tq_hip_prefill_packed_ws_bytes(None, 1, None, C.addressof(start)) == 0
+    assert lib.tq_hip_prefill_packed_async(None, 1, None, None, C.addressof(start), P, P, P, P, P, P, P, 1 << 20,
+                                           None) == nat.EINVAL
