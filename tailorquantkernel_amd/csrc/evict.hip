@@ -14,11 +14,17 @@
 // one token for each new one moves one row where closing the gap in order
 // would move all behind it.
 //
-// evict_select_kernel, one work-group per (sequence, kv head): the keep-th
-//   largest key by radix selection (digits of 11, 11 and 10 bits, a histogram
-//   in LDS each), then the slots in order: wave w owns one sixteenth of them,
-//   so ranks are ballots within a wave and one sum over the waves before it.
-// evict_move_kernel: the listed rows, K and V, in whole pieces.
+// evict_select_kernel, one work-group per (sequence, kv head), holds the keys in
+//   registers (the one pass over totals and positions) and finds the keep-th
+//   largest by counting: the codes between the smallest and the largest key are
+//   cut into 2,048 bins, those of the bin that holds the edge again, until a bin
+//   is one code.  Bins over the range that the keys really have spread them
+//   (digits of the code itself put totals of like size into a few bins, whose
+//   counters then take a wave's adds one by one), and a second round sees a few
+//   keys only.  Wave w owns one run of slots, so ranks in slot order are ballots
+//   within a wave and one sum over the waves before it.
+// evict_move_kernel: the listed rows, K and V, in whole pieces; a few rows are
+//   moved by the selecting work-group itself.
 #include <algorithm>
 
 #include "tq_common.hpp"
@@ -27,10 +33,9 @@ namespace {
 
 using namespace tq;
 
-constexpr int kSelThreads = 1024;
-constexpr int kSelWaves = kSelThreads / 64;
 constexpr int kBins = 2048;
 constexpr uint32_t kSafe = 0xFFFFFFFFu;
+constexpr int kFewMoves = 128;       // most moves a work-group makes itself
 
 struct EvictArgs {
     PagedView view;
@@ -52,24 +57,73 @@ __device__ __forceinline__ int32_t *list_of(const EvictArgs &a, int i, int kvh) 
     return a.list + ((size_t)i * a.view.n_kv_heads + kvh) * (2 * (size_t)a.cap + 4);
 }
 
-// Order-preserving code of a total: NaN below -inf, never kSafe.
+// Order-preserving code of a total, at least 1 (NaN, below -inf) and less than
+// kSafe; 0 is no token.
 __device__ __forceinline__ uint32_t total_key(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);   // -0 ranks as 0
     const uint32_t k = (u & 0x80000000u) ? ~u : u | 0x80000000u;
-    return x != x ? 0u : k;
+    return x != x ? 1u : k;
 }
 
-__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
+// Largest of 64 lanes' values, and each lane's sum of the lanes up to it.
+__device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
+    x = max(x, dpp_u<kDppQuadXor1>(x));
+    x = max(x, dpp_u<kDppQuadXor2>(x));
+    x = max(x, dpp_u<kDppRowHalfMirror>(x));
+    x = max(x, dpp_u<kDppRowMirror>(x));
+    auto at = [&](int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)x, lane); };
+    return max(max(at(0), at(16)), max(at(32), at(48)));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+    // row_shr 1, 2, 4, 8 within the rows of 16, then the rows before
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xF, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xF, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xF, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xF, 0xF, false);
+    const uint32_t r0 = (uint32_t)__builtin_amdgcn_readlane((int)x, 15), r1 = (uint32_t)__builtin_amdgcn_readlane((int)x, 31),
+                   r2 = (uint32_t)__builtin_amdgcn_readlane((int)x, 47);
+    const int row = (threadIdx.x & 63) >> 4;
+    return x + (row > 0 ? r0 : 0u) + (row > 1 ? r1 : 0u) + (row > 2 ? r2 : 0u);
+}
+
+// Row piece q (of 2 * per: K's, then V's) of a move, VB bytes, and with the
+// first one the token's total and position.
+template <int VB>
+__device__ __forceinline__ void move_piece(const EvictArgs &a, int seq, int kvh, size_t row, int to, int from, int q,
+                                           int per) {
+    typedef uint32_t piece_t __attribute__((ext_vector_type(VB / 4)));
+    const PagedView &v = a.view;
+    const int kv = q >= per, c = q - kv * per;
+    const int pt = phys_page(v, seq, to / kPage), pf = phys_page(v, seq, from / kPage);
+    if (pt >= 0 && pf >= 0) {
+        const unsigned char *src = head_run_ptr(v, pf, kvh) + kv * v.kv_chunk + (from % kPage) * v.row_bytes + c * VB;
+        unsigned char *dst = head_run_ptr(v, pt, kvh) + kv * v.kv_chunk + (to % kPage) * v.row_bytes + c * VB;
+        *reinterpret_cast<piece_t *>(dst) = *reinterpret_cast<const piece_t *>(src);
+    }
+    if (q == 0) {
+        a.total_out[row + to] = a.total[row + from];
+        a.where_out[row + to] = a.where[row + from];
+    }
+}
+
+// PER > 0: up to PER keys a lane, in registers.  PER == 0: any length, each
+// look at a key reads its total and position again.  FEW: the moves (at most
+// kFewMoves) are made here; else they are listed for evict_move_kernel.
+template <int WAVES, int PER, bool FEW>
+__global__ __launch_bounds__(64 * WAVES) void evict_select_kernel(EvictArgs a) {
+    constexpr int THREADS = 64 * WAVES;
+    constexpr int BPT = kBins / THREADS;     // bins per thread in the scan
     __shared__ uint32_t hist[kBins];
-    __shared__ uint32_t wsum[kSelWaves], wtie[kSelWaves];
-    __shared__ uint32_t pick[2];     // the chosen bin, and the keys wanted in it
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ uint32_t w1[WAVES], w2[WAVES], w3[WAVES];
+    __shared__ uint32_t pick[3];             // the chosen bin, the keys wanted in it, the keys it has
+    __shared__ int few[FEW ? 2 * kFewMoves : 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kvh = blockIdx.x, i = blockIdx.y;
     const int seq = a.seq_of ? a.seq_of[i] : i;
-    int32_t *list = list_of(a, i, kvh);
+    int32_t *list = FEW ? nullptr : list_of(a, i, kvh);
     const int len = min(a.len_of[i], a.max_len);
     if (seq < 0 || seq >= a.view.max_seqs || len <= 0) {
-        if (tid == 0) list[0] = 0;
+        if (!FEW && tid == 0) list[0] = 0;
         return;
     }
     const size_t row = ((size_t)seq * a.view.n_kv_heads + kvh) * a.stride;
@@ -79,9 +133,9 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
     int32_t *where_out = a.where_out + row;
     const bool copy = a.total_out != a.total;
     if (len <= a.keep) {
-        if (tid == 0) list[0] = 0;
+        if (!FEW && tid == 0) list[0] = 0;
         if (copy)
-            for (int t = tid; t < len; t += kSelThreads) {
+            for (int t = tid; t < len; t += THREADS) {
                 total_out[t] = total[t];
                 where_out[t] = where[t];
             }
@@ -89,140 +143,285 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
     }
     const int next = a.next_of ? a.next_of[i] : len;
     const long window = (long)next - a.recent;
-    auto key_at = [&](int t) -> uint32_t {
-        const int p = where[t];
-        return p < a.sinks || p >= window ? kSafe : total_key(total[t]);
+    const int per = (len + THREADS - 1) / THREADS;
+    const int w0 = wave * per * 64 + lane;   // this lane's slots: w0 + 64 j
+    auto key_of = [&](int t, float x, int p) -> uint32_t {
+        return t >= len ? 0u : p < a.sinks || p >= window ? kSafe : total_key(x);
     };
-
-    // the keep-th largest key, digit by digit from the top
-    uint32_t prefix = 0, known = 0, want = (uint32_t)a.keep;
-    for (int d = 0; d < 3; d++) {
-        const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, bins = d == 2 ? 1024 : 2048;
-        for (int b = tid; b < kBins; b += kSelThreads) hist[b] = 0;
-        __syncthreads();
-        for (int t = tid; t < len; t += kSelThreads) {
-            const uint32_t k = key_at(t);
-            if ((k & known) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
-        }
-        __syncthreads();
-        // bins from the top: thread t holds bins 2t, 2t+1 counted down
-        const int hi = bins - 1 - 2 * tid;
-        const uint32_t c0 = hi >= 0 ? hist[hi] : 0u, c1 = hi >= 1 ? hist[hi - 1] : 0u;
-        uint32_t sum = c0 + c1;
+    uint32_t keys[PER ? PER : 1];
+    if constexpr (PER > 0) {
+        constexpr int B = PER < 16 ? PER : 16;   // loads in flight together, twice
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint32_t o = __shfl_up(sum, off);
-            if (lane >= off) sum += o;
+        for (int j0 = 0; j0 < PER; j0 += B) {
+            if (j0 >= per) break;
+            float x[B];
+            int p[B];
+#pragma unroll
+            for (int j = 0; j < B; j++) {
+                const int t = min(w0 + 64 * (j0 + j), len - 1);
+                x[j] = total[t];
+                p[j] = where[t];
+            }
+#pragma unroll
+            for (int j = 0; j < B; j++) {
+                const int t = w0 + 64 * (j0 + j);
+                keys[j0 + j] = key_of(t, x[j], p[j]);
+                // every slot of the budget is written: what stays here, what moves in over it
+                if (copy && j0 + j < per && t < a.keep) {
+                    total_out[t] = x[j];
+                    where_out[t] = p[j];
+                }
+            }
         }
-        if (lane == 63) wsum[wave] = sum;
-        __syncthreads();
-        uint32_t before = 0;
-        for (int w = 0; w < wave; w++) before += wsum[w];
-        const uint32_t above = before + sum - c0 - c1;
-        if (above < want && want <= above + c0) {
-            pick[0] = (uint32_t)hi;
-            pick[1] = want - above;
-        } else if (above + c0 < want && want <= above + c0 + c1) {
-            pick[0] = (uint32_t)(hi - 1);
-            pick[1] = want - above - c0;
-        }
-        __syncthreads();
-        prefix |= pick[0] << shift;
-        known |= (uint32_t)(bins - 1) << shift;
-        want = pick[1];
-        __syncthreads();
-    }
-    const uint32_t edge = prefix;        // the keep-th largest key; `want` of its ties stay
-
-    // ranks in slot order: wave w's slots are one run
-    const int per = (len + kSelThreads - 1) / kSelThreads;
-    const int w0 = wave * per * 64;
-    uint32_t ties = 0;
-    for (int j = 0; j < per; j++) {
-        const int t = w0 + 64 * j + lane;
-        const bool tie = t < len && key_at(t) == edge;
-        ties += __popcll(__ballot(tie));
-    }
-    if (lane == 0) wtie[wave] = ties;
-    __syncthreads();
-    uint32_t tie0 = 0;
-    for (int w = 0; w < wave; w++) tie0 += wtie[w];
-    const unsigned long long below = (1ull << lane) - 1;
-    uint32_t holes = 0, movers = 0, tie = tie0;
-    for (int j = 0; j < per; j++) {
-        const int t = w0 + 64 * j + lane;
-        const uint32_t k = t < len ? key_at(t) : 0u;
-        const bool eq = t < len && k == edge;
-        const unsigned long long m = __ballot(eq);
-        const bool stays = t < len && (k > edge || (eq && tie + __popcll(m & below) < want));
-        tie += __popcll(m);
-        holes += __popcll(__ballot(t < a.keep && t < len && !stays));
-        movers += __popcll(__ballot(t >= a.keep && stays));
-    }
-    __syncthreads();
-    if (lane == 0) {
-        wsum[wave] = holes;
-        wtie[wave] = movers;
-    }
-    __syncthreads();
-    uint32_t hole = 0, mover = 0, all = 0;
-    for (int w = 0; w < kSelWaves; w++) {
-        if (w < wave) {
-            hole += wsum[w];
-            mover += wtie[w];
-        }
-        all += wtie[w];
-    }
-    if (tid == 0) list[0] = (int32_t)all;
-    tie = tie0;
-    for (int j = 0; j < per; j++) {
-        const int t = w0 + 64 * j + lane;
-        const uint32_t k = t < len ? key_at(t) : 0u;
-        const bool eq = t < len && k == edge;
-        const unsigned long long m = __ballot(eq);
-        const bool stays = t < len && (k > edge || (eq && tie + __popcll(m & below) < want));
-        tie += __popcll(m);
-        const bool is_hole = t < a.keep && t < len && !stays, is_mover = t >= a.keep && stays;
-        const unsigned long long hm = __ballot(is_hole), mm = __ballot(is_mover);
-        const uint32_t h = hole + __popcll(hm & below), v = mover + __popcll(mm & below);
-        if (is_hole && h < (uint32_t)a.cap) list[4 + h] = t;
-        if (is_mover && v < (uint32_t)a.cap) list[4 + a.cap + v] = t;
-        if (copy && stays && t < a.keep) {
+    } else if (copy) {
+        for (int t = tid; t < a.keep; t += THREADS) {
             total_out[t] = total[t];
             where_out[t] = where[t];
         }
-        hole += __popcll(hm);
-        mover += __popcll(mm);
+    }
+    // f(slot of lane 0, key) for this wave's slots in order, 64 at a time
+    auto each = [&](auto f) {
+        if constexpr (PER > 0) {
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+                if (j >= per) break;
+                f(wave * per * 64 + 64 * j, keys[j]);
+            }
+        } else {
+            for (int j = 0; j < per; j++) {
+                const int t = w0 + 64 * j, r = min(t, len - 1);
+                f(wave * per * 64 + 64 * j, key_of(t, total[r], where[r]));
+            }
+        }
+    };
+    auto sum_before = [&](const uint32_t *w, uint32_t *all) {
+        uint32_t before = 0, sum = 0;
+#pragma unroll
+        for (int v = 0; v < WAVES; v++) {
+            before += v < wave ? w[v] : 0u;
+            sum += w[v];
+        }
+        if (all) *all = sum;
+        return before;
+    };
+
+    // how many are safe, and the range of the other keys
+    uint32_t safe = 0, lo = kSafe, hi = 0;
+    each([&](int, uint32_t k) {
+        const bool is_safe = k == kSafe;
+        safe += __popcll(__ballot(is_safe));
+        lo = min(lo, k - 1u);   // (no token: kSafe)
+        hi = max(hi, is_safe ? 0u : k);
+    });
+    lo = ~wave_umax(~lo);
+    hi = wave_umax(hi);
+    if (lane == 0) {
+        w1[wave] = safe;
+        w2[wave] = lo;
+        w3[wave] = hi;
+    }
+    __syncthreads();
+    safe = 0;
+#pragma unroll
+    for (int v = 0; v < WAVES; v++) {
+        safe += w1[v];
+        lo = min(lo, w2[v]);
+        hi = max(hi, w3[v]);
+    }
+    lo += 1u;
+
+    // the edge: the keep-th largest key, of whose ties `want` stay
+    uint32_t edge = kSafe, want = (uint32_t)a.keep;
+    if (safe < (uint32_t)a.keep) {
+        want -= safe;
+        while (lo != hi) {
+            // bins of 2^shift codes from lo up; the range shrinks to one of them
+            const int bits = 32 - __clz(hi - lo);
+            const int shift = bits > 11 ? bits - 11 : 0;
+            for (int b = tid; b < kBins; b += THREADS) hist[b] = 0;
+            __syncthreads();
+            each([&](int, uint32_t k) {
+                const uint32_t over = k - lo, bin = over >> shift;
+                const bool in = over <= hi - lo;
+                const unsigned long long m = __ballot(in);
+                if (m == 0) return;
+                // a wave of equal keys (totals still 0) makes one add, not 64 to one counter
+                const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)bin, __ffsll((long long)m) - 1);
+                if (__ballot(in && bin != first) == 0) {
+                    if (lane == 0) atomicAdd(&hist[first], (uint32_t)__popcll(m));
+                } else if (in) {
+                    atomicAdd(&hist[bin], 1u);
+                }
+            });
+            __syncthreads();
+            // thread t holds BPT bins, counted from the top
+            uint32_t c[BPT], sum = 0;
+            const int top = kBins - 1 - BPT * tid;
+#pragma unroll
+            for (int b = 0; b < BPT; b++) {
+                c[b] = hist[top - b];
+                sum += c[b];
+            }
+            const uint32_t incl = wave_scan(sum);
+            if (lane == 63) w1[wave] = incl;
+            __syncthreads();
+            uint32_t above = sum_before(w1, nullptr) + incl - sum;
+#pragma unroll
+            for (int b = 0; b < BPT; b++) {
+                if (above < want && want <= above + c[b]) {
+                    pick[0] = (uint32_t)(top - b);
+                    pick[1] = want - above;
+                    pick[2] = c[b];
+                }
+                above += c[b];
+            }
+            __syncthreads();
+            lo += pick[0] << shift;
+            hi = min(hi, lo + ((1u << shift) - 1u));
+            want = pick[1];
+            if (want == pick[2]) {   // all of the bin stay
+                want = kSafe;
+                break;
+            }
+        }
+        edge = lo;
+    }
+
+    // which of a wave's 64 slots stay, as a mask; where not all ties do, `tie`
+    // of them came before.  Called for the slots in order.
+    const bool all_ties = want == kSafe;
+    uint32_t tie = 0;
+    const unsigned long long below = (1ull << lane) - 1;
+    auto staying = [&](uint32_t k) {
+        if (all_ties) return __ballot(k >= edge);
+        const bool eq = k == edge;
+        const unsigned long long m = __ballot(eq);
+        const unsigned long long yes = __ballot(k > edge || (eq && tie + __popcll(m & below) < want));
+        tie += __popcll(m);
+        return yes;
+    };
+    // the slots of [t, t + 64) below keep
+    auto inside = [&](int t) {
+        const int n = a.keep - t;
+        return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
+    };
+    uint32_t tie0 = 0;
+    if (!all_ties) {
+        uint32_t ties = 0;
+        each([&](int, uint32_t k) { ties += __popcll(__ballot(k == edge)); });
+        __syncthreads();   // w1 is free again
+        if (lane == 0) w1[wave] = ties;
+        __syncthreads();
+        tie0 = sum_before(w1, nullptr);
+    }
+    uint32_t holes = 0, movers = 0;
+    tie = tie0;
+    each([&](int t, uint32_t k) {
+        const unsigned long long s = staying(k), in = inside(t);
+        holes += __popcll(in & ~s);   // (slots below keep are tokens: keep < len)
+        movers += __popcll(s & ~in);
+    });
+    if (lane == 0) {
+        w2[wave] = holes;
+        w3[wave] = movers;
+    }
+    __syncthreads();
+    uint32_t all = 0;
+    uint32_t hole = sum_before(w2, nullptr), mover = sum_before(w3, &all);
+    if (!FEW && tid == 0) list[0] = (int32_t)all;
+    int32_t *to_list = FEW ? few : list + 4, *from_list = FEW ? few + kFewMoves : list + 4 + a.cap;
+    tie = tie0;
+    each([&](int t, uint32_t k) {
+        const unsigned long long s = staying(k), in = inside(t), h = in & ~s, m = s & ~in;
+        if ((h >> lane) & 1) to_list[hole + __popcll(h & below)] = t + lane;
+        if ((m >> lane) & 1) from_list[mover + __popcll(m & below)] = t + lane;
+        hole += __popcll(h);
+        mover += __popcll(m);
+    });
+    if constexpr (FEW) {
+        __syncthreads();
+        const int vb = a.view.row_bytes % 16 == 0 ? 16 : a.view.row_bytes % 8 == 0 ? 8 : 4;
+        const int pieces = (int)a.view.row_bytes / vb, n = (int)all * 2 * pieces;
+        for (int p = tid; p < n; p += THREADS) {
+            const int m = p / (2 * pieces), q = p % (2 * pieces), to = few[m], from = few[kFewMoves + m];
+            if (vb == 16)
+                move_piece<16>(a, seq, kvh, row, to, from, q, pieces);
+            else if (vb == 8)
+                move_piece<8>(a, seq, kvh, row, to, from, q, pieces);
+            else
+                move_piece<4>(a, seq, kvh, row, to, from, q, pieces);
+        }
     }
 }
 
-// Piece p of the listed moves: K or V of one move, VB bytes.
-template <int VB>
+// The listed moves, kMoves per work-group: first where each row lies (one of
+// the moves' 2 kMoves ends per thread: list, page table), then the pieces, each
+// thread's loads all in flight before its stores.
+constexpr int kMoves = 64;
+template <int VB, int NB>
 __global__ __launch_bounds__(kThreads) void evict_move_kernel(EvictArgs a) {
     typedef uint32_t piece_t __attribute__((ext_vector_type(VB / 4)));
+    constexpr int PER = NB * kBlockBytes / VB;             // pieces of a row
+    constexpr int ALL = kMoves * 2 * PER;
+    constexpr int STEPS = (ALL + kThreads - 1) / kThreads;
+    static_assert(2 * kMoves <= kThreads, "one end per thread");
+    __shared__ long base[2][kMoves];                       // of the slot's K row in the pool, or -1
     const PagedView &v = a.view;
-    const int kvh = blockIdx.y, i = blockIdx.z;
+    const int tid = threadIdx.x, kvh = blockIdx.y, i = blockIdx.z;
     const int32_t *list = list_of(a, i, kvh);
-    const int count = min(list[0], a.cap);
+    const int m0 = (int)blockIdx.x * kMoves;
+    const int count = min(list[0], a.cap) - m0;            // of this work-group
+    if (count <= 0) return;
     const int seq = a.seq_of ? a.seq_of[i] : i;
-    const int per = (int)v.row_bytes / VB;            // pieces of a row
-    const int span = kThreads;                        // pieces per step of the grid
-    const size_t row = ((size_t)seq * v.n_kv_heads + kvh) * a.stride;
-    for (long p = (long)blockIdx.x * span + threadIdx.x; p < (long)count * 2 * per; p += (long)gridDim.x * span) {
-        const int m = (int)(p / (2 * per)), q = (int)(p % (2 * per));
-        const int kv = q / per, c = q % per;
-        const int to = list[4 + m], from = list[4 + a.cap + m];
-        const int pt = phys_page(v, seq, to / kPage), pf = phys_page(v, seq, from / kPage);
-        if (pt >= 0 && pf >= 0) {
-            const unsigned char *src = head_run_ptr(v, pf, kvh) + kv * v.kv_chunk + (from % kPage) * v.row_bytes + c * VB;
-            unsigned char *dst = head_run_ptr(v, pt, kvh) + kv * v.kv_chunk + (to % kPage) * v.row_bytes + c * VB;
-            *reinterpret_cast<piece_t *>(dst) = *reinterpret_cast<const piece_t *>(src);
+    if (tid < 2 * kMoves) {
+        const int end = tid / kMoves, m = tid % kMoves;
+        long at = -1;
+        if (m < count) {
+            const int t = list[4 + end * a.cap + m0 + m];
+            const int phys = phys_page(v, seq, t / kPage);
+            if (phys >= 0) at = (long)((size_t)phys * v.page_bytes + (size_t)kvh * v.head_run + (t % kPage) * v.row_bytes);
         }
-        if (q == 0) {
-            a.total_out[row + to] = a.total[row + from];
-            a.where_out[row + to] = a.where[row + from];
-        }
+        base[end][m] = at;
+    } else if (tid - 2 * kMoves < min(count, kMoves)) {
+        const int m = m0 + tid - 2 * kMoves, to = list[4 + m], from = list[4 + a.cap + m];
+        const size_t row = ((size_t)seq * v.n_kv_heads + kvh) * a.stride;
+        a.total_out[row + to] = a.total[row + from];
+        a.where_out[row + to] = a.where[row + from];
     }
+    __syncthreads();
+    // no branch around a load (the compiler would wait for each at its end): a
+    // piece that is not moved is read at the pool's start instead
+    piece_t x[STEPS];
+    long to[STEPS];
+#pragma unroll
+    for (int k = 0; k < STEPS; k++) {
+        const int p = tid + kThreads * k, m = min(p / (2 * PER), kMoves - 1), q = p % (2 * PER);
+        const long off = q >= PER ? (long)v.kv_chunk + (q - PER) * VB : (long)q * VB;
+        const long t = base[0][m], f = base[1][m];
+        const bool real = p < ALL && t >= 0 && f >= 0;
+        to[k] = real ? t + off : -1;
+        x[k] = *reinterpret_cast<const piece_t *>(v.pool + (real ? f + off : 0));
+    }
+#pragma unroll
+    for (int k = 0; k < STEPS; k++)
+        if (to[k] >= 0) *reinterpret_cast<piece_t *>(v.pool + to[k]) = x[k];
+}
+
+// 4 waves up to 1,024 tokens, 8 to 4,096, then 16: of 4,096, 4 / 8 / 16 waves take
+// 22.8 / 16.1 / 17.2 us (512 heads); more keys a lane than 32 spill.
+template <bool FEW>
+hipError_t launch_select(const EvictArgs &a, dim3 grid, hipStream_t s) {
+    if (a.max_len <= 4 * 64 * 4)
+        hipLaunchKernelGGL((evict_select_kernel<4, 4, FEW>), grid, dim3(256), 0, s, a);
+    else if (a.max_len <= 8 * 64 * 8)
+        hipLaunchKernelGGL((evict_select_kernel<8, 8, FEW>), grid, dim3(512), 0, s, a);
+    else if (a.max_len <= 16 * 64 * 16)
+        hipLaunchKernelGGL((evict_select_kernel<16, 16, FEW>), grid, dim3(1024), 0, s, a);
+    else if (a.max_len <= 16 * 64 * 32)
+        hipLaunchKernelGGL((evict_select_kernel<16, 32, FEW>), grid, dim3(1024), 0, s, a);
+    else
+        hipLaunchKernelGGL((evict_select_kernel<16, 0, FEW>), grid, dim3(1024), 0, s, a);
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -250,17 +449,17 @@ hipError_t tq_launch_evict(const TqEvictArgs &t, hipStream_t s) {
     a.list = t.list;
     a.cap = (int)((tq_evict_list_ints(t.max_len, t.keep) - 4) / 2);
     const int nkv = t.view.n_kv_heads;
-    hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)nkv, (unsigned)t.n), dim3(kSelThreads), 0, s, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.cap == 0) return e;
-    const int vb = t.view.row_bytes % 16 == 0 ? 16 : t.view.row_bytes % 8 == 0 ? 8 : 4;
-    const long pieces = (long)a.cap * 2 * (long)(t.view.row_bytes / vb);
-    const dim3 grid((unsigned)std::min<long>(256, (pieces + kThreads - 1) / kThreads), (unsigned)nkv, (unsigned)t.n);
-    if (vb == 16)
-        hipLaunchKernelGGL(evict_move_kernel<16>, grid, dim3(kThreads), 0, s, a);
-    else if (vb == 8)
-        hipLaunchKernelGGL(evict_move_kernel<8>, grid, dim3(kThreads), 0, s, a);
-    else
-        hipLaunchKernelGGL(evict_move_kernel<4>, grid, dim3(kThreads), 0, s, a);
+    const dim3 heads((unsigned)nkv, (unsigned)t.n);
+    if (a.cap <= kFewMoves) return launch_select<true>(a, heads, s);
+    const hipError_t e = launch_select<false>(a, heads, s);
+    if (e != hipSuccess) return e;
+    const dim3 grid((unsigned)((a.cap + kMoves - 1) / kMoves), (unsigned)nkv, (unsigned)t.n);
+    switch (t.view.nb) {
+        case 1: hipLaunchKernelGGL((evict_move_kernel<4, 1>), grid, dim3(kThreads), 0, s, a); break;
+        case 2: hipLaunchKernelGGL((evict_move_kernel<8, 2>), grid, dim3(kThreads), 0, s, a); break;
+        case 4: hipLaunchKernelGGL((evict_move_kernel<16, 4>), grid, dim3(kThreads), 0, s, a); break;
+        case 8: hipLaunchKernelGGL((evict_move_kernel<16, 8>), grid, dim3(kThreads), 0, s, a); break;
+        default: return hipErrorInvalidValue;
+    }
     return hipGetLastError();
 }
