@@ -68,23 +68,18 @@
 #include <algorithm>
 
 #include "prefill_runs.hpp"
-#include "tq_common.hpp"
+#include "prefill_stage.hpp"
 
 namespace {
 
 using namespace tq;
 
-typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 
 constexpr int NJ = 2;                    // row tiles (of 16) per wave
 constexpr int kMaxPrefillKeys = 65536;   // keys [0, kend) the dense path serves
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.0f;            // log2 headroom before the running max moves
-constexpr float kLazyH = 4.0f, kShift = 11.0f;   // fp16 P: the headroom, and log2 of what P is multiplied by
 constexpr int kCounterStrideP = 64;      // ints: one 256-byte line per counter
 constexpr int kCoherentP = 16;           // cache policy sc1: agent-coherent access
 
@@ -103,9 +98,7 @@ struct TileImg {
     static constexpr int ROUNDS = CHUNKS / kThreads;           // whole rounds of 16-byte copies
     static constexpr int REM = CHUNKS % kThreads;              // copies of the last, partial round
     static_assert(BYTES % 16 == 0 && KD_OFF % 16 == 0 && VH_OFF % 16 == 0, "16-byte chunks");
-    static constexpr int VE_OFF = KD_OFF + 1008;               // fp16 images: the tile's V' unit, whether it is wild
-    static constexpr int VK_OFF = KD_OFF + 768;                //   and then each key's unit, in operand order [4][8]
-    static_assert(2 * NB * 16 * 4 <= 768, "K scales and units fit their 1 KB");
+    static_assert(2 * NB * 16 * 4 <= 1024, "K scales fit their 1 KB");
     static_assert(REM % 64 == 0, "the partial round is whole waves");
 };
 
@@ -113,10 +106,6 @@ struct TileImg {
 // keys 4g..4g+3 then 16+4g..16+4g+3 (the rows a lane holds of S^T).
 __device__ __forceinline__ int perm_key(int g, int i) { return i < 4 ? 4 * g + i : 12 + 4 * g + i; }
 
-__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
-    v2bf v = {(__bf16)a, (__bf16)b};
-    return __builtin_bit_cast(uint32_t, v);
-}
 // bf16 hi | lo parts of four pairs of values.
 __device__ __forceinline__ void split_bf16(const float (&x)[8], u32x4 &hi, u32x4 &lo) {
 #pragma unroll
@@ -127,26 +116,6 @@ __device__ __forceinline__ void split_bf16(const float (&x)[8], u32x4 &hi, u32x4
     }
 }
 
-// fp16 hi | lo parts of four pairs of values: x to 2^-22.
-__device__ __forceinline__ uint32_t f16_pair(float a, float b) {
-    v2h v = {(_Float16)a, (_Float16)b};
-    return __builtin_bit_cast(uint32_t, v);
-}
-__device__ __forceinline__ void split_f16(const float (&x)[8], u32x4 &hi, u32x4 &lo) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        uint32_t h = f16_pair(x[2 * i], x[2 * i + 1]);
-        // lo is taken from the stored bits: left to see through them, the compiler
-        // rounds x's own product straight to fp16 for one of the two and by way of
-        // fp32 for the other, which differ now and then
-        asm("" : "+v"(h));
-        const v2h hv = __builtin_bit_cast(v2h, h);
-        hi[i] = h;
-        lo[i] = f16_pair(x[2 * i] - (float)hv[0], x[2 * i + 1] - (float)hv[1]);
-    }
-}
-
-__device__ __forceinline__ v8h as_v8h(u32x4 w) { return __builtin_bit_cast(v8h, w); }
 __device__ __forceinline__ v8bf as_v8bf(u32x4 w) { return __builtin_bit_cast(v8bf, w); }
 
 // Max / sum over lanes l, l^16, l^32, l^48 (the four 16-lane rows), the same
@@ -165,98 +134,17 @@ __device__ __forceinline__ float xrow_sum(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-typedef __attribute__((address_space(3))) unsigned char lds_u8;
-
-// 16 bytes from each lane's global address into LDS at dst + 16*lane
-// (global_load_lds_dwordx4, M0 = LDS byte address, restored after; a scalar
-// write of M0 needs one wait state before the copy, the s_nop).  Inline
-// assembly keeps the compiler from following the copy with a full vmcnt(0)
-// wait before every LDS access; the kernel waits for its copies itself.
-__device__ __forceinline__ void dma16(const void *src, unsigned char *dst) {
-    const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8 *)dst;
-    uint32_t saved;
-    asm volatile(
-        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\t"
-        "global_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-        : "=&s"(saved)
-        : "v"(src), "s"(lds));
-}
-
-// Wait until at most N vector memory operations of this wave are outstanding
-// (the copies above are counted in issue order).
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-    static_assert(N >= 0 && N < 64, "vmcnt immediate");
-    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
-}
-
-struct StageArgs {
-    PagedView view;
-    int seq;
-    int kend;            // keys [0, kend)
-    int n_tiles;         // tiles per kv head in the image buffer
-    unsigned char *img;  // [n_kv][n_tiles][TileImg::BYTES]
-    int contig_first;
-    int contig_pages;
-    // the q blocks: tokens [pos0, pos0 + n), blocks of QB queries
-    int pos0;
-    int n;
-    int qblocks;
-    int n_q_heads;
-    const float *q;      // [n][n_q_heads][hd], pre-RoPE if cos_t
-    const float *cos_t;  // [n][hd/2] or null
-    const float *sin_t;
-    unsigned char *qimg; // [n_kv][qblocks][PShape::Q_BYTES]
-    // the new K, V rows [n][n_kv][hd] (K pre-RoPE if cos_t), appended here;
-    // null: rows [pos0, pos0 + n) are already in the cache
-    const float *k_new;
-    const float *v_new;
-    // RMSNorm weights of q and of the new K rows (applied before RoPE), or null
-    const float *q_norm;
-    const float *k_norm;
-    float rms_eps;
-};
-
-// 1 / rms of an hd-value row, as model/rmsnorm.c:4-12 computes it: the
-// squares summed serially in element order, then a correctly rounded sqrt and
-// divide; eight 16-byte loads in flight at a time.
-template <int HD>
-__device__ __forceinline__ float row_inv_rms(const float *row, float eps) {
-#pragma clang fp contract(off)
-    float sum = 0.0f;
-    for (int i0 = 0; i0 < HD; i0 += 32) {
-        v4f v[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = *reinterpret_cast<const v4f *>(row + i0 + 4 * j);
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            sum += v[j].x * v[j].x;
-            sum += v[j].y * v[j].y;
-            sum += v[j].z * v[j].z;
-            sum += v[j].w * v[j].w;
-        }
-    }
-    return 1.0f / sqrtf(eps + sum / (float)HD);
-}
-
-// (x * inv) * w, rounded as model/rmsnorm.c:14-18 does, on four values.
-__device__ __forceinline__ v4f norm4(v4f x, float inv, v4f w) {
-#pragma clang fp contract(off)
-    return v4f{x.x * inv * w.x, x.y * inv * w.y, x.z * inv * w.z, x.w * inv * w.w};
-}
-
 template <int HD, int G>
 struct PShape {
     using I = TileImg<HD>;
     static constexpr int NB = I::NB;
     static constexpr int RW = 64 * NJ;             // (query, head) rows per work-group
-    static constexpr int QT = RW / 16 / G;         // query tiles per head
-    static constexpr int QB = 16 * QT;             // query tokens per work-group
-    static constexpr int TILES = G * QT;           // row tiles in use (groups of 3, 5, 6, 7 leave some idle)
+    static constexpr int QB = RW / G;              // query tokens per work-group
+    static constexpr int QT = QB / 16;             // query tiles per head
     static constexpr int MT = I::MT;               // output column tiles
     static constexpr int QCS = HD + 8;             // LDS stride of a q code row
     static constexpr int Q_BYTES = RW * QCS + RW * NB * 4;   // staged q: codes | scales
-    static_assert(QT >= 1, "a query tile per head");
+    static_assert(RW % G == 0 && QB % 16 == 0, "whole query tiles");
     static_assert(Q_BYTES <= I::BYTES, "q staging fits one tile buffer");
 };
 
@@ -290,7 +178,7 @@ __device__ __forceinline__ void stage_q(const StageArgs &a, int kvh, int blk) {
             const int nt = r >> 4;
             const int qi = i0 + (nt % S::QT) * 16 + (r & 15);
             xl[t] = xu[t] = cs[t] = sn[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            if (qi < a.n && nt < S::TILES) {
+            if (qi < a.n) {
                 const float *head = a.q + ((size_t)qi * a.n_q_heads + (size_t)kvh * G + nt / S::QT) * HD;
                 xl[t] = *reinterpret_cast<const v4f *>(head + 4 * c);
                 xu[t] = *reinterpret_cast<const v4f *>(head + HALF + 4 * c);
@@ -315,7 +203,7 @@ __device__ __forceinline__ void stage_q(const StageArgs &a, int kvh, int blk) {
         if (tid < S::RW) {
             const int r = tid, nt = r >> 4;
             const int qi = i0 + (nt % S::QT) * 16 + (r & 15);
-            inv_s[r] = qi < a.n && nt < S::TILES ? row_inv_rms<HD>(a.q + ((size_t)qi * a.n_q_heads + (size_t)kvh * G + nt / S::QT) * HD,
+            inv_s[r] = qi < a.n ? row_inv_rms<HD>(a.q + ((size_t)qi * a.n_q_heads + (size_t)kvh * G + nt / S::QT) * HD,
                                                   a.rms_eps)
                                 : 0.0f;
         }
@@ -355,153 +243,21 @@ __device__ __forceinline__ void stage_q(const StageArgs &a, int kvh, int blk) {
     }
 }
 
-// Key tile kt of kv head kvh: the new rows appended, the tile's image written,
-// V' in bf16 or (F16) in fp16.
-//
-// fp16 keeps 22 bits of V' in the two parts where bf16 keeps 16, but not its
-// range.  A tile's V' are stored in units of the power of two just above its
-// largest scale.  A wild tile, one with a key whose scales are all below 2^-9 of
-// that or with one that is no number, has a unit for each key instead, which
-// goes to P: what a causal mask hides of such a tile then neither costs the
-// rows before it their bits nor, as 0 times infinity, makes them NaN.
-template <int HD, bool F16>
-__device__ __forceinline__ void stage_tile(const StageArgs &a, const int kt, const int kvh) {
+// Grid (n_tiles + qblocks, n_kv): x < n_tiles stages key tile x, the rest
+// stage q block x - n_tiles.
+template <int HD, int G>
+__global__ __launch_bounds__(kThreads) void prefill_stage_kernel(StageArgs a) {
+    if ((int)blockIdx.x >= a.n_tiles) {
+        stage_q<HD, G>(a, blockIdx.y, (int)blockIdx.x - a.n_tiles);
+        return;
+    }
     using I = TileImg<HD>;
     constexpr int ROW = I::ROW;
-    constexpr int RDW = kKT * ROW / 4;   // dwords of one tile's K (or V) rows
-    __shared__ __align__(16) uint32_t raw[2][RDW];
-    __shared__ int page[2];
+    __shared__ __align__(16) uint32_t raw[2][kKT * ROW / 4];   // the tile's K | V rows
     const int tid = threadIdx.x;
-    const PagedView &v = a.view;
-    if (tid < 2) {
-        const int lp = 2 * kt + tid;
-        int p = -1;
-        if (lp * kPage < a.kend) {
-            if (a.contig_first >= 0 && lp < a.contig_pages)
-                p = a.contig_first + lp;
-            else
-                p = phys_page(v, a.seq, lp);
-        }
-        page[tid] = p;
-    }
-    __syncthreads();
-    // Rows of the tile: a new row (position in [pos0, kend) on a mapped page,
-    // with k_new given) is computed here and appended; an older one is read
-    // from the cache; every other row (past the keys, unmapped) is zero so that
-    // no stale scale reaches P.V.
-    const int t0 = kt * kKT;
-    auto fresh = [&](int p, int phys) { return a.k_new && p >= a.pos0 && p < a.kend && phys >= 0; };
-    // a page's K (or V) rows are one contiguous run: copy them in CB-byte
-    // pieces, whole rows per piece
-    constexpr int CB = ROW % 16 == 0 ? 16 : 8;
-    constexpr int PR = kPage * ROW / CB;   // pieces per page run
-    typedef uint32_t piece_t __attribute__((ext_vector_type(CB / 4)));
-    for (int i = tid; i < 2 * 2 * PR; i += kThreads) {
-        const int kv = i / (2 * PR), pg = (i / PR) & 1, ch = i % PR;
-        const int p = t0 + pg * kPage + (ch * CB) / ROW;
-        const int phys = page[pg];
-        if (fresh(p, phys)) continue;
-        piece_t x = piece_t(0u);
-        if (p < a.kend && phys >= 0)
-            x = *reinterpret_cast<const piece_t *>(head_run_ptr(v, phys, kvh) + kv * v.kv_chunk + ch * CB);
-        *reinterpret_cast<piece_t *>(reinterpret_cast<unsigned char *>(raw[kv]) + pg * kPage * ROW + ch * CB) = x;
-    }
-    // the new rows: store_kv's Q8 branch (model/attention_layer.c:66-90) with
-    // RoPE on K (:188), quantized exactly as quantize_row_q8 into the tile's
-    // LDS rows.  Task (row r, K|V, c) covers x[4c..4c+3] and its rotate-half
-    // partner x[HD/2+4c..+3]; the 8 lanes of a 32-value block share their row,
-    // so a whole block is computed or skipped together.
-    const bool has_new = a.k_new && t0 + kKT > a.pos0 && t0 < a.kend;
-    // with k_norm: 1/rms of each new K row of the tile, one row per thread;
-    // the tasks' own loads below are issued first, so the two overlap
-    __shared__ float kinv_s[kKT];
-    if (has_new) {
-        constexpr int HALF = HD / 2;
-        constexpr int CPR = HD / 8;
-        constexpr int TPT = kKT * 2 * CPR / kThreads;
-        static_assert(kKT * 2 * CPR % kThreads == 0 && CPR % 8 == 0, "whole tasks, whole blocks");
-        const bool rot = a.cos_t != nullptr;
-        v4f xl[TPT], xu[TPT], cs[TPT], sn[TPT];
-        bool mine[TPT];
-#pragma unroll
-        for (int t = 0; t < TPT; t++) {
-            const int task = tid + kThreads * t;
-            const int r = task / (2 * CPR), kv = (task / CPR) & 1, c = task % CPR;
-            const int p = t0 + r;
-            mine[t] = fresh(p, page[r / kPage]);
-            xl[t] = xu[t] = cs[t] = sn[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            if (mine[t]) {
-                const size_t row = (size_t)(p - a.pos0);
-                const float *src = (kv ? a.v_new : a.k_new) + (row * v.n_kv_heads + kvh) * HD;
-                xl[t] = *reinterpret_cast<const v4f *>(src + 4 * c);
-                xu[t] = *reinterpret_cast<const v4f *>(src + HALF + 4 * c);
-                if (!kv && rot) {
-                    cs[t] = *reinterpret_cast<const v4f *>(a.cos_t + row * HALF + 4 * c);
-                    sn[t] = *reinterpret_cast<const v4f *>(a.sin_t + row * HALF + 4 * c);
-                }
-            }
-        }
-        if (a.k_norm) {
-            // every task of a thread has the same columns: its weights once
-            const int cw = tid % CPR;
-            const v4f wlo = *reinterpret_cast<const v4f *>(a.k_norm + 4 * cw);
-            const v4f whi = *reinterpret_cast<const v4f *>(a.k_norm + HALF + 4 * cw);
-            if (tid < kKT) {
-                const int p = t0 + tid;
-                kinv_s[tid] = fresh(p, page[tid / kPage])
-                                  ? row_inv_rms<HD>(a.k_new + ((size_t)(p - a.pos0) * v.n_kv_heads + kvh) * HD,
-                                                    a.rms_eps)
-                                  : 0.0f;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int t = 0; t < TPT; t++) {
-                const int task = tid + kThreads * t;
-                const int r = task / (2 * CPR), kv = (task / CPR) & 1;
-                if (mine[t] && !kv) {
-                    xl[t] = norm4(xl[t], kinv_s[r], wlo);
-                    xu[t] = norm4(xu[t], kinv_s[r], whi);
-                }
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < TPT; t++) {
-            if (!mine[t]) continue;
-            const int task = tid + kThreads * t;
-            const int r = task / (2 * CPR), kv = (task / CPR) & 1, c = task % CPR;
-            float lo[4], up[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (!kv && rot) {
-                    lo[i] = rope_lower(xl[t][i], xu[t][i], cs[t][i], sn[t][i]);
-                    up[i] = rope_upper(xl[t][i], xu[t][i], cs[t][i], sn[t][i]);
-                } else {
-                    lo[i] = xl[t][i];
-                    up[i] = xu[t][i];
-                }
-            }
-            unsigned char *row = reinterpret_cast<unsigned char *>(raw[kv]) + r * ROW;
-            const bool leader = (c & 7) == 0;
-            const int bl = (4 * c) / kQK, bu = (HALF + 4 * c) / kQK;
-            quantize8x4(lo, reinterpret_cast<float *>(row + bl * kBlockBytes),
-                        row + bl * kBlockBytes + 4 + (4 * c) % kQK, leader);
-            quantize8x4(up, reinterpret_cast<float *>(row + bu * kBlockBytes),
-                        row + bu * kBlockBytes + 4 + (4 * c) % kQK, leader);
-        }
-    }
-    __syncthreads();
-    if (has_new) {
-        // the new rows into the cache, whole rows
-        for (int i = tid; i < 2 * 2 * PR; i += kThreads) {
-            const int kv = i / (2 * PR), pg = (i / PR) & 1, ch = i % PR;
-            const int p = t0 + pg * kPage + (ch * CB) / ROW;
-            const int phys = page[pg];
-            if (!fresh(p, phys)) continue;
-            *reinterpret_cast<piece_t *>(head_run_ptr(v, phys, kvh) + kv * v.kv_chunk + ch * CB) =
-                *reinterpret_cast<const piece_t *>(reinterpret_cast<const unsigned char *>(raw[kv]) + pg * kPage * ROW +
-                                                   ch * CB);
-        }
-    }
+    const int kt = blockIdx.x;
+    const int kvh = blockIdx.y;
+    stage_rows<HD>(a, kt, kvh, raw);
     const unsigned char *rk = reinterpret_cast<const unsigned char *>(raw[0]);
     const unsigned char *rv = reinterpret_cast<const unsigned char *>(raw[1]);
     unsigned char *out = a.img + ((size_t)a.n_tiles * kvh + kt) * I::BYTES;
@@ -521,43 +277,6 @@ __device__ __forceinline__ void stage_tile(const StageArgs &a, const int kt, con
         *reinterpret_cast<float *>(out + I::KD_OFF + e * 4) =
             *reinterpret_cast<const float *>(rk + key * ROW + b * kBlockBytes);
     }
-    [[maybe_unused]] float per_unit = 1.0f;
-    [[maybe_unused]] bool wild = false;
-    __shared__ float per_key[F16 ? kKT : 1];
-    if constexpr (F16) {
-        auto exponent = [](float d) { return min(max((int)(__float_as_uint(d) >> 23) - 126, -126), 126); };
-        __shared__ float shared_per_unit;
-        __shared__ int shared_wild;
-        if (tid < 64) {
-            float d = 0.0f;
-            bool odd = false;
-            if (tid < kKT)
-                for (int b = 0; b < I::NB; b++) {
-                    const float x = fabsf(*reinterpret_cast<const float *>(rv + tid * ROW + b * kBlockBytes));
-                    odd |= !(x < INFINITY);
-                    d = fmaxf(d, x);
-                }
-            const int e = exponent(wave_max(odd ? 0.0f : d));
-            const float unit = ldexpf(1.0f, e);
-            const bool any = __builtin_amdgcn_ballot_w64(odd || (d > 0.0f && d < unit * 0x1p-9f)) != 0;
-            if (tid < kKT) {
-                const int ek = exponent(d);
-                // operand order: perm_key's slot of this key
-                const int g = (tid & 15) >> 2, i = (tid >> 4) * 4 + (tid & 3);
-                *reinterpret_cast<float *>(out + I::VK_OFF + (g * 8 + i) * 4) = odd ? INFINITY : ldexpf(1.0f, ek);
-                per_key[tid] = odd ? 0.0f : ldexpf(1.0f, -ek);
-            }
-            if (tid == 0) {
-                shared_per_unit = ldexpf(1.0f, -e);
-                shared_wild = any;
-                *reinterpret_cast<float *>(out + I::VE_OFF) = unit;
-                *reinterpret_cast<int *>(out + I::VE_OFF + 4) = any;
-            }
-        }
-        __syncthreads();
-        per_unit = shared_per_unit;
-        wild = shared_wild;
-    }
     // V' = code * vd: entry (m, lane) = column m*16 + lane%16, keys perm_key(lane/16, 0..7)
     for (int e = tid; e < I::MT * 64; e += kThreads) {
         const int m = e / 64, ln = e % 64;
@@ -567,33 +286,13 @@ __device__ __forceinline__ void stage_tile(const StageArgs &a, const int kt, con
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const unsigned char *row = rv + perm_key(ln >> 4, i) * ROW + blk * kBlockBytes;
-            float d = *reinterpret_cast<const float *>(row);
-            if constexpr (F16) {
-                if (wild)
-                    d = fabsf(d) < INFINITY ? d * per_key[perm_key(ln >> 4, i)] : 1.0f;
-                else
-                    d *= per_unit;
-            }
-            x[i] = (float)(int8_t)row[4 + cb] * d;
+            x[i] = (float)(int8_t)row[4 + cb] * *reinterpret_cast<const float *>(row);
         }
         u32x4 hi, lo;
-        if constexpr (F16)
-            split_f16(x, hi, lo);
-        else
-            split_bf16(x, hi, lo);
+        split_bf16(x, hi, lo);
         *reinterpret_cast<u32x4 *>(out + I::VH_OFF + e * 16) = hi;
         *reinterpret_cast<u32x4 *>(out + I::VL_OFF + e * 16) = lo;
     }
-}
-
-// Grid (n_tiles + qblocks, n_kv): x < n_tiles stages key tile x, the rest
-// stage q block x - n_tiles.
-template <int HD, int G>
-__global__ __launch_bounds__(kThreads) void prefill_stage_kernel(StageArgs a) {
-    if ((int)blockIdx.x >= a.n_tiles)
-        stage_q<HD, G>(a, blockIdx.y, (int)blockIdx.x - a.n_tiles);
-    else
-        stage_tile<HD, false>(a, blockIdx.x, blockIdx.y);
 }
 
 
@@ -627,7 +326,6 @@ struct PRows {
     static constexpr int MT = PShape<HD, G>::MT;
     v4f o[MT][NJ];
     float mrow[NJ], moff[NJ], thr[NJ], lsum[NJ];
-    float unit[NJ], per_unit[NJ];   // F16: the unit of V' that o is kept in, and its inverse (0 before any key)
     __device__ __forceinline__ void init() {
 #pragma unroll
         for (int m = 0; m < MT; m++)
@@ -639,7 +337,6 @@ struct PRows {
             moff[j] = 0.0f;
             thr[j] = -INFINITY;
             lsum[j] = 0.0f;
-            unit[j] = per_unit[j] = 0.0f;
         }
     }
 };
@@ -688,74 +385,15 @@ struct PP {
     u32x4 hi[NJ], lo[NJ];
 };
 
-// P of one tile from its keys' weights: each row takes them in the largest unit
-// of V' among the keys it has seen (a row that sees none of a tile's keys does
-// not take its unit, so o keeps its bits whatever the mask hides), o rescaled
-// where that grows.  A wild tile brings a unit for each key.
-template <int HD, int G>
-__device__ __forceinline__ void into_units(const unsigned char *T, int lg, PRows<HD, G> &st, float (&p)[NJ][8]) {
-    using I = TileImg<HD>;
-    const uint2 head = *reinterpret_cast<const uint2 *>(T + I::VE_OFF);
-    const float unit = __uint_as_float(__builtin_amdgcn_readfirstlane(head.x));
-    const bool wild = __builtin_amdgcn_readfirstlane(head.y) != 0;
-    const float *vk = reinterpret_cast<const float *>(T + I::VK_OFF) + 8 * lg;
-    bool grow = wild;
-#pragma unroll
-    for (int j = 0; j < NJ; j++) grow |= unit > st.unit[j];
-    if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-#pragma unroll
-        for (int j = 0; j < NJ; j++) {
-            float top = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float u = wild ? vk[i] : unit;
-                top = p[j][i] > 0.0f && u < INFINITY ? fmaxf(top, u) : top;
-            }
-            const float now = fmaxf(st.unit[j], xrow_max(top));
-            const float c = now > 0.0f ? st.unit[j] / now : 1.0f;
-#pragma unroll
-            for (int m = 0; m < PShape<HD, G>::MT; m++) st.o[m][j] *= c;
-            st.unit[j] = now;
-            st.per_unit[j] = now > 0.0f ? 1.0f / now : 0.0f;
-        }
-    }
-    if (wild) {
-#pragma unroll
-        for (int j = 0; j < NJ; j++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) p[j][i] = p[j][i] == 0.0f ? 0.0f : p[j][i] * (vk[i] * st.per_unit[j]);
-    } else {
-        bool other = false;
-        float f[NJ];
-#pragma unroll
-        for (int j = 0; j < NJ; j++) {
-            f[j] = unit * st.per_unit[j];
-            other |= f[j] != 1.0f;
-        }
-        if (__builtin_amdgcn_ballot_w64(other) != 0) {
-            // a row that sees nothing of the tile has P = 0 and maybe no unit
-#pragma unroll
-            for (int j = 0; j < NJ; j++)
-#pragma unroll
-                for (int i = 0; i < 8; i++) p[j][i] = p[j][i] == 0.0f ? 0.0f : p[j][i] * f[j];
-        }
-    }
-}
-
 // One key tile kt (image T in LDS) against the wave's rows, first part:
 // exact scores, the causal mask, the online softmax (o and lsum rescaled when
 // the max moves) and this tile's P.
-//
-// F16: P and V' are split into fp16 parts.  P is taken 2^kShift times as large
-// (o and lsum alike), at most 2^15, so that the parts of all but negligible
-// weights are normal numbers, and in the tile's units over the row's (into_units).
-template <int HD, int G, bool F16>
+template <int HD, int G>
 __device__ __forceinline__ void tile_scores(const PrefillArgs &a, const unsigned char *T, int kt, int i0, int lane,
                                             const PQ<HD, G> &q, PRows<HD, G> &st, PP &pp) {
     using S = PShape<HD, G>;
     using I = TileImg<HD>;
     constexpr int NB = S::NB;
-    constexpr float kHead = F16 ? kLazyH : kLazy, kUp = F16 ? kShift : 0.0f;
     const int lg = lane >> 4;
     // S^T - moff for keys [32kt, 32kt+32) x the wave's queries: per block the
     // exact int32 dot on the matrix cores, then (kd * qd') * dot added in
@@ -809,8 +447,8 @@ __device__ __forceinline__ void tile_scores(const PrefillArgs &a, const unsigned
 #pragma unroll
         for (int j = 0; j < NJ; j++) {
             const float mx = xrow_max(max8(s[0][j], s[1][j])) + st.moff[j];
-            const float mnew = mx > st.mrow[j] + kHead ? mx : st.mrow[j];
-            const float onew = mnew == -INFINITY ? 0.0f : mnew - kUp;
+            const float mnew = mx > st.mrow[j] + kLazy ? mx : st.mrow[j];
+            const float onew = mnew == -INFINITY ? 0.0f : mnew;
             // nothing is accumulated while mrow is -inf: corr 0, not exp2 of a difference
             corr[j] = st.mrow[j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.moff[j] - onew);
             const float delta = st.moff[j] - onew;
@@ -822,7 +460,7 @@ __device__ __forceinline__ void tile_scores(const PrefillArgs &a, const unsigned
             st.lsum[j] *= corr[j];
             st.mrow[j] = mnew;
             st.moff[j] = onew;
-            st.thr[j] = mnew == -INFINITY ? -INFINITY : kHead + kUp;
+            st.thr[j] = mnew == -INFINITY ? -INFINITY : kLazy;
         }
         if (__builtin_amdgcn_ballot_w64(rescale) != 0) {
 #pragma unroll
@@ -831,61 +469,48 @@ __device__ __forceinline__ void tile_scores(const PrefillArgs &a, const unsigned
                 for (int j = 0; j < NJ; j++) st.o[m][j] *= corr[j];
         }
     }
-    // P = exp2(S - moff) <= 2^kLazy (F16: 2^(kLazyH + kShift)), split into hi | lo (B operands)
-    float p[NJ][8];
+    // P = exp2(S - moff) <= 2^kLazy, split into bf16 hi | lo (B operands)
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
+        float p[8];
         float ps = 0.0f;
 #pragma unroll
         for (int mt = 0; mt < 2; mt++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                p[j][mt * 4 + r] = __builtin_amdgcn_exp2f(s[mt][j][r]);
-                ps += p[j][mt * 4 + r];
+                p[mt * 4 + r] = __builtin_amdgcn_exp2f(s[mt][j][r]);
+                ps += p[mt * 4 + r];
             }
         st.lsum[j] += ps;
-    }
-    if constexpr (F16) into_units<HD, G>(T, lg, st, p);
-#pragma unroll
-    for (int j = 0; j < NJ; j++) {
-        if constexpr (F16)
-            split_f16(p[j], pp.hi[j], pp.lo[j]);
-        else
-            split_bf16(p[j], pp.hi[j], pp.lo[j]);
+        split_bf16(p, pp.hi[j], pp.lo[j]);
     }
 }
 
 // Second part: O^T += V'^T . P^T with the tile's V' (image T) and its P.
-template <int HD, int G, bool F16>
+template <int HD, int G>
 __device__ __forceinline__ void tile_pv(const unsigned char *T, int lane, const PP &pp, PRows<HD, G> &st) {
     using S = PShape<HD, G>;
     using I = TileImg<HD>;
 #pragma unroll
     for (int m = 0; m < S::MT; m++) {
-        const u32x4 vhi = *reinterpret_cast<const u32x4 *>(T + I::VH_OFF + (m * 64 + lane) * 16);
-        const u32x4 vlo = *reinterpret_cast<const u32x4 *>(T + I::VL_OFF + (m * 64 + lane) * 16);
-        auto mul = [](u32x4 v, u32x4 p, v4f o) {
-            if constexpr (F16)
-                return __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(v), as_v8h(p), o, 0, 0, 0);
-            else
-                return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_v8bf(v), as_v8bf(p), o, 0, 0, 0);
-        };
+        const v8bf ahi = as_v8bf(*reinterpret_cast<const u32x4 *>(T + I::VH_OFF + (m * 64 + lane) * 16));
+        const v8bf alo = as_v8bf(*reinterpret_cast<const u32x4 *>(T + I::VL_OFF + (m * 64 + lane) * 16));
 #pragma unroll
         for (int j = 0; j < NJ; j++) {
-            st.o[m][j] = mul(vhi, pp.hi[j], st.o[m][j]);
-            st.o[m][j] = mul(vhi, pp.lo[j], st.o[m][j]);
-            st.o[m][j] = mul(vlo, pp.hi[j], st.o[m][j]);
+            st.o[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ahi, as_v8bf(pp.hi[j]), st.o[m][j], 0, 0, 0);
+            st.o[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ahi, as_v8bf(pp.lo[j]), st.o[m][j], 0, 0, 0);
+            st.o[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(alo, as_v8bf(pp.hi[j]), st.o[m][j], 0, 0, 0);
         }
     }
 }
 
 // Both parts of one tile.
-template <int HD, int G, bool F16>
+template <int HD, int G>
 __device__ __forceinline__ void tile_update(const PrefillArgs &a, const unsigned char *T, int kt, int i0, int lane,
                                             const PQ<HD, G> &q, PRows<HD, G> &st) {
     PP pp;
-    tile_scores<HD, G, F16>(a, T, kt, i0, lane, q, st, pp);
-    tile_pv<HD, G, F16>(T, lane, pp, st);
+    tile_scores<HD, G>(a, T, kt, i0, lane, q, st, pp);
+    tile_pv<HD, G>(T, lane, pp, st);
 }
 
 // Normalise and store row tile nt (16 rows): lane holds columns
@@ -898,7 +523,6 @@ __device__ __forceinline__ void store_rows(const PrefillArgs &a, int kvh, int i0
     const int l16 = lane & 15, lg = lane >> 4;
     const float inv = 1.0f / lrow;
     const int g = nt / S::QT;
-    if (S::TILES < S::RW / 16 && nt >= S::TILES) return;   // an idle row tile (wave-uniform)
     const int qi = i0 + (nt % S::QT) * 16 + l16;
     if (a.out_xs) {
         // block b of a head is columns 32b..32b+31, tiles m = 2b (codes 0-15)
@@ -991,12 +615,8 @@ __device__ __forceinline__ bool tile_has_rem(int gwave) {
 // agent-coherent stores, waits for them, then arrives on the block's counter;
 // the last to arrive merges all of them in run order (its own from registers)
 // and puts the counter back to 0.  Nothing waits on another work-group.
-//
-// pblock: the first of the block's partials in units of one ([RW][HD + 4]);
-// counter: the block's.
-template <int HD, int G, bool F16>
-__device__ __forceinline__ void run_block(const PrefillArgs &a, const int kvh, const BlockRun at_run,
-                                          const size_t pblock, int *counter) {
+template <int HD, int G>
+__global__ __launch_bounds__(2 * kThreads, 1) void prefill_block_kernel(PrefillArgs a) {
     using S = PShape<HD, G>;
     using I = TileImg<HD>;
     constexpr int MT = S::MT;
@@ -1004,6 +624,8 @@ __device__ __forceinline__ void run_block(const PrefillArgs &a, const int kvh, c
     // tile buffers: half 0 uses 0, 1; half 1 uses 2, 3
     __shared__ __attribute__((aligned(16))) unsigned char tiles[4][I::BYTES];
     static_assert(2 * 4 * 64 * (MT * 16 + 8) <= 4 * I::BYTES, "the halves' row tiles fit the tile buffers");
+    const int kvh = (int)blockIdx.x % a.n_kv;
+    const BlockRun at_run = plan_item(a.pos0, a.n, S::QB, a.qblocks, a.whole, a.chunk, (int)blockIdx.x / a.n_kv);
     const int blk = at_run.blk, sp = at_run.run, segs = at_run.runs;
     const int all = block_tiles(a.pos0, a.n, S::QB, blk);
     // runs of whole tile pairs, as even as they go
@@ -1060,18 +682,12 @@ __device__ __forceinline__ void run_block(const PrefillArgs &a, const int kvh, c
         asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
         __syncthreads();
         if (s + 1 < mine) fetch_tile<HD>(img, 2 * (s + 1) + half, buf(s + 1), htid, wave);
-        if (s < mine) tile_update<HD, G, F16>(a, buf(s), kt0 + 2 * s + half, i0, lane, q, st);
+        if (s < mine) tile_update<HD, G>(a, buf(s), kt0 + 2 * s + half, i0, lane, q, st);
     }
 
     float lrow[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; j++) lrow[j] = xrow_sum(st.lsum[j]);
-    if constexpr (F16) {
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int j = 0; j < NJ; j++) st.o[m][j] *= st.unit[j];
-    }
     // row tile j of both halves is finished by half j; the other half leaves it
     // in the free tile buffers lane by lane (the waves of both halves hold the
     // same rows and columns in the same lanes)
@@ -1113,8 +729,10 @@ __device__ __forceinline__ void run_block(const PrefillArgs &a, const int kvh, c
 
     const int l16 = lane & 15, lg = lane >> 4;
     constexpr int PS = HD + 4;
+    const size_t pblock = ((size_t)kvh * a.qblocks + blk) * a.nsp;
     const __amdgpu_buffer_rsrc_t prs =
         __builtin_amdgcn_make_buffer_rsrc(a.partials + pblock * S::RW * PS, 0, segs * S::RW * PS * 4, 0x00020000);
+    int *counter = a.counters + ((size_t)kvh * a.qblocks + blk) * kCounterStrideP;
     const int r = tile * 16 + l16;
     const int base = (sp * S::RW + r) * PS;
 #pragma unroll
@@ -1164,108 +782,8 @@ __device__ __forceinline__ void run_block(const PrefillArgs &a, const int kvh, c
     store_rows<HD, G>(a, kvh, i0, tile, lane, acc2, L2);
 }
 
-template <int HD, int G>
-__global__ __launch_bounds__(2 * kThreads, 1) void prefill_block_kernel(PrefillArgs a) {
-    const int kvh = (int)blockIdx.x % a.n_kv;
-    const BlockRun run =
-        plan_item(a.pos0, a.n, PShape<HD, G>::QB, a.qblocks, a.whole, a.chunk, (int)blockIdx.x / a.n_kv);
-    const size_t at = (size_t)kvh * a.qblocks + run.blk;
-    run_block<HD, G, false>(a, kvh, run, at * a.nsp, a.counters + at * kCounterStrideP);
-}
-
-// ---- several sequences in one call ------------------------------------------
-//
-// The rows of up to kMaxPack sequences lie one behind the other in q, k, v, cos,
-// sin and out; each sequence has its own key tiles, query blocks and runs, as
-// many as if it were alone, numbered through in the order of the table (longest
-// first).  A work-group looks its sequence up (one entry per lane), makes the
-// arguments of that sequence's own call, and does that call's work, in fp16
-// parts.  The images of one sequence are read by work-groups next to each other
-// in the grid, so that an XCD's L2 holds the few that are in use.
-struct PackArgs {
-    TqPackTable t;
-    StageArgs st;        // of the whole call; per sequence: filled in by the kernels
-    int n_tiles;         // of all sequences
-    int n_blocks;
-    int n_runs;
-    float *partials;     // [n_kv][n_runs][RW][HD + 4]
-    int *counters;       // [n_kv][n_runs] x kCounterStrideP
-    float *out;
-    float scale;
-};
-
-// The sequence whose share of a numbering holds x: first[i] <= x < first[i + 1].
-__device__ __forceinline__ int pack_find(const int (&first)[TQ_MAX_PACK + 1], int n, int x) {
-    const int lane = threadIdx.x & 63;
-    const bool at = lane < n && first[lane] <= x;
-    return __builtin_amdgcn_readfirstlane(__popcll(__builtin_amdgcn_ballot_w64(at)) - 1);
-}
-
-// Grid (n_tiles + n_blocks, n_kv), as prefill_stage_kernel; also clears the
-// counters of the launch that follows.
-template <int HD, int G>
-__global__ __launch_bounds__(kThreads) void pack_stage_kernel(PackArgs a) {
-    const int x = blockIdx.x, kvh = blockIdx.y;
-    if (threadIdx.x == 0 && a.counters) {
-        const size_t wgs = (size_t)gridDim.x * gridDim.y, n = (size_t)a.n_runs * gridDim.y;
-        for (size_t c = (size_t)kvh * gridDim.x + x; c < n; c += wgs) a.counters[c * kCounterStrideP] = 0;
-    }
-    const bool keys = x < a.n_tiles;
-    const int i = keys ? pack_find(a.t.tile0, a.t.n_seqs, x) : pack_find(a.t.blk0, a.t.n_seqs, x - a.n_tiles);
-    StageArgs s = a.st;
-    const int row0 = a.t.start[i], half = HD / 2;
-    s.seq = a.t.seq[i];
-    s.pos0 = a.t.pos0[i];
-    s.n = a.t.n[i];
-    s.kend = s.pos0 + s.n;
-    s.contig_first = -1;
-    s.contig_pages = 0;
-    s.q += (size_t)row0 * s.n_q_heads * HD;
-    s.k_new += (size_t)row0 * s.view.n_kv_heads * HD;
-    s.v_new += (size_t)row0 * s.view.n_kv_heads * HD;
-    if (s.cos_t) {
-        s.cos_t += (size_t)row0 * half;
-        s.sin_t += (size_t)row0 * half;
-    }
-    s.img += (size_t)a.t.tile0[i] * TileImg<HD>::BYTES;
-    s.qimg += (size_t)a.t.blk0[i] * PShape<HD, G>::Q_BYTES;
-    if (keys)
-        stage_tile<HD, true>(s, x - a.t.tile0[i], kvh);
-    else
-        stage_q<HD, G>(s, kvh, x - a.n_tiles - a.t.blk0[i]);
-}
-
-// Grid: run r of all sequences' for kv head h is work-group r * n_kv + h.
-template <int HD, int G>
-__global__ __launch_bounds__(2 * kThreads, 1) void pack_block_kernel(PackArgs a) {
-    using S = PShape<HD, G>;
-    const int n_kv = a.st.view.n_kv_heads;
-    const int kvh = (int)blockIdx.x % n_kv, item = (int)blockIdx.x / n_kv;
-    const int i = pack_find(a.t.run0, a.t.n_seqs, item);
-    PrefillArgs p;
-    p.pos0 = a.t.pos0[i];
-    p.n = a.t.n[i];
-    p.qblocks = a.n_blocks;
-    p.whole = 0;
-    p.chunk = a.t.chunk;
-    p.nsp = 0;
-    p.n_kv = n_kv;
-    p.partials = a.partials;
-    p.counters = a.counters;
-    p.n_q_heads = a.st.n_q_heads;
-    p.scale = a.scale;
-    p.n_tiles = a.n_tiles;
-    p.img = a.st.img + (size_t)a.t.tile0[i] * TileImg<HD>::BYTES;
-    p.qimg = a.st.qimg + (size_t)a.t.blk0[i] * S::Q_BYTES;
-    p.out = a.out + (size_t)a.t.start[i] * p.n_q_heads * HD;
-    p.out_xs = nullptr;
-    const BlockRun run = block_of_run(p.pos0, p.n, S::QB, a.t.blk0[i + 1] - a.t.blk0[i], p.chunk, item - a.t.run0[i]);
-    const size_t at = (size_t)kvh * a.n_runs + item - run.run;
-    run_block<HD, G, true>(p, kvh, run, at, a.counters + at * kCounterStrideP);
-}
-
 // Query tokens per work-group for a group size (the kernel's QB).
-int prefill_qb(int g) { return 16 * (64 * NJ / 16 / g); }
+int prefill_qb(int g) { return 64 * NJ / g; }
 
 // TQ_HIP_PREFILL_WHOLE=1 keeps every block one run, =0 cuts every block into
 // as many runs as the plan may (tests of both at any size); read on every
@@ -1335,125 +853,7 @@ hipError_t launch_hd(const TqPrefillArgs &t, const PrefillArgs &a, int g, int it
     }
 }
 
-// Tiles and blocks of every sequence of a table, and the length of a run.
-//
-// chunk 0 leaves every block one run.  Where that leaves CUs idle, or one long
-// block at the end, blocks are cut; the cost of a choice is plan_runs' for many
-// work-groups: the CUs' share of all steps, a third of the longest work-group at
-// the end, and the merge.
-void plan_pack(TqPackTable &t, int qb, int n_kv, int *n_tiles, int *n_blocks, int *n_runs) {
-    int most = 1;
-    double tiles = 0.0;
-    t.tile0[0] = t.blk0[0] = t.run0[0] = 0;
-    for (int i = 0; i < t.n_seqs; i++) {
-        const int blocks = (t.n[i] + qb - 1) / qb, all = (t.pos0[i] + t.n[i] + kKT - 1) / kKT;
-        t.tile0[i + 1] = t.tile0[i] + all;
-        t.blk0[i + 1] = t.blk0[i] + blocks;
-        most = std::max(most, all);
-        // the blocks' tiles are an arithmetic sequence that ends with `all`
-        tiles += blocks * (all - 0.5 * (blocks - 1) * qb / kKT);
-    }
-    *n_tiles = t.tile0[t.n_seqs];
-    *n_blocks = t.blk0[t.n_seqs];
-    double best = 0.0;
-    t.chunk = 0;
-    for (int k = 1; k <= kMaxRuns && (k == 1 || (most + 1) / 2 >= k); k++) {
-        const int chunk = k == 1 ? 0 : (((most + k - 1) / k) + 1) & ~1;
-        double items = 0.0;
-        for (int i = 0; i < t.n_seqs; i++)
-            items += (double)total_runs(t.pos0[i], t.n[i], qb, t.blk0[i + 1] - t.blk0[i], chunk);
-        const double item = kItemCost + (k > 1 ? kRunCost : 0.0), one = 0.5 * (k == 1 ? most : chunk) + item;
-        const double share = n_kv * (0.5 * tiles + items * item) / kCUs;
-        const double cost = (items * n_kv <= kCUs ? one : std::max(one, share + 0.3 * one)) + (k > 1 ? kMergeCost * k : 0.0);
-        if (k == 1 || cost < best) {
-            best = cost;
-            t.chunk = chunk;
-        }
-    }
-    for (int i = 0; i < t.n_seqs; i++)
-        t.run0[i + 1] = t.run0[i] + (int)total_runs(t.pos0[i], t.n[i], qb, t.blk0[i + 1] - t.blk0[i], t.chunk);
-    *n_runs = t.run0[t.n_seqs];
-}
-
-// Offsets of a packed call's workspace: images, q blocks, partials, counters.
-struct PackSpace {
-    size_t qimg, partials, counters, bytes;
-};
-PackSpace pack_space(int hd, int n_kv, const TqPackTable &t, int n_tiles, int n_blocks, int n_runs) {
-    auto al = [](size_t x) { return (x + 255) & ~(size_t)255; };
-    const size_t tile = hd == 64 ? TileImg<64>::BYTES : TileImg<128>::BYTES;
-    const size_t block = hd == 64 ? PShape<64, 1>::Q_BYTES : PShape<128, 1>::Q_BYTES;
-    const size_t cut = t.chunk ? (size_t)n_kv * n_runs : 0;
-    PackSpace w;
-    w.qimg = al((size_t)n_kv * n_tiles * tile);
-    w.partials = w.qimg + al((size_t)n_kv * n_blocks * block);
-    w.counters = w.partials + al(cut * (64 * NJ) * (hd + 4) * sizeof(float));
-    w.bytes = w.counters + cut * kCounterStrideP * sizeof(int);
-    return w;
-}
-
-template <int HD, int G>
-hipError_t launch_pack(const PackArgs &a, hipStream_t s) {
-    const int n_kv = a.st.view.n_kv_heads;
-    hipLaunchKernelGGL((pack_stage_kernel<HD, G>), dim3(a.n_tiles + a.n_blocks, n_kv), dim3(kThreads), 0, s, a);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((pack_block_kernel<HD, G>), dim3(a.n_runs * n_kv), dim3(2 * kThreads), 0, s, a);
-    return hipGetLastError();
-}
-
-template <int HD>
-hipError_t launch_pack_g(const PackArgs &a, int g, hipStream_t s) {
-    switch (g) {
-        case 1: return launch_pack<HD, 1>(a, s);
-        case 2: return launch_pack<HD, 2>(a, s);
-        case 3: return launch_pack<HD, 3>(a, s);
-        case 4: return launch_pack<HD, 4>(a, s);
-        case 5: return launch_pack<HD, 5>(a, s);
-        case 6: return launch_pack<HD, 6>(a, s);
-        case 7: return launch_pack<HD, 7>(a, s);
-        case 8: return launch_pack<HD, 8>(a, s);
-        default: return hipErrorInvalidValue;
-    }
-}
-
 }  // namespace
-
-bool tq_pack_supported(int head_dim, int group) {
-    return (head_dim == 64 || head_dim == 128) && group >= 1 && group <= 8;
-}
-
-size_t tq_pack_bytes(int head_dim, int group, int n_kv_heads, TqPackTable &t) {
-    int tiles, blocks, runs;
-    plan_pack(t, prefill_qb(group), n_kv_heads, &tiles, &blocks, &runs);
-    return pack_space(head_dim, n_kv_heads, t, tiles, blocks, runs).bytes;
-}
-
-hipError_t tq_launch_pack(const TqPackArgs &p, hipStream_t s) {
-    const int g = p.n_q_heads / p.view.n_kv_heads;
-    if (!tq_pack_supported(p.head_dim, g) || p.table->n_seqs < 1 || p.table->n_seqs > TQ_MAX_PACK)
-        return hipErrorInvalidValue;
-    PackArgs a{};
-    a.t = *p.table;
-    plan_pack(a.t, prefill_qb(g), p.view.n_kv_heads, &a.n_tiles, &a.n_blocks, &a.n_runs);
-    const PackSpace w = pack_space(p.head_dim, p.view.n_kv_heads, a.t, a.n_tiles, a.n_blocks, a.n_runs);
-    a.st.view = p.view;
-    a.st.n_tiles = a.n_tiles;
-    a.st.img = p.ws;
-    a.st.qimg = p.ws + w.qimg;
-    a.st.qblocks = a.n_blocks;
-    a.st.n_q_heads = p.n_q_heads;
-    a.st.q = p.q;
-    a.st.cos_t = p.cos_t;
-    a.st.sin_t = p.sin_t;
-    a.st.k_new = p.k;
-    a.st.v_new = p.v;
-    a.partials = a.t.chunk ? reinterpret_cast<float *>(p.ws + w.partials) : nullptr;
-    a.counters = a.t.chunk ? reinterpret_cast<int *>(p.ws + w.counters) : nullptr;
-    a.out = p.out;
-    a.scale = p.scale;
-    return p.head_dim == 64 ? launch_pack_g<64>(a, g, s) : launch_pack_g<128>(a, g, s);
-}
 
 bool tq_prefill_mfma_supported(int head_dim, int group, int kend) {
     const bool hd_ok = head_dim == 64 || head_dim == 128;

@@ -406,7 +406,7 @@ struct TqEvictArgs {
 size_t tq_evict_list_ints(int max_len, int keep);
 hipError_t tq_launch_evict(const TqEvictArgs &a, hipStream_t s);
 
-// tq_hip_prefill_packed_async's dense form (prefill.hip): the sequences of one
+// tq_hip_prefill_packed_async's dense form (prefill_packed.hip): the sequences of one
 // launch, none of them empty, longest first.
 #define TQ_MAX_PACK 64
 struct TqPackTable {
@@ -416,9 +416,8 @@ struct TqPackTable {
     int pos0[TQ_MAX_PACK];
     int start[TQ_MAX_PACK];         // first row
     int n[TQ_MAX_PACK];             // rows
-    int tile0[TQ_MAX_PACK + 1];     // the plan's: first key tile, query block
-    int blk0[TQ_MAX_PACK + 1];      //   and run of each
-    int run0[TQ_MAX_PACK + 1];
+    int tile0[TQ_MAX_PACK + 1];     // the plan's: first key tile
+    int run0[TQ_MAX_PACK + 1];      //   and run of each
 };
 struct TqPackArgs {
     tq::PagedView view;
