@@ -251,7 +251,10 @@ __device__ __forceinline__ void split3_bf16(const float (&x)[8], v8bf &hi, v8bf 
 // partial of its split, and the combine is left to decode_weights_kernel, which
 // follows; W is split in three parts instead of two, so that out is as exact as
 // the weights beside it (2^-25 instead of 2^-18 per term; the third product
-// and its split take no time beside the stream: 64 sequences of 512-8,192).
+// and its split take no time beside the stream).  The scores' stores take 20 of
+// 150 us (64 sequences of 512-8,192 tokens, 36 MB of scores beside 560 of K and V):
+// bandwidth; nontemporal or coherent stores and waits that do not include them
+// changed nothing.
 template <int HD, int G, int W, bool SC>
 __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
     using L = L3<HD, G>;

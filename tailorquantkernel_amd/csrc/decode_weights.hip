@@ -13,6 +13,10 @@
 // Grid (token chunks and one more, kv head, query): the last x merges the
 // partials, the others take kChunkT tokens each.  Every work-group derives M
 // and L itself from the splits' (m, l), so nothing waits for another.
+//
+// Bound by those reads: 64 sequences of 512 .. 8,192 tokens (32 heads of 128 over
+// 8, 54 MB of scores and totals) 12 us, 16 of 16,384 (64 heads over 8) 17; with the
+// scores read after M and L instead of before, 16 and 20.
 #include "tq_common.hpp"
 
 namespace {
@@ -22,6 +26,7 @@ using namespace tq;
 typedef float v4f __attribute__((ext_vector_type(4)));
 
 constexpr int kChunkT = 1024;
+constexpr int kPer = kChunkT / kThreads;
 constexpr int kMaxSplitsW = 64;
 
 template <int G>
@@ -40,6 +45,22 @@ __global__ __launch_bounds__(kThreads) void decode_weights_kernel(TqWeightsArgs 
     const size_t pair = (size_t)qi * a.n_kv_heads + kvh;
     const int pstride = (G * (hd + 2) + 3) / 4 * 4;
     const float *part = a.partials + pair * a.n_splits * pstride;
+    const int seq = a.seq_of ? a.seq_of[qi] : qi;
+    const bool known = seq >= 0 && seq < a.max_seqs;
+    const size_t row = ((size_t)(known ? seq : 0) * a.n_kv_heads + kvh) * a.stride;
+    const float *sc = a.scores + pair * a.score_stride * G;
+    // this thread's scores and totals, in flight while M and L are derived (past
+    // the chunk's tokens: those of the last one)
+    float score[kPer][G], old[kPer];
+    if (!merge) {
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            const int t = min(t0 + j * kThreads + tid, len - 1);
+#pragma unroll
+            for (int h = 0; h < G; h++) score[j][h] = sc[(size_t)t * G + h];
+            old[j] = a.total[row + t];
+        }
+    }
     // M and 1 / L of a head, one wave per head, one lane per split
     for (int h = wave; h < G; h += kThreads / 64) {
         const bool ok = lane < nvalid;
@@ -65,16 +86,16 @@ __global__ __launch_bounds__(kThreads) void decode_weights_kernel(TqWeightsArgs 
         }
         return;
     }
-    const int seq = a.seq_of ? a.seq_of[qi] : qi;
-    if (seq < 0 || seq >= a.max_seqs) return;
-    const size_t row = ((size_t)seq * a.n_kv_heads + kvh) * a.stride;
-    const float *sc = a.scores + pair * a.score_stride * G;
-    for (int t = t0 + tid; t < min(len, t0 + kChunkT); t += kThreads) {
+    if (!known) return;
+#pragma unroll
+    for (int j = 0; j < kPer; j++) {
+        const int t = t0 + j * kThreads + tid;
+        if (t >= len) break;
         float w = 0.0f;
 #pragma unroll
-        for (int h = 0; h < G; h++) w += __builtin_amdgcn_exp2f(sc[(size_t)t * G + h] - ms[h]) * inv[h];
+        for (int h = 0; h < G; h++) w += __builtin_amdgcn_exp2f(score[j][h] - ms[h]) * inv[h];
         // a slot begins with the token that takes it
-        a.total[row + t] = t < pos ? a.total[row + t] + w : w;
+        a.total[row + t] = t < pos ? old[j] + w : w;
         if (t == pos && a.where) a.where[row + t] = a.at_of ? a.at_of[qi] : pos;
     }
 }
