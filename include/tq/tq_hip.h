@@ -227,7 +227,8 @@ int tq_hip_decode_step_norm_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq, 
  * slot t <= p, with the softmax weights w of the group's query heads:
  *   total[(s*n_kv_heads + h)*stride + t]  = (t < p ? its value : 0) + sum w[t]
  *   where[(s*n_kv_heads + h)*stride + p]  = d_at[i] (NULL: p)
- * so a slot's total begins with the token that takes it.  d_at is the token's
+ * so a slot's total begins with the token that takes it.  A sequence appears at
+ * most once per call.  d_at is the token's
  * position in its text, which after an eviction is past its slot; d_where may be
  * NULL.  Slots past p are not touched, nor anything for a negative d_pos[i].
  * Head dims 32/64/128 with groups 1..8, TQ_HIP_ETYPE otherwise; fp32 arrays
@@ -456,8 +457,8 @@ typedef struct {
 /* Device workspace of tq_hip_logits_process with a d_token, or 0 for a bad shape. */
 size_t tq_hip_logits_ws_bytes(int rows, int vocab);
 /* Row r of vocab logits at logits + r*stride through the rules (NULL: none) into
- * out + r*out_stride (in place where out == logits and the strides agree; NULL:
- * not written).  In this order, each step rounded to fp32: repetition, frequency
+ * out + r*out_stride (in place where out == logits: the strides must agree; NULL:
+ * not written; other arrays' rows must not overlap the logits').  In this order, each step rounded to fp32: repetition, frequency
  * times the count, presence, bias, and -inf for a token that the mask does not
  * allow.  d_token[r] (NULL: not wanted) is the first index of the row's largest
  * result, as sample_greedy (model/sampler.c:3-13) takes it, but -1 for a row

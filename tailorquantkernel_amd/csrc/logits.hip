@@ -263,6 +263,7 @@ int tq_hip_logits_process(const float *logits, size_t stride, int rows, int voca
     if (rows == 0) return TQ_HIP_OK;
     if (!logits || (!out && !d_token) || stride < (size_t)vocab || (out && out_stride < (size_t)vocab))
         return TQ_HIP_EINVAL;
+    if (out == logits && out_stride != stride && rows > 1) return TQ_HIP_EINVAL;   // rows over one another
     if (((uintptr_t)logits | (uintptr_t)out | (uintptr_t)d_token) & 3) return TQ_HIP_EINVAL;
     if (d_token && (!d_ws || ((uintptr_t)d_ws & 15) || ws_bytes < tq_hip_logits_ws_bytes(rows, vocab)))
         return TQ_HIP_EINVAL;

@@ -34,7 +34,7 @@ def rules(nat, **over):
 @pytest.mark.parametrize("over", [
     dict(rows=-1), dict(rows=65536), dict(vocab=0), dict(vocab=-5), dict(logits=None), dict(out=None, token=None),
     dict(stride=99), dict(out_stride=99), dict(logits=P + 2), dict(out=P + 1), dict(token=P + 3), dict(ws=None),
-    dict(ws=P + 8), dict(ws_bytes=15)])
+    dict(ws=P + 8), dict(ws_bytes=15), dict(out_stride=104), dict(stride=104)])
 def test_logits_arguments(nat, over):
     assert logits(nat, **over) == nat.EINVAL
 
