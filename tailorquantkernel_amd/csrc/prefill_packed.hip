@@ -593,8 +593,9 @@ __global__ __launch_bounds__(kThreads, 2) void pack_block_kernel(PackArgs a) {
     Row<HD> st;
     st.init();
 
-    // the wave's tiles, the rest is masked for all of its rows
-    const int mine = min(nt, last / kKT + 1 - kt0);
+    // the wave's tiles: the rest is masked for all of its rows, all of them for a
+    // wave without rows
+    const int mine = first > last ? 0 : min(nt, last / kKT + 1 - kt0);
     float s[16];
     if (nt > 0) {
         if (nt > 1) {
