@@ -247,13 +247,14 @@ __device__ __forceinline__ void split3_bf16(const float (&x)[8], v8bf &hi, v8bf 
 }
 
 // W waves per work-group (4, or 8 when each wave has only a tile or two).
-// SC (the step that gathers weights): every score goes to a.scores, always as a
-// partial of its split, and the combine is left to decode_weights_kernel, which
-// follows; W is split in three parts instead of two, so that out is as exact as
+// SC (the step that gathers weights): every score goes to a.scores, and with more
+// than one split the combine is left to decode_weights_kernel, which follows; a
+// single split knows its rows' sums and adds the weights itself (256 keys of 8 / 2
+// heads of 64: 7.0 us in one launch, 9.1 in two; 64 sequences of 512-8,192 tokens,
+// 32 / 8 heads of 128: 155 and 160).  W is split in three parts instead of two, so that out is as exact as
 // the weights beside it (2^-25 instead of 2^-18 per term; the third product
 // and its split take no time beside the stream).  The scores' stores take 20 of
-// 150 us (64 sequences of 512-8,192 tokens, 36 MB of scores beside 560 of K and V):
-// bandwidth; nontemporal or coherent stores and waits that do not include them
+// 150 us (those 64 sequences, 36 MB of scores beside 560 of K and V): bandwidth; nontemporal or coherent stores and waits that do not include them
 // changed nothing.
 template <int HD, int G, int W, bool SC>
 __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
@@ -830,7 +831,7 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
 
     const size_t out_row = (size_t)qi * a.n_q_heads + (size_t)kvh * G;
     const size_t pbase = ((size_t)qi * a.n_kv_heads + kvh) * a.n_splits;
-    const bool single = !SC && a.n_splits == 1;
+    const bool single = a.n_splits == 1;
     // Float4 f4 / 4 of this (query, kv head)'s G output rows.  With completion
     // flags the rows are stored through to system scope, every wave waits for
     // its acknowledgements, and then one lane raises the flag: a host that sees
@@ -888,7 +889,52 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
             }
         }
     }
-    if constexpr (SC) return;
+    if constexpr (SC) {
+        if (!single) return;
+        // the weights, from this work-group's scores (stored before the merge's
+        // first barrier) and the waves' (m, l): the new token is the last one
+        __shared__ float fin[2 * G];
+        if (tid < G) {
+            float M = -INFINITY, Lsum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) M = fmaxf(M, mw[w * G + tid]);
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) Lsum += __builtin_amdgcn_exp2f(mw[w * G + tid] - M) * lw[w * G + tid];
+            fin[tid] = M;
+            fin[G + tid] = 1.0f / Lsum;
+        }
+        __syncthreads();
+        const int to = a.seq_of ? a.seq_of[qi] : qi;
+        if (to < 0 || to >= a.max_seqs) return;
+        const float *sc = a.scores + ((size_t)qi * a.n_kv_heads + kvh) * a.score_stride * G;
+        const size_t row = ((size_t)to * a.n_kv_heads + kvh) * a.total_stride;
+        // kAhead tokens' scores and totals of each thread in flight at once (past
+        // the end: those of the last token)
+        constexpr int kAhead = 4;
+        const int end = min(len, a.max_len);
+        for (int t0 = tid; t0 < end; t0 += kAhead * kThreads) {
+            float score[kAhead][G], old[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; j++) {
+                const int t = min(t0 + j * kThreads, end - 1);
+#pragma unroll
+                for (int h = 0; h < G; h++) score[j][h] = sc[(size_t)t * G + h];
+                old[j] = a.total[row + t];
+            }
+#pragma unroll
+            for (int j = 0; j < kAhead; j++) {
+                const int t = t0 + j * kThreads;
+                if (t >= end) break;
+                float w = 0.0f;
+#pragma unroll
+                for (int h = 0; h < G; h++) w += __builtin_amdgcn_exp2f(score[j][h] - fin[h]) * fin[G + h];
+                // a slot begins with the token that takes it
+                a.total[row + t] = t < pos_new ? old[j] + w : w;
+                if (t == pos_new && a.where) a.where[row + t] = a.at_of ? a.at_of[qi] : pos_new;
+            }
+        }
+        return;
+    }
     if (single) {
         if (a.done) signal_done();
         return;

@@ -1,5 +1,5 @@
-// decode_weights.hip — the second half of the decode step that gathers
-// attention weights (decode3.hip with scores): the splits' partials become the
+// decode_weights.hip — the second half of a decode step that gathers attention
+// weights over several splits (decode3.hip with scores): their partials become the
 // output rows, and the scores become weights, which are added to the totals
 // that eviction goes by.  No counterpart in the reference.
 //
@@ -14,9 +14,8 @@
 // partials, the others take kChunkT tokens each.  Every work-group derives M
 // and L itself from the splits' (m, l), so nothing waits for another.
 //
-// Bound by those reads: 64 sequences of 512 .. 8,192 tokens (32 heads of 128 over
-// 8, 54 MB of scores and totals) 12 us, 16 of 16,384 (64 heads over 8) 17; with the
-// scores read after M and L instead of before, 16 and 20.
+// Bound by those reads: 16 sequences of 16,384 tokens (64 heads of 128 over 8, 84 MB
+// of scores and totals) 17 us, 20 with the scores read after M and L.
 #include "tq_common.hpp"
 
 namespace {

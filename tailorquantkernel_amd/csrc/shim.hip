@@ -460,11 +460,15 @@ struct CallScratch {
     size_t counter_ints;
 };
 
-// Where a step that gathers weights leaves its splits' partials and its scores;
-// decode_common fills in the splits.
+// Where a step that gathers weights leaves its splits' partials, its scores and
+// the weights; decode_common fills in the splits.
 struct ScoreScratch {
     float *partials;
     float *scores;
+    const int32_t *at_of;
+    float *total;
+    int32_t *where;
+    size_t stride;
     int split_tokens;
     int n_splits;
 };
@@ -474,7 +478,8 @@ struct ScoreScratch {
 // kernel with q_norm / k_norm and eps (MFMA kernel only).
 // scratch non-null: the split-K partials and counters come from it (a call
 // that needs more returns TQ_HIP_ESCRATCH) and nothing is allocated.
-// ss non-null: the first half of a step that gathers weights (MFMA kernel only).
+// ss non-null: a step that gathers weights (MFMA kernel only), the whole of it with
+// one split, the first launch of two with more.
 int decode_common(tq_hip_kv *kv, int n_q, const int32_t *d_seq, const int32_t *d_len, int len_plus,
                   int seq_const, int seq_stride, int pos0, int max_len, const float *d_q, const float *d_cos,
                   const float *d_sin, const float *d_k, const float *d_v, float *d_out,
@@ -543,6 +548,12 @@ int decode_common(tq_hip_kv *kv, int n_q, const int32_t *d_seq, const int32_t *d
         a.partials = ss->partials;
         a.scores = ss->scores;
         a.score_stride = a.n_splits * a.split_tokens;
+        a.max_len = max_len;
+        a.max_seqs = D.max_seqs;
+        a.at_of = ss->at_of;
+        a.total = ss->total;
+        a.where = ss->where;
+        a.total_stride = ss->stride;
         ss->split_tokens = a.split_tokens;
         ss->n_splits = a.n_splits;
         return herr(tq_launch_decode3(a, waves, s));
@@ -1051,11 +1062,11 @@ int tq_hip_decode_step_weights_async(tq_hip_kv *kv, int n_q, const int32_t *d_se
     const OnDevice on(kv->device);
     if (on.rc != TQ_HIP_OK) return on.rc;
     unsigned char *ws = static_cast<unsigned char *>(d_ws);
-    ScoreScratch ss{reinterpret_cast<float *>(ws), reinterpret_cast<float *>(ws + scores_at), 0, 0};
+    ScoreScratch ss{reinterpret_cast<float *>(ws), reinterpret_cast<float *>(ws + scores_at), d_at, d_total, d_where, stride, 0, 0};
     const hipStream_t s = pick(kv, stream);
     const int rc = decode_common(kv, n_q, d_seq, d_pos, 1, 0, 1, 0, max_pos + 1, d_q, d_cos, d_sin, d_k, d_v, d_out, s,
                                  (!d_seq && n_q == 1) ? 0 : -1, nullptr, nullptr, 0.0f, nullptr, nullptr, &ss);
-    if (rc != TQ_HIP_OK) return rc;
+    if (rc != TQ_HIP_OK || ss.n_splits == 1) return rc;
     TqWeightsArgs a;
     a.seq_of = d_seq;
     a.pos_of = d_pos;

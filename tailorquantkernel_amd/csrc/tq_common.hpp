@@ -250,10 +250,16 @@ struct TqDecodeArgs {
     unsigned *done;
     unsigned done_seq;
     // The step that gathers weights (MFMA kernel only), or null: every score
-    // (exp2 domain) goes to scores[query][kv head][score_stride][group], every
-    // split leaves a partial, and tq_launch_decode_weights finishes the call.
+    // (exp2 domain) goes to scores[query][kv head][score_stride][group].  One
+    // split adds the weights to the totals itself; of more each leaves a partial,
+    // and tq_launch_decode_weights finishes the call.
     float *scores;
     int score_stride;        // >= n_splits * split_tokens
+    int max_len, max_seqs;   // as in TqWeightsArgs
+    const int32_t *at_of;
+    float *total;
+    int32_t *where;
+    size_t total_stride;
 };
 
 hipError_t tq_launch_quantize(const float *x, block_q8 *out, int n, hipStream_t s);
