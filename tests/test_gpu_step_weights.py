@@ -200,6 +200,35 @@ def test_captured_and_replayed(nat, oracle):
             t.check(t.results())
 
 
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("group", [1, 2, 3, 4, 5, 6, 7, 8])
+def test_one_split(nat, oracle, hd, group):
+    """One sequence of up to 256 keys is one split, which finishes the call itself."""
+    length = 97 + 19 * group
+    c = Cache(nat, oracle, 100 + hd + group, 3 * group, 3, hd, [length], room=1)
+    st = Step(c, [length], at=[5 * length], stride=301)
+    st.check(st.run())
+
+
+def test_one_split_batch(nat, oracle):
+    """A batch with a work-group for each (sequence, kv head): lengths from nothing to many passes, idle queries."""
+    r = np.random.default_rng(12)
+    lens = [0, 1, 2100, 31, 32, 600] + [int(x) for x in r.integers(0, 90, 60)]
+    c = Cache(nat, oracle, 13, 16, 8, 32, lens, room=1)
+    seqs = [int(x) for x in r.permutation(len(lens))]
+    pos = [lens[s] if i % 9 else -1 for i, s in enumerate(seqs)]
+    st = Step(c, pos, seqs=seqs, at=[abs(p) + 7 for p in pos], stride=2200, max_pos=2150)
+    out, total, where = st.run()
+    st.check((out, total, where))
+    st = Step(c, [lens[s] if i % 9 else -1 for i, s in enumerate(seqs)], seqs=seqs, stride=2200, max_pos=2150)
+    out, total, where = st.run(where=False)
+    assert (where == st.where).all()
+    for s, p in zip(seqs, st.pos):
+        if p >= 0:
+            where[s, :, p] = p                             # as if it had been given
+    st.check((out, total, where))
+
+
 def test_refusals(nat, oracle):
     c = Cache(nat, oracle, 9, 8, 2, 64, [50, 60], room=1)
     lib, P = c.lib, 4096
