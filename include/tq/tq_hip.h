@@ -233,8 +233,8 @@ int tq_hip_decode_step_norm_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq, 
  * NULL.  Slots past p are not touched, nor anything for a negative d_pos[i].
  * Head dims 32/64/128 with groups 1..8, TQ_HIP_ETYPE otherwise; fp32 arrays
  * 16-byte aligned (the totals 4), d_pos at most max_pos < stride.  d_ws:
- * tq_hip_decode_step_weights_ws_bytes (0: a shape that is not served), 16-byte
- * aligned, nothing is kept in it between calls. */
+ * tq_hip_decode_step_weights_ws_bytes for the same n_q and max_pos (0: a shape that
+ * is not served), 16-byte aligned, nothing is kept in it between calls. */
 size_t tq_hip_decode_step_weights_ws_bytes(const tq_hip_kv *kv, int n_q, int max_pos);
 int tq_hip_decode_step_weights_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq, const int32_t *d_pos, int max_pos,
                                      const float *d_q, const float *d_k, const float *d_v, const float *d_cos,
@@ -261,8 +261,8 @@ int tq_hip_decode_step_weights_async(tq_hip_kv *kv, int n_q, const int32_t *d_se
  * slots' entries; nothing else of them is written.  Lengths are cut to max_len
  * and sequences outside the cache are skipped; a sequence appears at most once
  * per call, and its tokens' pages are mapped and its own.  sinks + recent at most
- * keep; n at most 65535.  d_ws: tq_hip_kv_evict_ws_bytes, 16-byte aligned,
- * nothing is kept in it between calls. */
+ * keep; n at most 65535.  d_ws: tq_hip_kv_evict_ws_bytes for the same n, max_len
+ * and keep, 16-byte aligned, nothing is kept in it between calls. */
 size_t tq_hip_kv_evict_ws_bytes(const tq_hip_kv *kv, int n, int max_len, int keep);
 int tq_hip_kv_evict_async(tq_hip_kv *kv, int n, const int32_t *d_seq, const int32_t *d_len, int max_len,
                           const int32_t *d_next, int keep, int sinks, int recent, const float *d_total,
@@ -455,7 +455,8 @@ typedef struct {
     size_t mask_stride;       /* words per row, or 0: one mask for every row    */
 } tq_hip_logits_rules;
 
-/* Device workspace of tq_hip_logits_process with a d_token, or 0 for a bad shape. */
+/* Device workspace of tq_hip_logits_process with a d_token, or 0 for a bad shape;
+ * enough for fewer rows and a smaller vocab too. */
 size_t tq_hip_logits_ws_bytes(int rows, int vocab);
 /* Row r of vocab logits at logits + r*stride through the rules (NULL: none) into
  * out + r*out_stride (in place where out == logits: the strides must agree; NULL:

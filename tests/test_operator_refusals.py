@@ -52,6 +52,13 @@ def test_logits_workspace(nat):
     assert 0 < f(1, 1) <= f(2, 1) and f(65535, 2 ** 31 - 1) > 2 ** 31
 
 
+@pytest.mark.parametrize("vocab", [1, 1000, 5000, 128256])
+def test_logits_workspace_of_a_batch_serves_smaller_ones(nat, vocab):
+    f = nat.load().tq_hip_logits_ws_bytes
+    sizes = [f(rows, vocab) for rows in range(1, 700)]
+    assert sizes == sorted(sizes) and f(9, max(1, vocab - 1)) <= f(9, vocab)
+
+
 def test_evict_without_a_cache(nat):
     lib = nat.load()
     assert lib.tq_hip_kv_evict_ws_bytes(None, 1, 64, 32) == 0
