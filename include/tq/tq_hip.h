@@ -258,7 +258,7 @@ int tq_hip_decode_step_weights_async(tq_hip_kv *kv, int n_q, const int32_t *d_se
  *
  * d_total_out and d_where_out are the inputs themselves (in place: only moved
  * entries are written) or two other arrays of that shape, which receive the kept
- * slots' entries; nothing else of them is written.  Lengths are cut to max_len
+ * slots' entries; nothing else of them is written.  Tokens past max_len are left out
  * and sequences outside the cache are skipped; a sequence appears at most once
  * per call, and its tokens' pages are mapped and its own.  sinks + recent at most
  * keep; n at most 65535.  d_ws: tq_hip_kv_evict_ws_bytes for the same n, max_len

@@ -49,7 +49,7 @@ struct EvictArgs {
     PagedView view;
     const int32_t *seq_of;   // or null: sequence i
     const int32_t *len_of;
-    const int32_t *next_of;  // or null: the length
+    const int32_t *next_of;  // or null: the length, as given
     int max_len;
     int keep, sinks, recent;
     const float *total;      // [max_seqs][n_kv][stride]
@@ -94,6 +94,9 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
     return x + (row > 0 ? r0 : 0u) + (row > 1 ? r1 : 0u) + (row > 2 ? r2 : 0u);
 }
 
+// A listed slot that is one (all are, see the listing).
+__device__ __forceinline__ bool is_slot(const EvictArgs &a, int t) { return t >= 0 && t < a.max_len; }
+
 // Row piece q (of 2 * per: K's, then V's) of a move, VB bytes, and with the
 // first one the token's total and position.
 template <int VB>
@@ -129,7 +132,7 @@ __global__ __launch_bounds__(64 * WAVES) void evict_select_kernel(EvictArgs a) {
     const int kvh = blockIdx.x, i = blockIdx.y;
     const int seq = a.seq_of ? a.seq_of[i] : i;
     int32_t *list = FEW ? nullptr : list_of(a, i, kvh);
-    const int len = min(a.len_of[i], a.max_len);
+    const int whole = a.len_of[i], len = min(whole, a.max_len);
     if (seq < 0 || seq >= a.view.max_seqs || len <= 0) {
         if (!FEW && tid == 0) list[0] = 0;
         return;
@@ -149,7 +152,7 @@ __global__ __launch_bounds__(64 * WAVES) void evict_select_kernel(EvictArgs a) {
             }
         return;
     }
-    const int next = a.next_of ? a.next_of[i] : len;
+    const int next = a.next_of ? a.next_of[i] : whole;
     const long window = (long)next - a.recent;
     const int per = (len + THREADS - 1) / THREADS;
     const int w0 = wave * per * 64 + lane;   // this lane's slots: w0 + 64 j
@@ -242,8 +245,10 @@ __global__ __launch_bounds__(64 * WAVES) void evict_select_kernel(EvictArgs a) {
     uint32_t edge = kSafe, want = (uint32_t)a.keep;
     if (safe < (uint32_t)a.keep) {
         want -= safe;
-        while (lo != hi) {
+#pragma unroll 1
+        for (int round = 0; round < 3 && lo != hi; round++) {
             // bins of 2^shift codes from lo up; the range shrinks to one of them
+            // (32 bits, 21, 10, one code)
             const int bits = 32 - __clz(hi - lo);
             const int shift = bits > 11 ? bits - 11 : 0;
             for (int b = tid; b < kBins; b += THREADS) hist[b] = 0;
@@ -334,15 +339,21 @@ __global__ __launch_bounds__(64 * WAVES) void evict_select_kernel(EvictArgs a) {
         w3[wave] = movers;
     }
     __syncthreads();
-    uint32_t all = 0;
-    uint32_t hole = sum_before(w2, nullptr), mover = sum_before(w3, &all);
+    // as many holes as movers and no more than there is room for, unless the totals
+    // change under a look that reads them again (a sequence named twice, against the
+    // contract): such a call ends and stays in its arrays, whatever it moves
+    const uint32_t room = FEW ? kFewMoves : (uint32_t)a.cap;
+    uint32_t all = 0, all_holes = 0;
+    uint32_t hole = sum_before(w2, &all_holes), mover = sum_before(w3, &all);
+    all = min(min(all, all_holes), room);
     if (!FEW && tid == 0) list[0] = (int32_t)all;
     int32_t *to_list = FEW ? few : list + 4, *from_list = FEW ? few + kFewMoves : list + 4 + a.cap;
     tie = tie0;
     each([&](int t, uint32_t k) {
         const unsigned long long s = staying(k), in = inside(t), h = in & ~s, m = s & ~in;
-        if ((h >> lane) & 1) to_list[hole + __popcll(h & below)] = t + lane;
-        if ((m >> lane) & 1) from_list[mover + __popcll(m & below)] = t + lane;
+        const uint32_t to_at = hole + __popcll(h & below), from_at = mover + __popcll(m & below);
+        if (((h >> lane) & 1) && (PER > 0 || to_at < room)) to_list[to_at] = t + lane;
+        if (((m >> lane) & 1) && (PER > 0 || from_at < room)) from_list[from_at] = t + lane;
         hole += __popcll(h);
         mover += __popcll(m);
     });
@@ -352,6 +363,7 @@ __global__ __launch_bounds__(64 * WAVES) void evict_select_kernel(EvictArgs a) {
         const int pieces = (int)a.view.row_bytes / vb, n = (int)all * 2 * pieces;
         for (int p = tid; p < n; p += THREADS) {
             const int m = p / (2 * pieces), q = p % (2 * pieces), to = few[m], from = few[kFewMoves + m];
+            if (PER == 0 && (!is_slot(a, to) || !is_slot(a, from))) continue;
             if (vb == 16)
                 move_piece<16>(a, seq, kvh, row, to, from, q, pieces);
             else if (vb == 8)
@@ -386,15 +398,17 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(EvictArgs a) {
         long at = -1;
         if (m < count) {
             const int t = list[4 + end * a.cap + m0 + m];
-            const int phys = phys_page(v, seq, t / kPage);
+            const int phys = is_slot(a, t) ? phys_page(v, seq, t / kPage) : -1;
             if (phys >= 0) at = (long)((size_t)phys * v.page_bytes + (size_t)kvh * v.head_run + (t % kPage) * v.row_bytes);
         }
         base[end][m] = at;
     } else if (tid - 2 * kMoves < min(count, kMoves)) {
         const int m = m0 + tid - 2 * kMoves, to = list[4 + m], from = list[4 + a.cap + m];
         const size_t row = ((size_t)seq * v.n_kv_heads + kvh) * a.stride;
-        a.total_out[row + to] = a.total[row + from];
-        a.where_out[row + to] = a.where[row + from];
+        if (is_slot(a, to) && is_slot(a, from)) {
+            a.total_out[row + to] = a.total[row + from];
+            a.where_out[row + to] = a.where[row + from];
+        }
     }
     __syncthreads();
     // no branch around a load (the compiler would wait for each at its end): a

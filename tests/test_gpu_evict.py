@@ -212,6 +212,33 @@ def test_captured_and_replayed(nat):
         assert total_out.download(c.total.shape, np.float32).tobytes() == want[1].tobytes()
 
 
+@pytest.mark.parametrize("length,keep", [(300, 150), (40000, 10000), (40000, 39950)])
+def test_a_sequence_named_twice(nat, length, keep):
+    """Against the contract: what becomes of that sequence is not said, everything else is as it should be."""
+    lib = nat.load()
+    c = Caches(nat, length, 2, 32, [length, 700, 90], stride=length + 3)
+    pages, guard = [p for i in (1, 2) for p in c.pages[i]], 4096
+    total, where = c.up(c.total), c.up(c.where)
+    order = np.asarray([0, 1, 0, 0], np.int32)
+    seq, length_of = c.up(order), c.up(np.asarray([c.lens[i] for i in order], np.int32))
+    nbytes = lib.tq_hip_kv_evict_ws_bytes(c.kv.h, 4, length, keep)
+    ws = c.up(np.full(nbytes + guard, 0xAB, np.uint8))
+    nat.check(lib.tq_hip_memcpy_h2d(c.base, c.pool.ctypes.data, c.nbytes, None), "pool")
+    nat.check(lib.tq_hip_kv_evict_async(c.kv.h, 4, seq.ptr, length_of.ptr, length, None, keep, 2, 10, total.ptr, where.ptr,
+                                        total.ptr, where.ptr, c.stride, ws.ptr, nbytes, None), "evict")
+    nat.check(lib.tq_hip_device_synchronize(), "sync")
+    pool = np.empty(c.nbytes, np.uint8)
+    nat.check(lib.tq_hip_memcpy_d2h(pool.ctypes.data, c.base, c.nbytes, None), "pool")
+    want = c.expect(keep, 2, 10, [1], True, length, c.lens, False, None, None)
+    nobody = sorted(set(range(c.view(pool).shape[0])) - set(c.pages[0]))
+    assert set(pages) <= set(nobody)
+    assert c.view(pool)[nobody].tobytes() == c.view(want[0])[nobody].tobytes()
+    got = total.download(c.total.shape, np.float32), where.download(c.where.shape, np.int32)
+    for g, w in zip(got, want[1:]):
+        assert g[1:].tobytes() == w[1:].tobytes() and g[0, :, length:].tobytes() == w[0, :, length:].tobytes()
+    assert (ws.download((nbytes + guard,), np.uint8)[nbytes:] == 0xAB).all()
+
+
 def test_refusals(nat):
     lib, P = nat.load(), 4096
     c = Caches(nat, 8, 2, 64, [100, 50])
