@@ -239,6 +239,41 @@ def test_captured_and_replayed(nat, oracle):
         p.check(p.results())
 
 
+@pytest.mark.parametrize("before,dense", [(65500, True), (65520, False)])
+def test_the_longest_sequences(nat, oracle, before, dense):
+    """Up to 65,536 tokens take the dense kernel, one more the row form."""
+    p = Packed(nat, oracle, 14, 2, 1, 64, [36, 20], [before, 3])
+    p.check(p.run(), dense=dense)
+
+
+def test_two_calls_at_once(nat, oracle):
+    """Other sequences of one cache on two streams, each call with its own workspace."""
+    lens, before = [200, 90, 33, 150], [40, 0, 500, 7]
+    p = Packed(nat, oracle, 15, 8, 2, 128, lens, before)
+    a, b = Graphs(), Graphs()
+    out = p.run()
+    p.check(out)
+    parts = []
+    for order in ([0, 2], [1, 3]):
+        # each part's rows stay where they are: the other sequences have none
+        start = np.cumsum([0] + [lens[i] for i in range(4)]).astype(np.int32)
+        calls = []
+        for i in order:
+            at, pos0, seq = start[i:i + 2].copy(), np.asarray([before[i]], np.int32), np.asarray([i], np.int32)
+            nbytes = p.c.lib.tq_hip_prefill_packed_ws_bytes(p.c.kv.h, 1, pos0.ctypes.data, at.ctypes.data)
+            calls.append((seq, pos0, at, nbytes, p.c.up(np.full(nbytes, 0xFF, np.uint8))))
+        parts.append(calls)
+    for _ in range(5):
+        p.dev["out"].upload(np.full(p.q.shape, 9.0, np.float32))
+        p.c.sync()
+        for calls, s in ((parts[0], a.stream), (parts[1], b.stream)):
+            for seq, pos0, at, nbytes, ws in calls:
+                nat.check(p.c.lib.tq_hip_prefill_packed_async(
+                    p.c.kv.h, 1, seq.ctypes.data, pos0.ctypes.data, at.ctypes.data, *(p.dev[k].ptr for k in (
+                        "q", "k", "v", "cos", "sin", "out")), ws.ptr, nbytes, s), "packed")
+        p.check(p.results())
+
+
 def test_refusals(nat, oracle):
     c = Cache(nat, oracle, 12, 8, 2, 64, [50, 60, 70], room=20)
     lib, P = c.lib, 4096

@@ -210,6 +210,34 @@ def test_one_split(nat, oracle, hd, group):
     st.check(st.run())
 
 
+def test_a_long_context(nat, oracle):
+    c = Cache(nat, oracle, 21, 2, 1, 32, [70000, 12], room=1)
+    st = Step(c, [70000, 12], seqs=[0, 1])
+    st.check(st.run())
+
+
+def test_a_sequence_named_twice(nat, oracle):
+    """Against the contract: what its totals become is not said, the other sequences are as they should be."""
+    lens = [300, 40, 700]
+    c = Cache(nat, oracle, 22, 8, 2, 64, lens, room=2)
+    st = Step(c, [300, 40, 301, 700], seqs=[0, 1, 0, 2], stride=800, max_seqs=3)
+    out, total, where = st.run()
+    kq = quantized(c.oracle, rotated(c.oracle, st.k, st.cos, st.sin))
+    vq, qq = quantized(c.oracle, st.v), quantized(c.oracle, rotated(c.oracle, st.q, st.cos, st.sin))
+    for i in (1, 3):
+        s, p = st.seqs[i], st.pos[i]
+        c.put(s, [p], np.stack([kq[i], vq[i]], 1)[None])
+        ref, bound, w, loose = attention(c, qq[i:i + 1], c.rows(s, p + 1), [p])
+        assert (np.abs(out[i] - ref[0]) <= bound[0]).all()
+        w, loose = w[0].reshape(c.nkv, -1, p + 1), loose[0].reshape(c.nkv, -1, 1)
+        before = st.total[s, :, :p + 1].astype(np.float64)
+        before[:, p] = 0.0
+        off = (w * loose).sum(1) + 2.0 ** -24 * (before + 10 * w.sum(1))
+        assert (np.abs(total[s, :, :p + 1] - before - w.sum(1)) <= off).all()
+        assert (total[s, :, p + 1:] == st.total[s, :, p + 1:]).all() and (where[s, :, p] == p).all()
+    assert (total[0, :, 302:] == st.total[0, :, 302:]).all()
+
+
 def test_one_split_batch(nat, oracle):
     """A batch with a work-group for each (sequence, kv head): lengths from nothing to many passes, idle queries."""
     r = np.random.default_rng(12)
