@@ -148,23 +148,31 @@ __global__ __launch_bounds__(kThreads) void append_run_kernel(PagedView view, in
     }
 }
 
-// Sequence and position of every row of the packed sequences: grid (rows of the
-// longest / 256, sequence).
-__global__ __launch_bounds__(256) void pack_rows_kernel(TqPackTable t, int row0, int32_t *seq_of, int32_t *pos_of) {
-    const int i = blockIdx.y, r = (int)blockIdx.x * 256 + (int)threadIdx.x;
-    if (r >= t.n[i]) return;
-    seq_of[t.start[i] - row0 + r] = t.seq[i];
-    pos_of[t.start[i] - row0 + r] = t.pos0[i] + r;
+// Rows of packed sequences, each with its sequence: append_row, and the entry for the
+// decode launches that follow.  Grid (rows, kv head).
+__global__ __launch_bounds__(512) void pack_rows_kernel(TqPackRows a, TqPackTable t, int first, bool clear) {
+    const int r = blockIdx.x, kvh = blockIdx.y, lane = threadIdx.x & 63;
+    const unsigned long long before = __builtin_amdgcn_ballot_w64(lane < t.n_seqs && t.run0[lane] <= r);
+    const int i = __builtin_amdgcn_readfirstlane(__popcll(before) - 1);
+    const int j = r - t.run0[i], seq = t.seq[i], pos = t.pos0[i] + j, row = t.start[i] + j;
+    if (kvh == 0 && threadIdx.x == 0) {
+        a.seq_of[first + r] = seq;
+        a.pos_of[first + r] = pos;
+        a.row_of[first + r] = row;
+    }
+    if (clear)
+        for (size_t c = ((size_t)kvh * gridDim.x + r) * blockDim.x + threadIdx.x; c < a.n_counters;
+             c += (size_t)gridDim.x * gridDim.y * blockDim.x)
+            a.counters[c] = 0;
+    const int phys = phys_page(a.view, seq, pos / kPage);
+    if (phys >= 0) append_row(a.view, phys, pos, row, kvh, a.k, a.v, a.cos_t, a.sin_t, a.head_dim);
 }
 
 }  // namespace
 
-hipError_t tq_launch_pack_rows(const TqPackTable &t, int row0, int32_t *seq_of, int32_t *pos_of, hipStream_t s) {
-    int longest = 0;
-    for (int i = 0; i < t.n_seqs; i++) longest = t.n[i] > longest ? t.n[i] : longest;
-    if (longest == 0) return hipSuccess;
-    hipLaunchKernelGGL(pack_rows_kernel, dim3((unsigned)((longest - 1) / 256 + 1), (unsigned)t.n_seqs), dim3(256), 0, s,
-                       t, row0, seq_of, pos_of);
+hipError_t tq_launch_pack_rows(const TqPackRows &a, const TqPackTable &t, int first, bool clear, hipStream_t s) {
+    hipLaunchKernelGGL(pack_rows_kernel, dim3((unsigned)t.run0[t.n_seqs], (unsigned)a.view.n_kv_heads),
+                       dim3((unsigned)(2 * a.head_dim)), 0, s, a, t, first, clear);
     return hipGetLastError();
 }
 

@@ -458,6 +458,8 @@ struct CallScratch {
     size_t partial_bytes;
     int *counters;         // zero between launches
     size_t counter_ints;
+    const int32_t *row_of = nullptr;   // TqDecodeArgs's
+    bool exact = false;
 };
 
 // Where a step that gathers weights leaves its splits' partials, its scores and
@@ -557,6 +559,11 @@ int decode_common(tq_hip_kv *kv, int n_q, const int32_t *d_seq, const int32_t *d
         ss->split_tokens = a.split_tokens;
         ss->n_splits = a.n_splits;
         return herr(tq_launch_decode3(a, waves, s));
+    }
+    if (scratch) {
+        if (scratch->row_of && !v3) return TQ_HIP_ETYPE;
+        a.row_of = scratch->row_of;
+        a.exact = scratch->exact;
     }
     if (a.n_splits > 1) {
         const size_t row = v3 ? (size_t)tq_decode3_partial_floats(D.head_dim, g) : (size_t)g * (D.head_dim + 2);
@@ -1308,22 +1315,24 @@ namespace {
 // Rows per decode launch of the row form: bounds its split-K partials.
 constexpr int kPackRows = 2048;
 
-// Walk the sequences of a packed call that have rows, longest first, in tables
-// of up to TQ_MAX_PACK.
+// The sequences of a packed call that have rows, longest first, and how each is
+// attended to: by the dense kernel, in tables of up to TQ_MAX_PACK, or row by row.
 struct PackWalk {
-    std::vector<int> order;
+    std::vector<int> dense, rows;
     const int32_t *seq, *pos0, *start;
     PackWalk(int n_seqs, const int32_t *seq_, const int32_t *pos0_, const int32_t *start_)
         : seq(seq_), pos0(pos0_), start(start_) {
-        order.reserve((size_t)n_seqs);
+        dense.reserve((size_t)n_seqs);
         for (int i = 0; i < n_seqs; i++)
-            if (start[i + 1] > start[i]) order.push_back(i);
-        std::stable_sort(order.begin(), order.end(), [this](int a, int b) { return end(a) > end(b); });
+            if (count(i) > 0) dense.push_back(i);
+        std::stable_sort(dense.begin(), dense.end(), [this](int a, int b) { return end(a) > end(b); });
     }
     int first(int i) const { return pos0 ? pos0[i] : 0; }
-    int end(int i) const { return first(i) + start[i + 1] - start[i]; }
-    size_t tables() const { return (order.size() + TQ_MAX_PACK - 1) / TQ_MAX_PACK; }
-    void fill(size_t table, TqPackTable &t) const {
+    int count(int i) const { return start[i + 1] - start[i]; }
+    int end(int i) const { return first(i) + count(i); }
+    static size_t tables(const std::vector<int> &order) { return (order.size() + TQ_MAX_PACK - 1) / TQ_MAX_PACK; }
+    // run0: rows before each sequence's
+    void fill(const std::vector<int> &order, size_t table, TqPackTable &t) const {
         const size_t at = table * TQ_MAX_PACK;
         t = TqPackTable{};
         t.n_seqs = (int)std::min<size_t>(TQ_MAX_PACK, order.size() - at);
@@ -1332,10 +1341,64 @@ struct PackWalk {
             t.seq[j] = seq ? seq[i] : i;
             t.pos0[j] = first(i);
             t.start[j] = start[i];
-            t.n[j] = start[i + 1] - start[i];
+            t.n[j] = count(i);
+            t.run0[j + 1] = t.run0[j] + t.n[j];
         }
     }
-    int longest() const { return order.empty() ? 0 : end(order[0]); }
+    int longest(const std::vector<int> &order) const { return order.empty() ? 0 : end(order[0]); }
+    int total(const std::vector<int> &order) const {
+        int n = 0;
+        for (const int i : order) n += count(i);
+        return n;
+    }
+    void all_by_rows() { rows.swap(dense); }
+
+    // Row by row where a sequence has few rows behind a long context: the dense form
+    // writes an image of every key tile and fills a block of 128 / group tokens,
+    // whatever the rows; the row form reads the cache once per row (from L2 for a
+    // sequence's later rows).  The most rows that go that way (0 .. kMaxShort) are
+    // chosen by the cost of the whole call in us, u the kv heads' size in 8 of 128:
+    //   dense    20 + 0.003 longest + 0.0038 u sum of len
+    //   by rows  10 + u (0.1 sum of n + 0.00038 sum of n len)
+    // which is within a third of both forms over 1, 8 and 32 sequences of 1 .. 64 rows
+    // behind 200 .. 16,000 tokens (32 heads of 128 over 8).  Measured, dense and by
+    // rows: 32 sequences behind up to 4,000, one row each 263 and 48 us, 8 rows 267
+    // and 167, 16 rows 275 and 310; 8 behind 16,000, 4 rows 362 and 127, 12 rows 361
+    // and 388; 32 behind 200, one row 35 and 12, 8 rows 37 and 51; one of 1,296, one
+    // row 49 and 12, 16 rows 50 and 26.  Both forms in one call must promise a gain of
+    // two sevenths: each then fills the card less (24 sequences of 1 .. 24 rows behind
+    // up to 4,000: 197 us split at 8 rows, 180 in either form alone; but 4 prompts of
+    // 500 and 60 single tokens behind up to 4,000: 355 split, 596 dense, 1,371 by rows).
+    static constexpr int kMaxShort = 32;
+    void split(double u) {
+        double best = 0.0;
+        int most = 0;
+        for (int limit = 0; limit <= kMaxShort; limit = limit ? 2 * limit : 1) {
+            double rows_us = 0.0, dense_us = 0.0, longest_us = 0.0;
+            for (const int i : dense) {
+                const double n = count(i), len = end(i);
+                if (n <= limit) {
+                    rows_us += u * (kRowUs * n + kRowKeyUs * n * len);
+                } else {
+                    dense_us += u * kDenseKeyUs * len;
+                    longest_us = std::max(longest_us, kLongestUs * len);
+                }
+            }
+            double cost = (rows_us > 0.0 ? rows_us + kRowsUs : 0.0) +
+                          (dense_us > 0.0 ? dense_us + longest_us + kDenseUs : 0.0);
+            if (rows_us > 0.0 && dense_us > 0.0) cost *= kBothForms;
+            if (limit == 0 || cost < best) {
+                best = cost;
+                most = limit;
+            }
+        }
+        if (most == 0) return;
+        std::vector<int> rest;
+        for (const int i : dense) (count(i) <= most ? rows : rest).push_back(i);
+        dense.swap(rest);
+    }
+    static constexpr double kDenseUs = 20.0, kLongestUs = 0.003, kDenseKeyUs = 0.0038;
+    static constexpr double kRowsUs = 10.0, kRowUs = 0.1, kRowKeyUs = 0.00038, kBothForms = 1.4;
 };
 
 // Whether a packed call's arrays are in order; `rows` and `longest` of it.
@@ -1354,10 +1417,10 @@ bool pack_dense(const tq_hip_kv *kv, int longest, uintptr_t addresses) {
            longest <= kMaxPackKeys;
 }
 
-// The row form's workspace: sequence and position of each row, the decode
+// The row form's workspace: sequence, position and row of each entry, the decode
 // launches' counters and partials, whichever decode kernel runs them.
 struct PackRows {
-    size_t pos, counters, partials, bytes, counter_ints, partial_bytes;
+    size_t pos, row, counters, partials, bytes, counter_ints, partial_bytes;
 };
 PackRows pack_rows_space(const tq_hip_kv *kv, int rows, int longest) {
     auto al = [](size_t x) { return (x + 255) & ~(size_t)255; };
@@ -1378,35 +1441,40 @@ PackRows pack_rows_space(const tq_hip_kv *kv, int rows, int longest) {
     }
     w.counter_ints = (size_t)std::min(rows, kPackRows) * D.n_kv_heads * TQ_DECODE_COUNTER_STRIDE;
     w.pos = al((size_t)rows * sizeof(int32_t));
-    w.counters = 2 * w.pos;
+    w.row = 2 * w.pos;
+    w.counters = 3 * w.pos;
     w.partials = w.counters + al(w.counter_ints * sizeof(int));
     w.bytes = w.partials + w.partial_bytes;
     return w;
 }
 
-int pack_by_rows(tq_hip_kv *kv, const PackWalk &walk, int row0, int rows, const float *d_q, const float *d_k,
-                 const float *d_v, const float *d_cos, const float *d_sin, float *d_out, unsigned char *ws,
-                 hipStream_t s) {
+// The sequences of walk.rows.  mapped: they are some of the call's, their rows
+// anywhere; else all of them, and an entry's row is its own.
+int pack_by_rows(tq_hip_kv *kv, const PackWalk &walk, bool mapped, const float *d_q, const float *d_k, const float *d_v,
+                 const float *d_cos, const float *d_sin, float *d_out, unsigned char *ws, hipStream_t s) {
     const tq_hip_kv_desc &D = kv->desc;
-    const PackRows w = pack_rows_space(kv, rows, walk.longest());
-    int32_t *seq_of = reinterpret_cast<int32_t *>(ws), *pos_of = reinterpret_cast<int32_t *>(ws + w.pos);
+    // in the rows' own order where entries are rows
+    std::vector<int> order = walk.rows;
+    if (!mapped) std::sort(order.begin(), order.end());
+    const int rows = walk.total(order), longest = walk.longest(walk.rows), row0 = walk.start[order[0]];
+    const PackRows w = pack_rows_space(kv, rows, longest);
+    TqPackRows a{kv->view, d_k, d_v, d_cos, d_sin, D.head_dim, reinterpret_cast<int32_t *>(ws),
+                 reinterpret_cast<int32_t *>(ws + w.pos), reinterpret_cast<int32_t *>(ws + w.row),
+                 reinterpret_cast<int *>(ws + w.counters), w.counter_ints};
     TqPackTable t;
-    for (size_t i = 0; i < walk.tables(); i++) {
-        walk.fill(i, t);
-        TQ_TRY(tq_launch_pack_rows(t, row0, seq_of, pos_of, s));
+    int entry = 0;
+    for (size_t i = 0; i < PackWalk::tables(order); i++) {
+        walk.fill(order, i, t);
+        TQ_TRY(tq_launch_pack_rows(a, t, entry, i == 0, s));
+        entry += t.run0[t.n_seqs];
     }
-    hipLaunchKernelGGL(zero_words_kernel, dim3(64), dim3(256), 0, s, reinterpret_cast<uint32_t *>(ws + w.counters),
-                       w.counter_ints);
-    TQ_TRY(hipGetLastError());
-    const size_t qd = (size_t)D.n_q_heads * D.head_dim, kd = (size_t)D.n_kv_heads * D.head_dim, half = D.head_dim / 2;
-    const float *cos0 = d_cos ? d_cos + (size_t)row0 * half : nullptr, *sin0 = d_sin ? d_sin + (size_t)row0 * half : nullptr;
-    TQ_TRY(tq_launch_append(kv->view, rows, seq_of, pos_of, 0, 0, d_k + (size_t)row0 * kd, d_v + (size_t)row0 * kd, cos0,
-                            sin0, D.head_dim, s));
-    const CallScratch sc{reinterpret_cast<float *>(ws + w.partials), w.partial_bytes,
-                         reinterpret_cast<int *>(ws + w.counters), w.counter_ints};
+    const size_t qd = (size_t)D.n_q_heads * D.head_dim, half = D.head_dim / 2;
+    CallScratch sc{reinterpret_cast<float *>(ws + w.partials), w.partial_bytes, a.counters, w.counter_ints};
+    sc.exact = true;
     for (int r = 0; r < rows; r += kPackRows) {
-        const size_t at = (size_t)row0 + r;
-        const int rc = decode_common(kv, std::min(kPackRows, rows - r), seq_of + r, pos_of + r, 1, 0, 1, 0, walk.longest(),
+        const size_t at = mapped ? 0 : (size_t)row0 + r;
+        sc.row_of = mapped ? a.row_of + r : nullptr;
+        const int rc = decode_common(kv, std::min(kPackRows, rows - r), a.seq_of + r, a.pos_of + r, 1, 0, 1, 0, longest,
                                      d_q + at * qd, d_cos ? d_cos + at * half : nullptr,
                                      d_sin ? d_sin + at * half : nullptr, nullptr, nullptr, d_out + at * qd, s, -1,
                                      nullptr, nullptr, 0.0f, &sc);
@@ -1415,18 +1483,25 @@ int pack_by_rows(tq_hip_kv *kv, const PackWalk &walk, int row0, int rows, const 
     return TQ_HIP_OK;
 }
 
-// The larger of the two forms' workspaces: which one runs also depends on the
-// call's addresses.
-size_t pack_bytes(const tq_hip_kv *kv, const PackWalk &walk, int rows) {
+// How a call's sequences are attended to; `addresses` of its arrays, or'ed.
+PackWalk pack_plan(const tq_hip_kv *kv, int n_seqs, const int32_t *seq, const int32_t *pos0, const int32_t *start,
+                   uintptr_t addresses) {
+    PackWalk walk(n_seqs, seq, pos0, start);
+    if (!pack_dense(kv, walk.longest(walk.dense), addresses))
+        walk.all_by_rows();
+    else if (use_decode3(kv))
+        walk.split(kv->desc.n_kv_heads * kv->desc.head_dim / 1024.0);
+    return walk;
+}
+
+// The workspace of a plan: the two forms run one after the other.
+size_t pack_bytes(const tq_hip_kv *kv, const PackWalk &walk) {
     const tq_hip_kv_desc &D = kv->desc;
-    const int g = D.n_q_heads / D.n_kv_heads;
-    size_t bytes = pack_rows_space(kv, rows, walk.longest()).bytes;
-    if (pack_dense(kv, walk.longest(), 0)) {
-        TqPackTable t;
-        for (size_t i = 0; i < walk.tables(); i++) {
-            walk.fill(i, t);
-            bytes = std::max(bytes, tq_pack_bytes(D.head_dim, g, D.n_kv_heads, t));
-        }
+    size_t bytes = walk.rows.empty() ? 0 : pack_rows_space(kv, walk.total(walk.rows), walk.longest(walk.rows)).bytes;
+    TqPackTable t;
+    for (size_t i = 0; i < PackWalk::tables(walk.dense); i++) {
+        walk.fill(walk.dense, i, t);
+        bytes = std::max(bytes, tq_pack_bytes(D.head_dim, D.n_q_heads / D.n_kv_heads, D.n_kv_heads, t));
     }
     return bytes;
 }
@@ -1436,9 +1511,11 @@ size_t pack_bytes(const tq_hip_kv *kv, const PackWalk &walk, int rows) {
 size_t tq_hip_prefill_packed_ws_bytes(const tq_hip_kv *kv, int n_seqs, const int32_t *pos0, const int32_t *start) {
     if (!kv || n_seqs <= 0 || !start || !pack_ok(n_seqs, pos0, start)) return 0;
     try {
-        const PackWalk walk(n_seqs, nullptr, pos0, start);
-        if (walk.longest() > max_context(kv)) return 0;
-        return std::max<size_t>(16, pack_bytes(kv, walk, start[n_seqs] - start[0]));
+        // of an aligned call and of another
+        const PackWalk walk = pack_plan(kv, n_seqs, nullptr, pos0, start, 0),
+                       other = pack_plan(kv, n_seqs, nullptr, pos0, start, 4);
+        if (other.longest(other.rows) > max_context(kv)) return 0;
+        return std::max({(size_t)16, pack_bytes(kv, walk), pack_bytes(kv, other)});
     } catch (...) {
         return 0;
     }
@@ -1473,16 +1550,18 @@ int tq_hip_prefill_packed_async(tq_hip_kv *kv, int n_seqs, const int32_t *seq, c
             for (long p = 0; p < pages; p++)
                 if (row[p] < 0) return TQ_HIP_EINVAL;
         }
-        const PackWalk walk(n_seqs, seq, pos0, start);
-        if (walk.longest() > max_context(kv)) return TQ_HIP_EINVAL;
-        if (ws_bytes < pack_bytes(kv, walk, rows)) return TQ_HIP_EINVAL;
+        const PackWalk walk = pack_plan(kv, n_seqs, seq, pos0, start, addresses);
+        if (std::max(walk.longest(walk.dense), walk.longest(walk.rows)) > max_context(kv)) return TQ_HIP_EINVAL;
+        if (ws_bytes < pack_bytes(kv, walk)) return TQ_HIP_EINVAL;
         const OnDevice on(kv->device);
         if (on.rc != TQ_HIP_OK) return on.rc;
         const hipStream_t s = pick(kv, stream);
         unsigned char *ws = static_cast<unsigned char *>(d_ws);
         const tq_hip_kv_desc &D = kv->desc;
-        if (!pack_dense(kv, walk.longest(), addresses))
-            return pack_by_rows(kv, walk, row0, rows, d_q, d_k, d_v, d_cos, d_sin, d_out, ws, s);
+        if (!walk.rows.empty()) {
+            const int rc = pack_by_rows(kv, walk, !walk.dense.empty(), d_q, d_k, d_v, d_cos, d_sin, d_out, ws, s);
+            if (rc != TQ_HIP_OK || walk.dense.empty()) return rc;
+        }
         TqPackTable t;
         TqPackArgs a;
         a.view = kv->view;
@@ -1497,8 +1576,8 @@ int tq_hip_prefill_packed_async(tq_hip_kv *kv, int n_seqs, const int32_t *seq, c
         a.head_dim = D.head_dim;
         a.scale = 1.0f / sqrtf((float)D.head_dim);
         a.ws = ws;
-        for (size_t i = 0; i < walk.tables(); i++) {
-            walk.fill(i, t);
+        for (size_t i = 0; i < PackWalk::tables(walk.dense); i++) {
+            walk.fill(walk.dense, i, t);
             TQ_TRY(tq_launch_pack(a, s));
         }
         return TQ_HIP_OK;

@@ -249,6 +249,10 @@ struct TqDecodeArgs {
     // at system scope and acknowledged, then done[i * n_kv_heads + h] = done_seq.
     unsigned *done;
     unsigned done_seq;
+    // MFMA kernel only: weights to 2^-25 instead of 2^-18, and query i's rows of q,
+    // cos, sin and out are row_of[i] (null: i).
+    bool exact;
+    const int32_t *row_of;
     // The step that gathers weights (MFMA kernel only), or null: every score
     // (exp2 domain) goes to scores[query][kv head][score_stride][group].  One
     // split adds the weights to the totals itself; of more each leaves a partial,
@@ -439,5 +443,15 @@ struct TqPackArgs {
 bool tq_pack_supported(int head_dim, int group);
 size_t tq_pack_bytes(int head_dim, int group, int n_kv_heads, TqPackTable &t);
 hipError_t tq_launch_pack(const TqPackArgs &a, hipStream_t s);
-// The row form's tables: seq_of[r - row0] and pos_of[r - row0] of every row of the table's sequences.
-hipError_t tq_launch_pack_rows(const TqPackTable &t, int row0, int32_t *seq_of, int32_t *pos_of, hipStream_t s);
+// The row form: K and V of the table's sequences appended, and for their r-th rows
+// entry e = first + r (run0 the first r of each sequence): sequence, position and row;
+// the first launch also clears the decode launches' counters.
+struct TqPackRows {
+    tq::PagedView view;
+    const float *k, *v, *cos_t, *sin_t;
+    int head_dim;
+    int32_t *seq_of, *pos_of, *row_of;
+    int *counters;
+    size_t n_counters;
+};
+hipError_t tq_launch_pack_rows(const TqPackRows &a, const TqPackTable &t, int first, bool clear, hipStream_t s);

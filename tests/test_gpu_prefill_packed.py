@@ -246,6 +246,51 @@ def test_the_longest_sequences(nat, oracle, before, dense):
     p.check(p.run(), dense=dense)
 
 
+@pytest.mark.parametrize("nq,nkv,hd", [(8, 2, 64), (16, 8, 128), (5, 1, 64)])
+def test_prompts_and_single_tokens(nat, oracle, nq, nkv, hd):
+    """Both forms in one call: long prompts, short turns and single tokens, in any order, other rows untouched."""
+    r = np.random.default_rng(nq)
+    lens = [1] * 30 + [150, 2, 300, 0, 7, 90]
+    before = [int(x) for x in r.integers(0, 1500, 30)] + [10, 700, 0, 5, 1200, 33]
+    mix = r.permutation(len(lens))
+    lens, before = [lens[i] for i in mix], [before[i] for i in mix]
+    seqs = [int(x) for x in r.permutation(len(lens))]
+    p = Packed(nat, oracle, 16, nq, nkv, hd, lens, before, seqs=seqs, first=3, spare=4)
+    p.check(p.run())
+
+
+def test_prompts_and_single_tokens_captured(nat, oracle):
+    lens, before = [1] * 40 + [200], [1200] * 40 + [0]
+    p = Packed(nat, oracle, 17, 8, 4, 128, lens, before)
+    gr = Graphs()
+    g = gr.capture(lambda s: nat.check(p.launch(s), "captured"))
+    for seed in range(3):
+        r = np.random.default_rng(seed)
+        for k in "qkv":
+            a = getattr(p, k)
+            a[:] = r.standard_normal(a.shape, dtype=np.float32)
+            p.dev[k].upload(a)
+        gr.replay(g)
+        p.check(p.results())
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, 3e38])
+def test_what_the_causal_mask_hides_row_by_row(nat, oracle, bad):
+    """A later token of a short turn changes no earlier row of it."""
+    args = (nat, oracle, 18, 8, 2, 64, [6, 3], [900, 700])
+    clean = Packed(*args)
+    want = clean.run()
+    clean.check(want)
+
+    def spoil(p):
+        p.k[4, 0], p.v[4, 0], p.v[4, 1, :5], p.k[8, 1, 3], p.v[8] = bad, bad, bad, bad, bad
+    p = Packed(*args, change=spoil)
+    got = p.run()
+    p.check(got, finite=False)
+    for at in (slice(0, 4), slice(6, 8)):
+        assert got[at].tobytes() == want[at].tobytes()
+
+
 def test_two_calls_at_once(nat, oracle):
     """Other sequences of one cache on two streams, each call with its own workspace."""
     lens, before = [200, 90, 33, 150], [40, 0, 500, 7]
