@@ -55,6 +55,8 @@
 // in the reference's order — one lane per head sums the squares serially —
 // and applies (x * inverse) * weight before RoPE, so the K codes stay
 // bit-exact with the whole attention_layer.
+#include <type_traits>
+
 #include "tq_common.hpp"
 
 namespace {
@@ -247,17 +249,19 @@ __device__ __forceinline__ void split3_bf16(const float (&x)[8], v8bf &hi, v8bf 
 }
 
 // W waves per work-group (4, or 8 when each wave has only a tile or two).
-// EX: W is split in three bf16 parts instead of two, so that out is as exact as the
-// weights beside it (2^-25 instead of 2^-18 per term; the third product and its
-// split take no time beside the stream), and query i may stand in row row_of[i].
-// With a.scores, the step that gathers weights: every score goes there, and with
+// MODE, but for kPlain: W is split in three bf16 parts instead of two, so that out is
+// exact to 2^-25 instead of 2^-18 per term (the third product and its split take no
+// time beside the stream).
+// kRows, rows of several sequences' prompts: query i may stand in row row_of[i].
+// kScores, the step that gathers weights: every score goes to a.scores, and with
 // more than one split the combine is left to decode_weights_kernel, which follows;
 // a single split knows its rows' sums and adds the weights itself (256 keys of 8 /
 // 2 heads of 64: 7.0 us in one launch, 9.1 in two; 64 sequences of 512-8,192 tokens,
 // 32 / 8 heads of 128: 155 and 160).  The scores' stores take 20 of 150 us (those 64
 // sequences, 36 MB of scores beside 560 of K and V): bandwidth; nontemporal or
 // coherent stores and waits that do not include them changed nothing.
-template <int HD, int G, int W, bool EX>
+constexpr int kPlain = 0, kRows = 1, kScores = 2;
+template <int HD, int G, int W, int MODE>
 __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
     using L = L3<HD, G>;
     constexpr int kWaves = W;
@@ -352,7 +356,7 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
         // norm weights the K and V slots are too (without a step they repeat q)
         constexpr int QC = G * HD / 4, RC = HD / 8, NC = HD / 4;
         const int nch = QC + 2 * RC + (nrm ? 4 * NC : (step ? 2 * NC : 0));
-        const int at = EX && a.row_of ? a.row_of[qi] : qi;
+        const int at = MODE == kRows && a.row_of ? a.row_of[qi] : qi;
         const float *qg = a.q + ((size_t)at * a.n_q_heads + (size_t)kvh * G) * HD;
         const size_t nrow = ((size_t)qi * a.n_kv_heads + kvh) * HD;
         for (int c0 = 0; c0 < nch; c0 += 64) {
@@ -693,7 +697,7 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
             }
         }
 
-        if (EX && a.scores) {
+        if constexpr (MODE == kScores) {
             // the tile's scores [key][head]: the NB lanes of a head hold the
             // same 8 keys' scores and store 8 / NB of them each, whole runs of
             // heads (G = 4, hd 128: two stores of 256 contiguous bytes)
@@ -731,7 +735,7 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
                 for (int i = 0; i < 8; i++) w[i] = k0 + slot_key(lg, i) < t_end ? w[i] : 0.0f;
             }
             l_part[nt] += ps;
-            if constexpr (EX)
+            if constexpr (MODE != kPlain)
                 split3_bf16(w, whi[nt], wmid[nt], wlo[nt]);
             else
                 split_bf16(w, whi[nt], wlo[nt]);
@@ -752,7 +756,7 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 o[c][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, whi[nt], o[c][nt], 0, 0, 0);
-                if constexpr (EX) o[c][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, wmid[nt], o[c][nt], 0, 0, 0);
+                if constexpr (MODE != kPlain) o[c][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, wmid[nt], o[c][nt], 0, 0, 0);
                 o[c][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, wlo[nt], o[c][nt], 0, 0, 0);
             }
         }
@@ -831,7 +835,7 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
     }
     __syncthreads();
 
-    const size_t out_row = (size_t)(EX && a.row_of ? a.row_of[qi] : qi) * a.n_q_heads + (size_t)kvh * G;
+    const size_t out_row = (size_t)(MODE == kRows && a.row_of ? a.row_of[qi] : qi) * a.n_q_heads + (size_t)kvh * G;
     const size_t pbase = ((size_t)qi * a.n_kv_heads + kvh) * a.n_splits;
     const bool single = a.n_splits == 1;
     // Float4 f4 / 4 of this (query, kv head)'s G output rows.  With completion
@@ -891,7 +895,7 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
             }
         }
     }
-    if (EX && a.scores) {
+    if constexpr (MODE == kScores) {
         if (!single) return;
         // the weights, from this work-group's scores (stored before the merge's
         // first barrier) and the waves' (m, l): the new token is the last one
@@ -1026,27 +1030,27 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
     if (a.done) signal_done();
 }
 
-template <int HD, int G, bool EX>
+template <int HD, int G, int MODE>
 hipError_t launch3_hd_g(const TqDecodeArgs &a, int waves, hipStream_t s) {
     const dim3 grid(a.n_splits, a.n_kv_heads, a.n_q);
     if (waves == 8)
-        hipLaunchKernelGGL((decode3_kernel<HD, G, 8, EX>), grid, dim3(512), 0, s, a);
+        hipLaunchKernelGGL((decode3_kernel<HD, G, 8, MODE>), grid, dim3(512), 0, s, a);
     else
-        hipLaunchKernelGGL((decode3_kernel<HD, G, 4, EX>), grid, dim3(256), 0, s, a);
+        hipLaunchKernelGGL((decode3_kernel<HD, G, 4, MODE>), grid, dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
-template <int HD, bool EX>
+template <int HD, int MODE>
 hipError_t launch3_hd(const TqDecodeArgs &a, int g, int waves, hipStream_t s) {
     switch (g) {
-        case 1: return launch3_hd_g<HD, 1, EX>(a, waves, s);
-        case 2: return launch3_hd_g<HD, 2, EX>(a, waves, s);
-        case 3: return launch3_hd_g<HD, 3, EX>(a, waves, s);
-        case 4: return launch3_hd_g<HD, 4, EX>(a, waves, s);
-        case 5: return launch3_hd_g<HD, 5, EX>(a, waves, s);
-        case 6: return launch3_hd_g<HD, 6, EX>(a, waves, s);
-        case 7: return launch3_hd_g<HD, 7, EX>(a, waves, s);
-        case 8: return launch3_hd_g<HD, 8, EX>(a, waves, s);
+        case 1: return launch3_hd_g<HD, 1, MODE>(a, waves, s);
+        case 2: return launch3_hd_g<HD, 2, MODE>(a, waves, s);
+        case 3: return launch3_hd_g<HD, 3, MODE>(a, waves, s);
+        case 4: return launch3_hd_g<HD, 4, MODE>(a, waves, s);
+        case 5: return launch3_hd_g<HD, 5, MODE>(a, waves, s);
+        case 6: return launch3_hd_g<HD, 6, MODE>(a, waves, s);
+        case 7: return launch3_hd_g<HD, 7, MODE>(a, waves, s);
+        case 8: return launch3_hd_g<HD, 8, MODE>(a, waves, s);
         default: return hipErrorInvalidValue;
     }
 }
@@ -1073,11 +1077,15 @@ hipError_t tq_launch_decode3(const TqDecodeArgs &a, int waves, hipStream_t s) {
         return hipErrorInvalidValue;
     const int g = a.n_q_heads / a.n_kv_heads;
     if (!tq_decode3_supported(a.head_dim, g)) return hipErrorInvalidValue;
-    const bool ex = a.scores || a.exact;
-    switch (a.head_dim) {
-        case 32: return ex ? launch3_hd<32, true>(a, g, waves, s) : launch3_hd<32, false>(a, g, waves, s);
-        case 64: return ex ? launch3_hd<64, true>(a, g, waves, s) : launch3_hd<64, false>(a, g, waves, s);
-        case 128: return ex ? launch3_hd<128, true>(a, g, waves, s) : launch3_hd<128, false>(a, g, waves, s);
-        default: return hipErrorInvalidValue;
-    }
+    auto launch = [&](auto mode) {
+        constexpr int MODE = decltype(mode)::value;
+        switch (a.head_dim) {
+            case 32: return launch3_hd<32, MODE>(a, g, waves, s);
+            case 64: return launch3_hd<64, MODE>(a, g, waves, s);
+            case 128: return launch3_hd<128, MODE>(a, g, waves, s);
+            default: return hipErrorInvalidValue;
+        }
+    };
+    if (a.scores) return launch(std::integral_constant<int, kScores>{});
+    return a.exact ? launch(std::integral_constant<int, kRows>{}) : launch(std::integral_constant<int, kPlain>{});
 }
