@@ -717,12 +717,19 @@ constexpr int kPackRuns = 32;        // most runs of one block
 // Tiles and runs of every sequence of a table, and the length of a run.
 //
 // chunk 0 leaves every block one run.  Where that leaves CUs idle, or one long
-// block at the end, blocks are cut; a choice costs the share of all steps that a
-// CU's two work-groups get, a third of the longest work-group at the end, and the
-// merge, in steps of one tile.
+// block at the end, blocks are cut; a choice costs, in steps of one tile, the share
+// of all steps that a CU's two work-groups get and a third of the longest
+// work-group at the end, or, where all run at once, the longest work-group, whose
+// steps are faster with its CU to itself; and the merge.  A cut run writes
+// 68 KB past the L2s and the last one reads them all, so a cut is dear: 4 prompts
+// of 2,048 tokens, 32 heads of 128 over 8, take 378 us in one run per block, 476 in
+// up to two, 662 in four; one of 2,048 132, 148, 173; but 333 tokens behind 1,300
+// 101, 77, 85.
 constexpr double kPackItem = 6.0;    // a work-group's q, first tiles and output
-constexpr double kPackCut = 3.0;     // and its partial
-constexpr double kPackMerge = 1.5;   // each run that the last one merges
+constexpr double kPackCut = 3.5;     // and its partial, more of it
+constexpr double kPackCutRun = 1.2;  //   the more runs are merged
+constexpr double kPackMerge = 2.5;   // each run that the last one merges
+constexpr double kPackAlone = 0.6;   // a step of the only work-group of a CU
 constexpr int kPackWgs = 2 * kCUs;   // work-groups at a time
 
 void plan_pack(TqPackTable &t, int g, int n_kv, int *n_tiles, int *n_runs) {
@@ -746,10 +753,14 @@ void plan_pack(TqPackTable &t, int g, int n_kv, int *n_tiles, int *n_runs) {
         const int chunk = k == 1 ? 0 : (most + k - 1) / k;
         double items = 0.0;
         for (int i = 0; i < t.n_seqs; i++) items += (double)runs_of(i, chunk);
-        const double fixed = kPackItem + (k > 1 ? kPackCut : 0.0), one = (k == 1 ? most : chunk) + fixed;
+        const double fixed = kPackItem + (k > 1 ? kPackCut + kPackCutRun * k : 0.0), steps = k == 1 ? most : chunk;
         const double share = n_kv * (tiles + items * fixed) / kPackWgs;
-        const double cost =
-            (items * n_kv <= kPackWgs ? one : std::max(one, share + 0.3 * one)) + (k > 1 ? kPackMerge * k : 0.0);
+        // of the longest work-group's steps, those beside another on its CU
+        const double wgs = items * n_kv, beside = std::min(std::max(wgs / kCUs - 1.0, 0.0), 1.0) *
+                                                  std::min(tiles / (items * steps), 1.0);
+        const double cost = (wgs <= kPackWgs ? std::max(share, (kPackAlone + (1.0 - kPackAlone) * beside) * steps + fixed)
+                                             : std::max(steps + fixed, share + 0.3 * (steps + fixed))) +
+                            (k > 1 ? kPackMerge * k : 0.0);
         if (k == 1 || cost < best) {
             best = cost;
             t.chunk = chunk;
