@@ -49,7 +49,7 @@
 // accvgpr_read each.
 //
 // Where blocks leave CUs idle they are cut into runs: each writes its rows' (o, m,
-// l) with agent-coherent stores, and the last of a block to arrive merges them in
+// l, unit) with agent-coherent stores, and the last of a block to arrive merges them in
 // run order.  No work-group waits on another.
 //
 // Precision: two fp16 parts keep 22 bits where bf16's keep 16, but not its range.
@@ -639,10 +639,10 @@ __global__ __launch_bounds__(kThreads, 2) void pack_block_kernel(PackArgs a) {
     for (; t < nt; t++) turn(t);
 
     float M = st.mrow, L = pair_sum(st.lsum);
-#pragma unroll
-    for (int c = 0; c < C; c++) st.o[c] *= st.unit;
-    // columns 32c + 8g + 4h .. + 3 of the row are o[c][4g ..]
-    auto store = [&](const v16f (&o)[C], float l) {
+    // columns 32c + 8g + 4h .. + 3 of the row are o[c][4g ..].  o / l is a mean of V',
+    // at most 127, and only that is taken out of its unit: o, a sum of P of 2^11 and
+    // more, would overflow where the mean does not, and unit / l underflow.
+    auto store = [&](const v16f (&o)[C], float l, float unit) {
         if (!real) return;
         const float inv = 1.0f / l;
         float *row = a.out + qrow + 4 * h;
@@ -651,10 +651,11 @@ __global__ __launch_bounds__(kThreads, 2) void pack_block_kernel(PackArgs a) {
 #pragma unroll
             for (int g = 0; g < 4; g++)
                 *reinterpret_cast<v4f *>(row + 32 * c + 8 * g) =
-                    v4f{o[c][4 * g] * inv, o[c][4 * g + 1] * inv, o[c][4 * g + 2] * inv, o[c][4 * g + 3] * inv};
+                    v4f{o[c][4 * g] * inv * unit, o[c][4 * g + 1] * inv * unit, o[c][4 * g + 2] * inv * unit,
+                        o[c][4 * g + 3] * inv * unit};
     };
     if (segs == 1) {
-        store(st.o, L);
+        store(st.o, L, st.unit);
         return;
     }
 
@@ -673,6 +674,7 @@ __global__ __launch_bounds__(kThreads, 2) void pack_block_kernel(PackArgs a) {
     if (h == 0) {
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(M), prs, place(run.run, HD), 0, kCoherent);
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(L), prs, place(run.run, HD + 1), 0, kCoherent);
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(st.unit), prs, place(run.run, HD + 2), 0, kCoherent);
     }
     __builtin_amdgcn_s_waitcnt(0);   // this thread's partial is at the point of coherence
     int *flag = reinterpret_cast<int *>(&tiles[0][0]);
@@ -683,9 +685,10 @@ __global__ __launch_bounds__(kThreads, 2) void pack_block_kernel(PackArgs a) {
     __syncthreads();
     if (!*flag) return;
     // in run order, a run's loads in flight while the one before is merged; a
-    // run in which the row saw no key (m = -inf) adds nothing
+    // run in which the row saw no key (m = -inf) adds nothing.  The sum is in the
+    // largest unit of the runs that count for something.
     v16f acc[C];
-    float MA = -INFINITY, LA = 0.0f;
+    float MA = -INFINITY, LA = 0.0f, unit = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; c++)
 #pragma unroll
@@ -699,17 +702,21 @@ __global__ __launch_bounds__(kThreads, 2) void pack_block_kernel(PackArgs a) {
                 w[c][g] = __builtin_amdgcn_raw_buffer_load_b128(prs, place(s, 32 * c + 8 * g + 4 * h), 0, kCoherent);
         const float ms = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, place(s, HD), 0, kCoherent));
         const float ls = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, place(s, HD + 1), 0, kCoherent));
+        const float un = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, place(s, HD + 2), 0, kCoherent));
         const float m = fmaxf(MA, ms);
         const float fa = MA == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(MA - m);
         const float fs = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - m);
+        const float ua = fa > 0.0f ? unit : 0.0f, us = fs > 0.0f ? un : 0.0f;
+        unit = fmaxf(ua, us);
+        const float per = unit > 0.0f ? 1.0f / unit : 0.0f, ga = fa * (ua * per), gs = fs * (us * per);
 #pragma unroll
         for (int c = 0; c < C; c++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) acc[c][i] = acc[c][i] * fa + __uint_as_float(w[c][i >> 2][i & 3]) * fs;
+            for (int i = 0; i < 16; i++) acc[c][i] = acc[c][i] * ga + __uint_as_float(w[c][i >> 2][i & 3]) * gs;
         LA = LA * fa + ls * fs;
         MA = m;
     }
-    store(acc, LA);
+    store(acc, LA, unit);
 }
 
 constexpr int kPackRuns = 32;        // most runs of one block

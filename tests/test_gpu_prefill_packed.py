@@ -174,6 +174,19 @@ def test_values_of_many_sizes(nat, oracle):
     p.check(p.run())
 
 
+@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** 120])
+@pytest.mark.parametrize("nq,nkv,hd,lens,before", [
+    (8, 2, 128, [700, 130], [0, 40]), (8, 2, 64, [100], [3000]), (2, 1, 64, [40, 500], [6000, 0])])
+def test_values_near_the_ends_of_the_type(nat, oracle, nq, nkv, hd, lens, before, scale):
+    """Sums of shifted weights times such values leave fp32's range, their means do not."""
+    def change(p):
+        p.v *= np.float32(scale)
+        p.c.pool["d"][:, :, 1] *= np.float32(scale)
+        p.c.upload()
+    p = Packed(nat, oracle, 24, nq, nkv, hd, lens, before, change=change)
+    p.check(p.run())
+
+
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf, 3e38])
 def test_what_the_causal_mask_hides(nat, oracle, bad):
     """A later token's K and V change no earlier row, whatever they are."""
