@@ -60,6 +60,41 @@ int main() {
 """
 
 
+# what a packed call makes of it: blocks of 128 / group tokens, any chunk, up to 32 runs
+# of the longest of its sequences, whose chunk the shorter ones are cut by too
+PACKED = r"""
+#include <algorithm>
+#include <cstdio>
+#include "prefill_runs.hpp"
+using namespace tq;
+int main() {
+    long seen = 0, wrong = 0, odd = 0, longest = 0;
+    for (int group = 1; group <= 8; group++)
+        for (int pos0 : {0, 1, 31, 33, 97, 1000, 4095, 16000, 65000})
+            for (int n : {1, 15, 17, 18, 21, 25, 33, 42, 43, 100, 127, 129, 333, 512, 513})
+                for (int other : {0, 700, 40000})
+                    for (int k = 1; k <= 32; k++) {
+                        const int qb = 128 / group, qblocks = (n + qb - 1) / qb;
+                        const int most = std::max(block_tiles(pos0, n, qb, qblocks - 1), (other + kKT - 1) / kKT);
+                        if (k > 1 && most < 2 * k) break;
+                        const int chunk = k == 1 ? 0 : (most + k - 1) / k;
+                        odd += chunk & 1;
+                        long item = 0;
+                        for (int b = qblocks - 1; b >= 0; b--) {
+                            const int runs = block_runs(block_tiles(pos0, n, qb, b), chunk);
+                            longest = std::max(longest, (long)runs);
+                            for (int s = 0; s < runs; s++, item++, seen++) {
+                                const BlockRun r = block_of_run(pos0, n, qb, qblocks, chunk, (int)item);
+                                wrong += r.blk != b || r.run != s || r.runs != runs;
+                            }
+                        }
+                        wrong += total_runs(pos0, n, qb, qblocks, chunk) != item;
+                    }
+    std::printf("%ld %ld %ld %ld\n", seen, wrong, odd, longest);
+}
+"""
+
+
 PLAN = r"""
 #include <cstdio>
 #include <cstdlib>
@@ -85,6 +120,11 @@ def build(tmp, text):
 def test_block_of_run_equals_the_count(tmp_path):
     seen, wrong, mixed = map(int, build(tmp_path, HARNESS)())
     assert seen > 100_000 and mixed > 100 and wrong == 0, (seen, wrong, mixed)
+
+
+def test_block_of_run_in_a_packed_call(tmp_path):
+    seen, wrong, odd, longest = map(int, build(tmp_path, PACKED)())
+    assert seen > 100_000 and odd > 1000 and longest == 32 and wrong == 0, (seen, wrong, odd, longest)
 
 
 def test_plan_takes_the_measured_cuts(tmp_path):
