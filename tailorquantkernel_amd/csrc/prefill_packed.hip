@@ -58,8 +58,10 @@
 // above its largest scale; o is kept per row in the largest unit of the keys that
 // the row has seen.  A wild tile, one with a key whose scales are all below 2^-9
 // of its largest or with one that is no number, has a unit per key instead,
-// which goes to P.  So what the causal mask hides neither costs a row its bits
-// nor, as 0 times infinity, makes it NaN.
+// which goes to P.  What a scale that is no number makes of a block is added to that
+// block's columns apart from the products, in the rows that see its key.  So what the
+// causal mask hides neither costs a row its bits nor, as 0 times infinity, makes it
+// NaN, and the key's other blocks count as they are.
 //
 // Grid: work-group w serves kv head w % n_kv, so with 8 kv heads an XCD works on
 // one head, and the blocks of one sequence, next to each other in the grid, read
@@ -94,14 +96,15 @@ struct Img {
     static constexpr int KC = 0;                               // [NB][2][64] x 16 B: key l32, values 16k + 8h ..
     static constexpr int KD = KC + NB * 2048;                  // [NB][2 h][16] scales of a lane's keys
     static constexpr int VK = KD + 768;                        // [2 h][16] units of its keys, a wild tile's
-    static constexpr int VE = KD + 1008;                       // the tile's unit, and whether it is wild
+    static constexpr int VO = KD + 896;                        // [C][2] keys whose block's scale is inf, -inf (NaN: both)
+    static constexpr int VE = KD + 1008;                       // the tile's unit; 1 wild, 3 with such a key
     static constexpr int VH = KD + 1024;                       // [C][2][64] x 16 B: column 32c + l32, keys
     static constexpr int VL = VH + C * 2048;                   //   key_of(h, 8k ..); lower parts
     static constexpr int BYTES = VL + C * 2048;
     static constexpr int CHUNKS = BYTES / 16;
     static constexpr int ROUNDS = CHUNKS / kThreads;           // whole rounds of 16-byte copies
     static constexpr int REM = CHUNKS % kThreads;              // copies of the last, partial one
-    static_assert(NB * 128 <= 768 && REM % 64 == 0, "the scales' room, whole waves");
+    static_assert(NB * 128 <= 768 && VO + 8 * C <= VE && REM % 64 == 0, "the scales' room, whole waves");
 };
 
 // The key in register i of lane half h of a 32 x 32 product.
@@ -202,27 +205,30 @@ __global__ __launch_bounds__(kThreads) void pack_stage_kernel(PackArgs a) {
     __shared__ int shared_wild;
     if (tid < 64) {
         auto exponent = [](float d) { return min(max((int)(__float_as_uint(d) >> 23) - 126, -126), 126); };
-        float d = 0.0f;
-        bool odd = false;
-        if (tid < kKT)
-            for (int b = 0; b < NB; b++) {
-                const float v = fabsf(*reinterpret_cast<const float *>(rv + tid * ROW + b * kBlockBytes));
-                odd |= !(v < INFINITY);
-                d = fmaxf(d, v);
-            }
-        const int e = exponent(wave_max(odd ? 0.0f : d));
+        float d = 0.0f;   // the largest that is a number
+        uint32_t odd = 0;
+        for (int b = 0; b < NB; b++) {
+            const float v = tid < kKT ? *reinterpret_cast<const float *>(rv + tid * ROW + b * kBlockBytes) : 0.0f;
+            const bool number = fabsf(v) < INFINITY;
+            d = fmaxf(d, number ? fabsf(v) : 0.0f);
+            const uint32_t up = (uint32_t)__builtin_amdgcn_ballot_w64(!number && !(v < 0.0f));
+            const uint32_t down = (uint32_t)__builtin_amdgcn_ballot_w64(!number && !(v > 0.0f));
+            odd |= up | down;
+            if (tid == 0) *reinterpret_cast<uint2 *>(out + I::VO + 8 * b) = make_uint2(up, down);
+        }
+        const int e = exponent(wave_max(d));
         const float unit = ldexpf(1.0f, e);
-        const bool any = __builtin_amdgcn_ballot_w64(odd || (d > 0.0f && d < unit * 0x1p-9f)) != 0;
+        const bool any = odd != 0 || __builtin_amdgcn_ballot_w64(d > 0.0f && d < unit * 0x1p-9f) != 0;
         if (tid < kKT) {
             const int ek = exponent(d), h = (tid >> 2) & 1, at = (tid >> 3) * 4 + (tid & 3);   // key_of's inverse
-            *reinterpret_cast<float *>(out + I::VK + (h * 16 + at) * 4) = odd ? INFINITY : ldexpf(1.0f, ek);
-            per_key[tid] = odd ? 0.0f : ldexpf(1.0f, -ek);
+            *reinterpret_cast<float *>(out + I::VK + (h * 16 + at) * 4) = ldexpf(1.0f, ek);
+            per_key[tid] = ldexpf(1.0f, -ek);
         }
         if (tid == 0) {
             shared_per_unit = ldexpf(1.0f, -e);
             shared_wild = any;
             *reinterpret_cast<float *>(out + I::VE) = unit;
-            *reinterpret_cast<int *>(out + I::VE + 4) = any;
+            *reinterpret_cast<int *>(out + I::VE + 4) = odd ? 3 : any;
         }
     }
     // K codes: entry (b, k, lane) = key l32, block b, codes 16k + 8h .. + 7
@@ -352,6 +358,36 @@ struct Row {
     }
 };
 
+// The blocks of a tile whose scales are no numbers, into the columns they have, for
+// the rows that see their keys: code (which stands in V') times inf, -inf or NaN.
+template <int HD>
+__device__ __forceinline__ void add_odd_blocks(const unsigned char *T, int h, const float (&p)[16], Row<HD> &st) {
+    using I = Img<HD>;
+    const int l32 = threadIdx.x & 31;
+    uint32_t seen = 0;   // keys with a weight in this lane's row
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        const unsigned long long m = __builtin_amdgcn_ballot_w64(p[i] > 0.0f);
+        seen |= ((uint32_t)(m >> l32) & 1u) << key_of(0, i) | ((uint32_t)(m >> (32 + l32)) & 1u) << key_of(1, i);
+    }
+#pragma unroll
+    for (int c = 0; c < I::C; c++) {
+        const uint2 odd = *reinterpret_cast<const uint2 *>(T + I::VO + 8 * c);
+        const uint32_t up = __builtin_amdgcn_readfirstlane(odd.x), down = __builtin_amdgcn_readfirstlane(odd.y);
+        for (uint32_t left = up | down; left != 0; left &= left - 1) {
+            const int key = __builtin_ctz(left), at = (key >> 3) * 4 + (key & 3);
+            const float d = ((up >> key) & 1 ? INFINITY : 0.0f) + ((down >> key) & 1 ? -INFINITY : 0.0f);
+            const unsigned char *codes = T + I::VH + ((2 * c + (at >> 3)) * 64 + 32 * ((key >> 2) & 1)) * 16 + 2 * (at & 7);
+            const bool sees = (seen >> key) & 1;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float code = (float)*reinterpret_cast<const _Float16 *>(codes + 16 * key_of(h, i));
+                st.o[c][i] += sees ? code * d : 0.0f;
+            }
+        }
+    }
+}
+
 // P in the units of V': the row takes the largest unit among the keys it has
 // seen, o rescaled where that grows; a row that sees none of a tile's keys does
 // not take its unit.
@@ -360,14 +396,15 @@ __device__ __forceinline__ void into_units(const unsigned char *T, int h, Row<HD
     using I = Img<HD>;
     const uint2 head = *reinterpret_cast<const uint2 *>(T + I::VE);
     const float unit = __uint_as_float(__builtin_amdgcn_readfirstlane(head.x));
-    const bool wild = __builtin_amdgcn_readfirstlane(head.y) != 0;
+    const int kind = __builtin_amdgcn_readfirstlane(head.y);
+    const bool wild = kind != 0;
     const float *vk = reinterpret_cast<const float *>(T + I::VK) + 16 * h;
     if (__builtin_amdgcn_ballot_w64(wild || unit > st.unit) != 0) {
         float top = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             const float u = wild ? vk[i] : unit;
-            top = p[i] > 0.0f && u < INFINITY ? fmaxf(top, u) : top;
+            top = p[i] > 0.0f ? fmaxf(top, u) : top;
         }
         const float now = fmaxf(st.unit, pair_max(top));
         const float c = now > 0.0f ? st.unit / now : 1.0f;
@@ -377,6 +414,7 @@ __device__ __forceinline__ void into_units(const unsigned char *T, int h, Row<HD
         st.per_unit = now > 0.0f ? 1.0f / now : 0.0f;
     }
     if (wild) {
+        if (kind == 3) add_odd_blocks<HD>(T, h, p, st);
 #pragma unroll
         for (int i = 0; i < 16; i++) p[i] = p[i] == 0.0f ? 0.0f : p[i] * (vk[i] * st.per_unit);
     } else {

@@ -304,6 +304,42 @@ def test_what_the_causal_mask_hides_row_by_row(nat, oracle, bad):
         assert got[at].tobytes() == want[at].tobytes()
 
 
+# (form, new tokens, cached ones) of a few sequences, all in that form
+FORMS = [("dense", [120, 40], [70, 0]), ("dense", [90], [3000]), ("rows", [6, 3], [900, 700])]
+
+
+@pytest.mark.parametrize("form,lens,before", FORMS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_value_blocks_that_are_no_numbers(nat, oracle, form, lens, before, hd, bad):
+    """One block of a key's values: only its own columns, in the rows that see the key, are no numbers."""
+    def change(p):
+        c, t = p.c, before[0] - 40
+        c.pool[c.pages[0][t // 16], 0, 1, t % 16]["d"][-1] = bad       # an old key
+        c.upload()
+        p.v[2, 1, 5] = np.inf                                            # a new one, its first block
+    p = Packed(nat, oracle, 25, 8, 2, hd, lens, before, change=change)
+    got = p.run()
+    p.check(got, finite=False)
+    c = p.c
+    qq = quantized(c.oracle, rotated(c.oracle, p.q, p.cos, p.sin))
+    for i, (n, b) in enumerate(zip(lens, before)):
+        rows, at = c.rows(i, b + n), slice(p.start[i], p.start[i + 1])
+        odd = ~np.isfinite(rows[:, :, 1]["d"])                           # [key][kv head][block]
+        assert odd.sum() == (2 if i == 0 else 0)
+        rows["d"][:, :, 1][odd] = 0.0
+        ref, bound, _, _ = attention(c, qq[at], rows, range(b, b + n), 2.0 ** -20 if form == "dense" else 2.0 ** -17)
+        if form == "dense":
+            top = rows[:, :, 1]["d"].max((0, 2)).astype(np.float64)
+            bound += (b + n) * 2.0 ** -28 * np.repeat(top, 4)[None, :, None]
+        seen = np.arange(b + n)[None, :] <= np.arange(b, b + n)[:, None]
+        hit = np.einsum("rt,thb->rhb", seen.astype(int), odd.astype(int)) > 0
+        hit = np.repeat(np.repeat(hit, 4, 1), 32, 2)                     # [row][head][column]
+        assert hit.any() == (i == 0)
+        assert not np.isfinite(got[at][hit]).any()
+        assert (np.abs(got[at] - ref)[~hit] <= bound[~hit]).all()
+
+
 def test_two_calls_at_once(nat, oracle):
     """Other sequences of one cache on two streams, each call with its own workspace."""
     lens, before = [200, 90, 33, 150], [40, 0, 500, 7]
