@@ -287,12 +287,14 @@ int tq_hip_prefill_async(tq_hip_kv *kv, int seq, int pos0, int n, const float *d
  * than the one before) are HOST arrays, read during the call.  TQ_HIP_EINVAL,
  * before any launch, for a sequence that appears twice or that has no page for one
  * of its tokens; a page that takes a token of one sequence is no other's.  Head
- * dims 64/128 with groups 1..8 and up to 65,536 tokens a sequence take the dense
- * kernel (arrays 16-byte aligned), which keeps P and V to 2^-22 where
- * tq_hip_prefill_async keeps 2^-16 (and no term below 2^-29 of the largest V scale
- * so far).  Sequences with few new tokens, and every sequence of other shapes,
- * attend row by row as decode steps do, with products as exact: prompts, short
- * turns and single tokens can share a call.  d_ws:
+ * dims 64/128 with groups 1..8 take the dense kernel (arrays 16-byte aligned), which
+ * keeps P and V to 2^-22 where tq_hip_prefill_async keeps 2^-16 (and no term below
+ * 2^-29 of the largest V scale so far).  Sequences with few new tokens, those of
+ * more than 65,536 tokens, and every sequence of other shapes, attend row by row as
+ * decode steps do, with products as exact: prompts, short turns and single tokens
+ * can share a call.  (A whole prompt row by row takes many times as long.)  The
+ * form of a sequence and the cuts of its blocks go by the cost of the whole call: its
+ * precision does not depend on the others, its last bits may.  d_ws:
  * tq_hip_prefill_packed_ws_bytes for the same pos0 and start (0: a call that is
  * refused), 16-byte aligned; nothing is kept in it. */
 size_t tq_hip_prefill_packed_ws_bytes(const tq_hip_kv *kv, int n_seqs, const int32_t *pos0, const int32_t *start);

@@ -1352,6 +1352,13 @@ struct PackWalk {
         return n;
     }
     void all_by_rows() { rows.swap(dense); }
+    // Those past the dense kernel's length, which stand in front.
+    void long_by_rows() {
+        size_t n = 0;
+        while (n < dense.size() && end(dense[n]) > kMaxPackKeys) n++;
+        rows.assign(dense.begin(), dense.begin() + (long)n);
+        dense.erase(dense.begin(), dense.begin() + (long)n);
+    }
 
     // Row by row where a sequence has few rows behind a long context: the dense form
     // writes an image of every key tile and fills a block of 128 / group tokens,
@@ -1369,6 +1376,7 @@ struct PackWalk {
     // two sevenths: each then fills the card less (24 sequences of 1 .. 24 rows behind
     // up to 4,000: 197 us split at 8 rows, 180 in either form alone; but 4 prompts of
     // 500 and 60 single tokens behind up to 4,000: 355 split, 596 dense, 1,371 by rows).
+    // Sequences that go by rows in any case (long_by_rows) count for nothing here.
     static constexpr int kMaxShort = 32;
     void split(double u) {
         double best = 0.0;
@@ -1401,7 +1409,7 @@ struct PackWalk {
     static constexpr double kRowsUs = 10.0, kRowUs = 0.1, kRowKeyUs = 0.00038, kBothForms = 1.4;
 };
 
-// Whether a packed call's arrays are in order; `rows` and `longest` of it.
+// Whether a packed call's pos0 and start are in order.
 bool pack_ok(int n_seqs, const int32_t *pos0, const int32_t *start) {
     if (start[0] < 0) return false;
     for (int i = 0; i < n_seqs; i++) {
@@ -1411,10 +1419,9 @@ bool pack_ok(int n_seqs, const int32_t *pos0, const int32_t *start) {
     return true;
 }
 
-bool pack_dense(const tq_hip_kv *kv, int longest, uintptr_t addresses) {
+bool pack_dense(const tq_hip_kv *kv, uintptr_t addresses) {
     const tq_hip_kv_desc &D = kv->desc;
-    return prefill_dense() && (addresses & 15) == 0 && tq_pack_supported(D.head_dim, D.n_q_heads / D.n_kv_heads) &&
-           longest <= kMaxPackKeys;
+    return prefill_dense() && (addresses & 15) == 0 && tq_pack_supported(D.head_dim, D.n_q_heads / D.n_kv_heads);
 }
 
 // The row form's workspace: sequence, position and row of each entry, the decode
@@ -1487,10 +1494,13 @@ int pack_by_rows(tq_hip_kv *kv, const PackWalk &walk, bool mapped, const float *
 PackWalk pack_plan(const tq_hip_kv *kv, int n_seqs, const int32_t *seq, const int32_t *pos0, const int32_t *start,
                    uintptr_t addresses) {
     PackWalk walk(n_seqs, seq, pos0, start);
-    if (!pack_dense(kv, walk.longest(walk.dense), addresses))
-        walk.all_by_rows();
-    else if (use_decode3(kv))
+    const bool pack = pack_dense(kv, addresses);
+    if (pack && use_decode3(kv)) {
+        walk.long_by_rows();
         walk.split(kv->desc.n_kv_heads * kv->desc.head_dim / 1024.0);
+    } else if (!pack || walk.longest(walk.dense) > kMaxPackKeys) {
+        walk.all_by_rows();   // (only the MFMA decode takes some of a call's rows)
+    }
     return walk;
 }
 

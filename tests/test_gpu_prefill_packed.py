@@ -340,6 +340,31 @@ def test_value_blocks_that_are_no_numbers(nat, oracle, form, lens, before, hd, b
         assert (np.abs(got[at] - ref)[~hit] <= bound[~hit]).all()
 
 
+@pytest.mark.parametrize("place", ["first", "last"])
+def test_a_long_sequence_and_its_neighbours(nat, oracle, place):
+    """One past the dense kernel's length goes row by row, the others as without it: bit for bit."""
+    lens, before = [300, 150, 40], [0, 20, 5]
+    others = slice(0, 3)
+    if place == "last":
+        lens, before = lens + [2], before + [65600]
+    else:
+        lens, before, others = [2] + lens, [65600] + before, slice(1, 4)
+    p = Packed(nat, oracle, 27, 2, 1, 64, lens, before)
+    out = p.run()
+    p.check(out)
+    seq = np.arange(4, dtype=np.int32)[others].copy()
+    pos0, start = p.pos0[others].copy(), p.start[others.start:others.stop + 1].copy()
+    nbytes = p.c.lib.tq_hip_prefill_packed_ws_bytes(p.c.kv.h, 3, pos0.ctypes.data, start.ctypes.data)
+    p.dev["out"].upload(np.full(p.q.shape, 9.0, np.float32))
+    ws = p.c.up(np.full(nbytes, 0xFF, np.uint8))
+    nat.check(p.c.lib.tq_hip_prefill_packed_async(
+        p.c.kv.h, 3, seq.ctypes.data, pos0.ctypes.data, start.ctypes.data, *(p.dev[k].ptr for k in (
+            "q", "k", "v", "cos", "sin", "out")), ws.ptr, nbytes, None), "packed")
+    alone = p.results()
+    at = slice(int(start[0]), int(start[-1]))
+    assert np.array_equal(alone[at].view(np.uint32), out[at].view(np.uint32))
+
+
 def test_two_calls_at_once(nat, oracle):
     """Other sequences of one cache on two streams, each call with its own workspace."""
     lens, before = [200, 90, 33, 150], [40, 0, 500, 7]
