@@ -606,7 +606,8 @@ __global__ __launch_bounds__(256) void decode_kernel(TqDecodeArgs a) {
             }
             const int uu = u0 + tid;
             const int gi = (4 * uu) / HD, j = 4 * uu - gi * HD;
-            *reinterpret_cast<float4 *>(a.out + ((size_t)qi * a.n_q_heads + (size_t)kvh * G + gi) * HD + j) = r;
+            *reinterpret_cast<v4f_any *>(a.out + ((size_t)qi * a.n_q_heads + (size_t)kvh * G + gi) * HD + j) =
+                v4f_any{r.x, r.y, r.z, r.w};
         }
         __syncthreads();
     }

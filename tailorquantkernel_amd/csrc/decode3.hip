@@ -847,7 +847,7 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
         if (a.done)
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, val), ors, 4 * f4, 0, kSystem);
         else
-            *reinterpret_cast<v4f *>(a.out + out_row * HD + f4) = val;
+            *reinterpret_cast<v4f_any *>(a.out + out_row * HD + f4) = val;
     };
     auto signal_done = [&]() {
         __builtin_amdgcn_s_waitcnt(0);

@@ -25,6 +25,9 @@ constexpr int kThreads = 256;     // work-group size of the attention kernels
 // 16-byte vector as a native clang vector, which stays in registers where
 // HIP's struct-wrapped uint4 can end up in scratch.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// Four floats on any float's boundary: where a caller's output may lie anywhere.  The
+// store is still one of 16 bytes, which a global address need not be a multiple of.
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
 
 // ---------------------------------------------------------------------------
 // Cross-lane moves with DPP (a VALU modifier, a few cycles) instead of

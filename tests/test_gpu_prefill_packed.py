@@ -340,6 +340,26 @@ def test_value_blocks_that_are_no_numbers(nat, oracle, form, lens, before, hd, b
         assert (np.abs(got[at] - ref)[~hit] <= bound[~hit]).all()
 
 
+class Shifted:
+    """A device array one float off the boundary it would have."""
+
+    def __init__(self, c, a):
+        self.buf = c.up(np.concatenate([np.zeros(1, np.float32), a]))
+        self.ptr = self.buf.ptr + 4
+
+    def download(self, shape, dtype):
+        return self.buf.download((shape[0] + 1,), dtype)[1:]
+
+
+@pytest.mark.parametrize("shifted", [["out"], ["q"], ["k", "v"], ["cos", "sin"], ["q", "k", "v", "cos", "sin"]])
+def test_some_arrays_off_the_boundary(nat, oracle, shifted):
+    p = Packed(nat, oracle, 26, 8, 2, 64, [40, 20, 1], [0, 40, 900])
+    for k in shifted:
+        a = np.full(p.q.shape, 9.0, np.float32) if k == "out" else getattr(p, k)
+        p.dev[k] = Shifted(p.c, a.reshape(-1))
+    p.check(p.run(), dense=False)
+
+
 @pytest.mark.parametrize("place", ["first", "last"])
 def test_a_long_sequence_and_its_neighbours(nat, oracle, place):
     """One past the dense kernel's length goes row by row, the others as without it: bit for bit."""
