@@ -260,6 +260,8 @@ __device__ __forceinline__ void split3_bf16(const float (&x)[8], v8bf &hi, v8bf 
 // 32 / 8 heads of 128: 155 and 160).  The scores' stores take 20 of 150 us (those 64
 // sequences, 36 MB of scores beside 560 of K and V): bandwidth; nontemporal or
 // coherent stores and waits that do not include them changed nothing.
+// RMSNorm and completion flags are kPlain's only; kRows appends nothing and takes its
+// pages from the table, kScores always appends.
 constexpr int kPlain = 0, kRows = 1, kScores = 2;
 template <int HD, int G, int W, int MODE>
 __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
@@ -325,9 +327,9 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
     const int t_begin = split * a.split_tokens;
     const int split_end = t_begin + a.split_tokens;
     const PagedView &view = a.view;
-    const bool contig = a.contig_first >= 0;
+    const bool contig = MODE != kRows && a.contig_first >= 0;
     const bool rot = a.cos_t != nullptr;
-    const bool step = a.k_new != nullptr;
+    const bool step = MODE == kScores || (MODE == kPlain && a.k_new != nullptr);
     unsigned char *tb0 = slot0[wave];
     unsigned char *tb1 = slot1[wave];
     // Uniform inputs: issued first as unconditional scalar loads (a dummy
@@ -340,7 +342,7 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
     //      front of its second slot: q rows of the group | cos | sin | new K | new V
     //      (fp32).  These copies go first so that waiting for them lets every
     //      later K/V copy stay in flight.
-    const bool nrm = a.q_norm != nullptr;
+    const bool nrm = MODE == kPlain && a.q_norm != nullptr;
     float *stq = reinterpret_cast<float *>(tb1);
     float *stc = stq + G * HD;
     float *sts = stc + HD / 2;
@@ -844,7 +846,7 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
     // the flag finds the rows in its memory (and the kernel writes nothing after).
     const __amdgpu_buffer_rsrc_t ors = __builtin_amdgcn_make_buffer_rsrc(a.out + out_row * HD, 0, G * HD * 4, kBufWord3);
     auto put_out = [&](int f4, v4f val) {
-        if (a.done)
+        if (MODE == kPlain && a.done)
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, val), ors, 4 * f4, 0, kSystem);
         else
             *reinterpret_cast<v4f_any *>(a.out + out_row * HD + f4) = val;
@@ -942,7 +944,7 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
         return;
     }
     if (single) {
-        if (a.done) signal_done();
+        if (MODE == kPlain && a.done) signal_done();
         return;
     }
     __builtin_amdgcn_s_waitcnt(0);   // the partial is at the point of coherence
@@ -1027,7 +1029,7 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
             __syncthreads();
         }
     }
-    if (a.done) signal_done();
+    if (MODE == kPlain && a.done) signal_done();
 }
 
 template <int HD, int G, int MODE>
@@ -1075,6 +1077,10 @@ hipError_t tq_launch_decode3(const TqDecodeArgs &a, int waves, hipStream_t s) {
     if (a.scores ? !a.partials || a.score_stride < (long)a.n_splits * a.split_tokens
                  : a.n_splits > 1 && (a.partials == nullptr || a.counters == nullptr))
         return hipErrorInvalidValue;
+    if (a.scores || a.exact) {   // what these instantiations leave out
+        if (a.q_norm || a.done) return hipErrorInvalidValue;
+        if (a.scores ? !a.k_new : a.k_new || a.contig_first >= 0) return hipErrorInvalidValue;
+    }
     const int g = a.n_q_heads / a.n_kv_heads;
     if (!tq_decode3_supported(a.head_dim, g)) return hipErrorInvalidValue;
     auto launch = [&](auto mode) {
