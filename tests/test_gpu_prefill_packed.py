@@ -385,6 +385,28 @@ def test_a_long_sequence_and_its_neighbours(nat, oracle, place):
     assert np.array_equal(alone[at].view(np.uint32), out[at].view(np.uint32))
 
 
+@pytest.mark.parametrize("rope", [True, False])
+@pytest.mark.parametrize("skew", [0, 1])
+def test_row_form_order_offset_and_spare_rows(nat, oracle, rope, skew):
+    """Short turns only: sequences in any order, rows that belong to none, with and without RoPE."""
+    p = Packed(nat, oracle, 28, 6, 2, 64, [2, 0, 5, 1], [900, 3, 1300, 700], seqs=[5, 1, 0, 3], first=9, spare=6, rope=rope,
+               skew=skew)
+    p.check(p.run(), dense=False)
+
+
+@pytest.mark.parametrize("nq,nkv,hd", [(3, 1, 128), (5, 1, 64), (12, 2, 128), (7, 1, 128)])
+def test_cut_blocks_of_odd_groups(nat, oracle, nq, nkv, hd):
+    """Runs of blocks that do not fill their rows, with values 2^40 apart from one stretch of keys to the next."""
+    def change(p):
+        rows = np.arange(4200) // 500 % 2
+        for t in range(4200):
+            if rows[t]:
+                p.c.pool["d"][p.c.pages[0][t // 16], :, 1, t % 16] *= np.float32(2.0 ** -40)
+        p.c.upload()
+    p = Packed(nat, oracle, 29, nq, nkv, hd, [70, 40], [4200, 0], change=change)
+    p.check(p.run())
+
+
 def test_two_calls_at_once(nat, oracle):
     """Other sequences of one cache on two streams, each call with its own workspace."""
     lens, before = [200, 90, 33, 150], [40, 0, 500, 7]
