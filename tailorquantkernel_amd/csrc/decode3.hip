@@ -256,7 +256,7 @@ __device__ __forceinline__ void split3_bf16(const float (&x)[8], v8bf &hi, v8bf 
 // kScores, the step that gathers weights: every score goes to a.scores, and with
 // more than one split the combine is left to decode_weights_kernel, which follows;
 // a single split knows its rows' sums and adds the weights itself (256 keys of 8 /
-// 2 heads of 64: 7.0 us in one launch, 9.1 in two; 64 sequences of 512-8,192 tokens,
+// 2 heads of 64: 6.8 us in one launch, 9.1 in two; 64 sequences of 512-8,192 tokens,
 // 32 / 8 heads of 128: 155 and 160).  The scores' stores take 20 of 150 us (those 64
 // sequences, 36 MB of scores beside 560 of K and V): bandwidth; nontemporal or
 // coherent stores and waits that do not include them changed nothing.

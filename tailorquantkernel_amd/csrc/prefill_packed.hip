@@ -39,13 +39,14 @@
 // What bounds it: the vector work and the products, added up.  A SIMD overlaps
 // four vector instructions with a 32x32x16 product and none with a 16x16x32 one
 // (probes: 33 cycles, 36 with 4 fma, 64 with 16; two of 16x16x32 as much without
-// any), a tile of 32 rows and 32 keys is 32 products and 357 vector
+// any), a tile of 32 rows and 32 keys is 32 products and 351 vector
 // instructions, and the clock falls to 1.8 .. 2.0 GHz under the load.  Measured,
-// 32 heads of 128 over 8: 16 prompts of 64 .. 2,048 tokens 640 us (staging 80,
-// blocks 560, 0.8 PFLOP/s of products); 24 turns of 8 .. 512 tokens behind up to
-// 4,000 cached 564 us (staging 110).  With 16x16x32 products
-// in place of 32x32x16 they took 685 and 585 us.  64 rows per wave and one wave per
-// SIMD would halve the LDS reads, but the products' results then lie in AGPRs, an
+// 32 heads of 128 over 8: 16 prompts of 64 .. 2,048 tokens 638 us a call, 24 turns of
+// 8 .. 512 tokens behind up to 4,000 cached 556.  A kernel trace of 40 such calls
+// from a card at rest on gives staging 80 and 114 us, blocks 619 and 512 in the mean,
+// 562 (0.8 PFLOP/s of products) and 464 at the least: the clock.  With 16x16x32
+// products in place of 32x32x16 the calls took 685 and 585.  64 rows per wave and one
+// wave per SIMD would halve the LDS reads, but the products' results then lie in AGPRs, an
 // accvgpr_read each.
 //
 // Where blocks leave CUs idle they are cut into runs: each writes its rows' (o, m,

@@ -25,8 +25,8 @@ struct BlockRun {
 
 // Run `item` in order of falling blocks.  Block b < the last ends at key
 // e = pos0 + (b + 1) qb and has ceil(e / (kKT chunk)) runs, so the blocks of r
-// runs are one interval: a step per run count (at most the longest block's, 8),
-// not one per block, of which 1 or 2 kv heads have hundreds (8 / 1 heads of
+// runs are one interval: a step per run count (at most the longest block's: 8,
+// 32 in a packed call), not one per block, of which 1 or 2 kv heads have hundreds (8 / 1 heads of
 // 128, 8,000 tokens after none: 464 us with a work-group counting block by
 // block, 348 so; 4,000 tokens 132 and 107).
 __host__ __device__ inline BlockRun block_of_run(int pos0, int n, int qb, int qblocks, int chunk, int item) {
@@ -77,7 +77,7 @@ __host__ __device__ inline BlockRun plan_item(int pos0, int n, int qb, int qbloc
 }
 
 constexpr int kCUs = 256;       // compute units of an MI355X
-constexpr int kMaxRuns = 8;     // runs of one query block
+constexpr int kMaxRuns = 8;     // runs of one query block in plan_runs
 // The plan's costs, in steps (a pair of key tiles, about 1.7 us at head_dim
 // 128): a work-group's prologue and store, its partial, and each run the last
 // one merges.

@@ -1369,13 +1369,14 @@ struct PackWalk {
     //   by rows  10 + u (0.1 sum of n + 0.00038 sum of n len)
     // which is within a third of both forms over 1, 8 and 32 sequences of 1 .. 64 rows
     // behind 200 .. 16,000 tokens (32 heads of 128 over 8).  Measured, dense and by
-    // rows: 32 sequences behind up to 4,000, one row each 263 and 48 us, 8 rows 267
-    // and 167, 16 rows 275 and 310; 8 behind 16,000, 4 rows 362 and 127, 12 rows 361
-    // and 388; 32 behind 200, one row 35 and 12, 8 rows 37 and 51; one of 1,296, one
-    // row 49 and 12, 16 rows 50 and 26.  Both forms in one call must promise a gain of
+    // rows: 32 sequences behind up to 4,000, one row each 267 and 47 us, 8 rows 270
+    // and 153, 16 rows 275 and 279; 8 behind 16,000, 4 rows 314 and 115, 12 rows 317
+    // and 347; 32 behind 200, one row 34 and 12, 8 rows 37 and 44; one of 1,296, one
+    // row 48 and 12, 16 rows 50 and 24.  Both forms in one call must promise a gain of
     // two sevenths: each then fills the card less (24 sequences of 1 .. 24 rows behind
-    // up to 4,000: 197 us split at 8 rows, 180 in either form alone; but 4 prompts of
-    // 500 and 60 single tokens behind up to 4,000: 355 split, 596 dense, 1,371 by rows).
+    // up to 4,000: 165 us split, 177 dense, 158 by rows; but 64, 4 prompts of
+    // 500 and 60 single tokens, all behind up to 4,000: 320 split, 529 dense, 1,247 by
+    // rows).
     // Sequences that go by rows in any case (long_by_rows) count for nothing here.
     static constexpr int kMaxShort = 32;
     void split(double u) {
