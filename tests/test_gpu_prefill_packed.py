@@ -407,6 +407,37 @@ def test_cut_blocks_of_odd_groups(nat, oracle, nq, nkv, hd):
     p.check(p.run())
 
 
+def test_a_long_prompt_in_groups_beside_others(nat, oracle):
+    """More rows than one decode launch takes, of a sequence past the dense kernel's length, between dense ones: the
+    bits of a call of that sequence alone (the others' blocks may be cut another way: right in both)."""
+    lens, before = [90, 2100, 50], [0, 64000, 7]
+    p = Packed(nat, oracle, 30, 2, 1, 64, lens, before)
+    out = p.run()
+    p.check(out, finite=False)
+    blank = np.full(p.q.shape, 9.0, np.float32)
+    ptrs = [p.dev[k].ptr for k in ("q", "k", "v", "cos", "sin", "out")]
+    got = np.zeros_like(out)
+    for i in range(3):
+        seq, pos0, start = np.asarray([i], np.int32), p.pos0[i:i + 1].copy(), p.start[i:i + 2].copy()
+        nbytes = p.c.lib.tq_hip_prefill_packed_ws_bytes(p.c.kv.h, 1, pos0.ctypes.data, start.ctypes.data)
+        ws = p.c.up(np.full(nbytes, 0xFF, np.uint8))
+        p.dev["out"].upload(blank)
+        nat.check(p.c.lib.tq_hip_prefill_packed_async(p.c.kv.h, 1, seq.ctypes.data, pos0.ctypes.data, start.ctypes.data,
+                                                      *ptrs, ws.ptr, nbytes, None), "packed")
+        alone, at = p.results(), slice(int(start[0]), int(start[1]))
+        assert (alone[:at.start] == 9.0).all() and (alone[at.stop:] == 9.0).all()
+        got[at] = alone[at]
+    at = slice(int(p.start[1]), int(p.start[2]))
+    assert np.array_equal(got[at].view(np.uint32), out[at].view(np.uint32))
+    qq = quantized(oracle, rotated(oracle, p.q, p.cos, p.sin))
+    for i in (0, 2):
+        n, b, at = lens[i], before[i], slice(int(p.start[i]), int(p.start[i + 1]))
+        rows = p.c.rows(i, b + n)
+        ref, bound, _, _ = attention(p.c, qq[at], rows, range(b, b + n), 2.0 ** -20)
+        bound += (b + n) * 2.0 ** -28 * float(rows[:, :, 1]["d"].max())
+        assert (np.abs(out[at] - ref) <= bound).all() and (np.abs(got[at] - ref) <= bound).all()
+
+
 def test_two_calls_at_once(nat, oracle):
     """Other sequences of one cache on two streams, each call with its own workspace."""
     lens, before = [200, 90, 33, 150], [40, 0, 500, 7]
