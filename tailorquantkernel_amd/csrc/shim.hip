@@ -1492,9 +1492,7 @@ int pack_by_rows(tq_hip_kv *kv, const PackWalk &walk, bool mapped, const float *
 }
 
 // How a call's sequences are attended to; `addresses` of its arrays, or'ed.
-PackWalk pack_plan(const tq_hip_kv *kv, int n_seqs, const int32_t *seq, const int32_t *pos0, const int32_t *start,
-                   uintptr_t addresses) {
-    PackWalk walk(n_seqs, seq, pos0, start);
+void pack_plan(const tq_hip_kv *kv, uintptr_t addresses, PackWalk &walk) {
     const bool pack = pack_dense(kv, addresses);
     if (pack && use_decode3(kv)) {
         walk.long_by_rows();
@@ -1502,7 +1500,6 @@ PackWalk pack_plan(const tq_hip_kv *kv, int n_seqs, const int32_t *seq, const in
     } else if (!pack || walk.longest(walk.dense) > kMaxPackKeys) {
         walk.all_by_rows();   // (only the MFMA decode takes some of a call's rows)
     }
-    return walk;
 }
 
 // The workspace of a plan: the two forms run one after the other.
@@ -1523,8 +1520,9 @@ size_t tq_hip_prefill_packed_ws_bytes(const tq_hip_kv *kv, int n_seqs, const int
     if (!kv || n_seqs <= 0 || !start || !pack_ok(n_seqs, pos0, start)) return 0;
     try {
         // of an aligned call and of another
-        const PackWalk walk = pack_plan(kv, n_seqs, nullptr, pos0, start, 0),
-                       other = pack_plan(kv, n_seqs, nullptr, pos0, start, 4);
+        PackWalk walk(n_seqs, nullptr, pos0, start), other = walk;
+        pack_plan(kv, 0, walk);
+        pack_plan(kv, 4, other);
         if (other.longest(other.rows) > max_context(kv)) return 0;
         return std::max({(size_t)16, pack_bytes(kv, walk), pack_bytes(kv, other)});
     } catch (...) {
@@ -1561,7 +1559,8 @@ int tq_hip_prefill_packed_async(tq_hip_kv *kv, int n_seqs, const int32_t *seq, c
             for (long p = 0; p < pages; p++)
                 if (row[p] < 0) return TQ_HIP_EINVAL;
         }
-        const PackWalk walk = pack_plan(kv, n_seqs, seq, pos0, start, addresses);
+        PackWalk walk(n_seqs, seq, pos0, start);
+        pack_plan(kv, addresses, walk);
         if (std::max(walk.longest(walk.dense), walk.longest(walk.rows)) > max_context(kv)) return TQ_HIP_EINVAL;
         if (ws_bytes < pack_bytes(kv, walk)) return TQ_HIP_EINVAL;
         const OnDevice on(kv->device);
