@@ -292,7 +292,8 @@ int tq_hip_prefill_async(tq_hip_kv *kv, int seq, int pos0, int n, const float *d
  * 2^-29 of the largest V scale so far).  Sequences with few new tokens, those of
  * more than 65,536 tokens, and every sequence of other shapes, attend row by row as
  * decode steps do, with products as exact: prompts, short turns and single tokens
- * can share a call.  (A whole prompt row by row takes many times as long.)  The
+ * can share a call.  (A whole prompt row by row takes many times as long, and there,
+ * as in a decode step, values past 2^120 divided by the tokens may overflow.)  The
  * form of a sequence and the cuts of its blocks go by the cost of the whole call: its
  * precision does not depend on the others, its last bits may.  d_ws:
  * tq_hip_prefill_packed_ws_bytes for the same pos0 and start (0: a call that is
