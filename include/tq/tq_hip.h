@@ -112,6 +112,70 @@ int tq_hip_attention_head_q8(const float *q, block_q8 *q_q8, const block_q8 *k_c
                              const block_q8 *v_cache, int n, int head_dim, float *scores,
                              float *out, void *stream);
 
+/* ---- rotary positions for long contexts -----------------------------------
+ * The reference's RoPE is a host table of whole heads, halves paired, at the
+ * positions themselves (model/rope.c:4-29).  Here pair i of the rotary_dim / 2
+ * turns by f_i radians per position, f_i = theta^(-2 i / rotary_dim) but for:
+ *   LINEAR  f_i / factor
+ *   NTK     theta * factor^(rotary_dim / (rotary_dim - 2)) in place of theta
+ *   BANDS   by the turns that a pair makes over trained_len positions, t =
+ *           trained_len f_i / (2 pi): f_i / factor for t <= low, f_i for t >= high,
+ *           and s f_i + (1 - s) f_i / factor between, s = (t - low) / (high - low)
+ *   YARN    f_i (1 - r) + f_i / factor r with a ramp r over the pairs from 0 to 1
+ *           between those that make `high` and `low` turns: i(t) = rotary_dim
+ *           ln(trained_len / (2 pi t)) / (2 ln theta), from max(floor(i(high)), 0)
+ *           to min(ceil(i(low)), rotary_dim - 1); cos and sin are multiplied by
+ *           `magnitude`, or by 0.1 ln(factor) + 1 where that is 0.
+ * Angles are made in 64 bits, cos and sin rounded to fp32 once. */
+#define TQ_HIP_ROPE_HALF 0          /* pair i: values i and i + rotary_dim / 2 */
+#define TQ_HIP_ROPE_INTERLEAVED 1   /* pair i: values 2 i and 2 i + 1          */
+#define TQ_HIP_ROPE_PLAIN 0
+#define TQ_HIP_ROPE_LINEAR 1
+#define TQ_HIP_ROPE_NTK 2
+#define TQ_HIP_ROPE_BANDS 3
+#define TQ_HIP_ROPE_YARN 4
+typedef struct {
+    int rotary_dim;      /* a head's first values that turn: even, 2 .. 256 */
+    int layout;
+    int scaling;
+    int trained_len;     /* BANDS, YARN: > 0                                */
+    double theta;        /* >= 1 (YARN: > 1)                                */
+    double factor;       /* scaled: >= 1                                    */
+    double low, high;    /* BANDS: 0 <= low < high; YARN: 0 < low <= high   */
+    double magnitude;    /* YARN: >= 0                                      */
+} tq_hip_rope;
+
+/* The cos and sin rows [n][rotary_dim / 2] of positions d_pos[r] (NULL: r), for the
+ * steps, prefills and layers that take such rows (their rotary_dim is the head's,
+ * their layout HALF; the layout makes no difference to the rows): made once, for
+ * all layers.  n * rotary_dim at most 2^33.  Asynchronous on `stream`, on the current
+ * device. */
+int tq_hip_rope_rows(const tq_hip_rope *rope, int n, const int32_t *d_pos, float *d_cos, float *d_sin, void *stream);
+
+/* Heads of n rows: head h of row r at x + r * stride + h * head_dim, the rows of a
+ * fused projection too.  norm: RMSNorm's head_dim weights, or NULL for none.  The
+ * results go to out + r * out_stride + h * head_dim; out may be x (the strides
+ * agree), and otherwise overlaps no x. */
+typedef struct {
+    const float *x;
+    int heads;           /* 0 .. 65536                     */
+    size_t stride;       /* floats, at least heads * head_dim */
+    const float *norm;
+    float *out;
+    size_t out_stride;
+} tq_hip_heads;
+
+/* The q and k heads (either may be NULL) of n rows in one pass: norm_heads
+ * (model/attention_layer.c:48-53) where there are weights, x / sqrt(eps + mean x^2) *
+ * weight, and then the first rotary_dim values of each head turned to position
+ * d_pos[r] (NULL: r), the others left.  What comes out goes into steps and prefills
+ * without cos and sin.  Within fp32 rounding of the formula (the squares are summed
+ * in parallel: tq_hip_decode_step_norm_async keeps the reference's order).  head_dim
+ * a multiple of 4 up to 256, n at most 2^23; arrays 4-byte aligned.
+ * Asynchronous on `stream`, on the current device. */
+int tq_hip_norm_rope(const tq_hip_rope *rope, int head_dim, int n, const int32_t *d_pos, const tq_hip_heads *q,
+                     const tq_hip_heads *k, float eps, void *stream);
+
 /* ---- paged KV cache -------------------------------------------------------
  * Replaces tq_kv_cache_init / tq_kv_cache_free (model/kv_cache.c:17-48) for a
  * device-resident Q8 cache; the reference's flat layout becomes one sequence

@@ -107,6 +107,8 @@ _PROTOS = {
                                              _vp, _sz, _vp]),
     "tq_hip_kv_evict_ws_bytes": (_sz, [_vp, _i, _i, _i]),
     "tq_hip_kv_evict_async": (_i, [_vp, _i, _vp, _vp, _i, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp]),
+    "tq_hip_rope_rows": (_i, [_vp, _i, _vp, _vp, _vp, _vp]),
+    "tq_hip_norm_rope": (_i, [_vp, _i, _i, _vp, _vp, _vp, C.c_float, _vp]),
     "tq_hip_logits_ws_bytes": (_sz, [_i, _i]),
     "tq_hip_logits_process": (_i, [_vp, _sz, _i, _i, _vp, _vp, _sz, _vp, _vp, _sz, _vp]),
 }
@@ -185,6 +187,24 @@ class LogitsRules(C.Structure):
                 ("frequency", C.c_void_p), ("bias_ids", C.c_void_p), ("bias_vals", C.c_void_p),
                 ("bias_stride", C.c_size_t), ("bias_len", C.c_void_p), ("mask", C.c_void_p),
                 ("mask_stride", C.c_size_t)]
+
+
+# tq_hip_rope: layouts and scalings
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_BANDS, ROPE_YARN = 0, 1, 2, 3, 4
+
+
+class Rope(C.Structure):
+    """tq_hip_rope: which of a head's values turn, and how far per position."""
+    _fields_ = [("rotary_dim", C.c_int), ("layout", C.c_int), ("scaling", C.c_int), ("trained_len", C.c_int),
+                ("theta", C.c_double), ("factor", C.c_double), ("low", C.c_double), ("high", C.c_double),
+                ("magnitude", C.c_double)]
+
+
+class Heads(C.Structure):
+    """tq_hip_heads: the heads of rows on the device, their norm's weights and where they go."""
+    _fields_ = [("x", C.c_void_p), ("heads", C.c_int), ("stride", C.c_size_t), ("norm", C.c_void_p),
+                ("out", C.c_void_p), ("out_stride", C.c_size_t)]
 
 
 class DeviceBuffer:
