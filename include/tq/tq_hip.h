@@ -333,6 +333,60 @@ int tq_hip_kv_evict_async(tq_hip_kv *kv, int n, const int32_t *d_seq, const int3
                           const int32_t *d_where, float *d_total_out, int32_t *d_where_out, size_t stride, void *d_ws,
                           size_t ws_bytes, void *stream);
 
+/* ---- long contexts in part: blocks chosen by what their keys can score ------
+ * No counterpart in the reference.  A sequence's tokens lie in blocks of `block`
+ * slots, a multiple of TQ_HIP_PAGE_TOKENS up to 1024.  The caller keeps, per block and
+ * kv head, the largest and the smallest cached key (code * scale, in fp32) of each
+ * channel, as bf16 rounded outward:
+ *   bounds[((s * n_kv_heads + h) * stride + b) * 2 * head_dim + {0, head_dim} + c]
+ * for sequence s and stride blocks each.  A key that is NaN counts for nothing; a
+ * channel without one that is a number has -inf and +inf.  A token that moves
+ * (tq_hip_kv_evict_async) leaves bounds behind that hold no more: they are made again.
+ *
+ * tq_hip_kv_bounds_async makes those of the blocks that hold tokens d_from[i] (NULL: 0)
+ * .. d_len[i] - 1 of sequence d_seq[i] (NULL: sequence i), from all of a block's tokens
+ * below d_len[i]; lengths past max_len are cut to it.  Sequences outside the cache are
+ * skipped; tokens without a page count for nothing.  n at most 65535; d_bounds 16-byte
+ * aligned; head dims 32/64/128/256. */
+int tq_hip_kv_bounds_async(tq_hip_kv *kv, int n, const int32_t *d_seq, const int32_t *d_from, const int32_t *d_len,
+                           int max_len, int block, uint16_t *d_bounds, size_t stride, void *stream);
+
+/* For query i, at position d_pos[i] <= max_pos of sequence d_seq[i] (NULL: i), and each
+ * kv head, the blocks to attend to, in order, in list[(i * n_kv_heads + h) * keep + ..]:
+ * the first `sinks` blocks, the last `recent` (at least 1: the block of the query's own
+ * token is always among them, and its bounds need not be there yet), and of the others
+ * those with the largest score
+ *   sum over the group's heads g and channels c of max(q_gc M_c, q_gc m_c),
+ * M and m the block's bounds: no key of the block scores more.  Scores are in 64 bits,
+ * NaN lowest; equal ones go to the lower block.  Entries past min(keep, d_pos[i] / block
+ * + 1) are -1, all of them for a negative d_pos[i] or a sequence outside the cache.  d_q
+ * [n_q][n_q_heads * head_dim], before RoPE with d_cos / d_sin, rotated with NULL.
+ * sinks + recent at most keep; n_q at most 65535; fp32 arrays and d_bounds 16-byte
+ * aligned; head dims 32/64/128 with groups 1..8, TQ_HIP_ETYPE otherwise.  d_ws:
+ * tq_hip_kv_select_ws_bytes for the same n_q, max_pos, block and keep (0: a call that is
+ * refused), 16-byte aligned, nothing is kept in it between calls. */
+size_t tq_hip_kv_select_ws_bytes(const tq_hip_kv *kv, int n_q, int max_pos, int block, int keep);
+int tq_hip_kv_select_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq, const int32_t *d_pos, int max_pos, int block,
+                           int keep, int sinks, int recent, const float *d_q, const float *d_cos, const float *d_sin,
+                           const uint16_t *d_bounds, size_t stride, int32_t *d_list, void *d_ws, size_t ws_bytes,
+                           void *stream);
+
+/* tq_hip_decode_step_async over the listed blocks alone: for each kv head the tokens of
+ * blocks list[(i * n_kv_heads + h) * keep + j], j < min(keep, d_pos[i] / block + 1),
+ * below d_pos[i], and the new token, whose block d_pos[i] / block is the last of them.
+ * The entries are those of tq_hip_kv_select_async or the caller's own: each once, on
+ * mapped pages.  The new key also enters the bounds of its block (d_bounds NULL: none
+ * are kept), which begin with the block's first token.  A sequence appears at most once
+ * per call.  Head dims 32/64/128 with groups 1..8, TQ_HIP_ETYPE otherwise; fp32 arrays
+ * and d_bounds 16-byte aligned; keep * block at most 2^19.  d_ws:
+ * tq_hip_decode_step_blocks_ws_bytes for the same n_q, max_pos, block and keep (0: a call
+ * that is refused), 16-byte aligned, nothing is kept in it between calls. */
+size_t tq_hip_decode_step_blocks_ws_bytes(const tq_hip_kv *kv, int n_q, int max_pos, int block, int keep);
+int tq_hip_decode_step_blocks_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq, const int32_t *d_pos, int max_pos,
+                                    int block, int keep, const int32_t *d_list, const float *d_q, const float *d_k,
+                                    const float *d_v, const float *d_cos, const float *d_sin, float *d_out,
+                                    uint16_t *d_bounds, size_t stride, void *d_ws, size_t ws_bytes, void *stream);
+
 /* ---- prefill: the attention loop of attention_layer_batch
  * (model/attention_layer.c:203-204,221-236): tokens pos0..pos0+n-1 of `seq`,
  * each stored then attending causally to [0, pos0+i].  q [n][nq*hd], k/v

@@ -1124,6 +1124,47 @@ int tq_hip_attend(tq_hip_kv *kv, int seq, int pos, const float *q, const float *
     return copy_out_sync(kv, out, oo, qb, &done);
 }
 
+// What a step over a part of each sequence passes to its two launches.
+static TqDecodeArgs step_args(const tq_hip_kv *kv, int n_q, const int32_t *d_seq, const int32_t *d_pos, const float *d_q,
+                              const float *d_k, const float *d_v, const float *d_cos, const float *d_sin, float *d_out) {
+    TqDecodeArgs a{};
+    a.view = kv->view;
+    a.seq_of = d_seq;
+    a.seq_stride = 1;
+    a.len_of = d_pos;
+    a.len_plus = 1;
+    a.q = d_q;
+    a.k_new = d_k;
+    a.v_new = d_v;
+    a.cos_t = d_cos;
+    a.sin_t = d_sin;
+    a.out = d_out;
+    a.n_q = n_q;
+    a.n_q_heads = kv->desc.n_q_heads;
+    a.n_kv_heads = kv->desc.n_kv_heads;
+    a.head_dim = kv->desc.head_dim;
+    a.scale = 1.0f / sqrtf((float)kv->desc.head_dim);
+    a.contig_first = -1;
+    return a;
+}
+
+static TqMergeArgs merge_args(const TqDecodeArgs &a) {
+    TqMergeArgs m{};
+    m.pos_of = a.len_of;
+    m.base_of = a.base_of;
+    m.keep = a.list ? a.keep : 0;
+    m.block_tokens = a.block_tokens;
+    m.n_q = a.n_q;
+    m.n_q_heads = a.n_q_heads;
+    m.n_kv_heads = a.n_kv_heads;
+    m.head_dim = a.head_dim;
+    m.partials = a.partials;
+    m.n_splits = a.n_splits;
+    m.split_tokens = a.split_tokens;
+    m.out = a.out;
+    return m;
+}
+
 // ---- eviction --------------------------------------------------------------------
 
 size_t tq_hip_kv_evict_ws_bytes(const tq_hip_kv *kv, int n, int max_len, int keep) {
@@ -1167,6 +1208,144 @@ int tq_hip_kv_evict_async(tq_hip_kv *kv, int n, const int32_t *d_seq, const int3
     a.stride = stride;
     a.list = static_cast<int32_t *>(d_ws);
     return herr(tq_launch_evict(a, pick(kv, stream)));
+}
+
+// ---- long contexts in part ---------------------------------------------------------
+
+namespace {
+
+// A block size, and what a call of tokens below max_pos + 1 in them may ask for.
+bool block_ok(int block) {
+    return block >= TQ_HIP_PAGE_TOKENS && block <= 1024 && block % TQ_HIP_PAGE_TOKENS == 0;
+}
+
+size_t select_ws(const tq_hip_kv *kv, int n_q, int max_pos, int block) {
+    const int blocks = max_pos / block + 1;
+    if (tq_select_chunk(n_q, kv->desc.n_kv_heads, blocks) == 0) return 16;
+    return (size_t)n_q * kv->desc.n_kv_heads * blocks * sizeof(uint64_t);
+}
+
+// Most tokens that a step over listed blocks attends to.
+long blocks_len(int max_pos, int block, int keep) { return std::min((long)max_pos + 1, (long)keep * block); }
+
+size_t blocks_ws(const tq_hip_kv *kv, int n_q, int max_pos, int block, int keep) {
+    const tq_hip_kv_desc &D = kv->desc;
+    int split_tokens = 0, n_splits = 0;
+    plan_decode3(kv, n_q, (int)blocks_len(max_pos, block, keep), &split_tokens, &n_splits);
+    if (n_splits == 1) return 16;
+    return (size_t)n_q * D.n_kv_heads * n_splits * tq_decode3_partial_floats(D.head_dim, D.n_q_heads / D.n_kv_heads) *
+           sizeof(float);
+}
+
+}  // namespace
+
+int tq_hip_kv_bounds_async(tq_hip_kv *kv, int n, const int32_t *d_seq, const int32_t *d_from, const int32_t *d_len,
+                           int max_len, int block, uint16_t *d_bounds, size_t stride, void *stream) {
+    if (!kv || n < 0 || !block_ok(block)) return TQ_HIP_EINVAL;
+    if (n == 0) return TQ_HIP_OK;
+    if (n > 65535 || kv->desc.n_kv_heads > 65535) return TQ_HIP_EINVAL;   // grid dimensions
+    if (max_len <= 0 || max_len > (long)kv->desc.max_pages_per_seq * TQ_HIP_PAGE_TOKENS) return TQ_HIP_EINVAL;
+    if (stride < (size_t)((max_len - 1) / block + 1) || !d_len || !d_bounds || ((uintptr_t)d_bounds & 15)) return TQ_HIP_EINVAL;
+    if (((uintptr_t)d_seq | (uintptr_t)d_from | (uintptr_t)d_len) & 3) return TQ_HIP_EINVAL;
+    if (!d_seq && n > kv->desc.max_seqs) return TQ_HIP_EINVAL;
+    const OnDevice on(kv->device);
+    if (on.rc != TQ_HIP_OK) return on.rc;
+    const TqBoundsArgs a{kv->view, n, d_seq, d_from, d_len, max_len, block, d_bounds, stride};
+    return herr(tq_launch_bounds(a, pick(kv, stream)));
+}
+
+size_t tq_hip_kv_select_ws_bytes(const tq_hip_kv *kv, int n_q, int max_pos, int block, int keep) {
+    if (!kv || n_q <= 0 || n_q > 65535 || max_pos < 0 || !block_ok(block) || keep <= 0) return 0;
+    const tq_hip_kv_desc &D = kv->desc;
+    if (max_pos >= (long)D.max_pages_per_seq * TQ_HIP_PAGE_TOKENS) return 0;
+    if (!tq_decode3_supported(D.head_dim, D.n_q_heads / D.n_kv_heads)) return 0;
+    return select_ws(kv, n_q, max_pos, block);
+}
+
+int tq_hip_kv_select_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq, const int32_t *d_pos, int max_pos, int block,
+                           int keep, int sinks, int recent, const float *d_q, const float *d_cos, const float *d_sin,
+                           const uint16_t *d_bounds, size_t stride, int32_t *d_list, void *d_ws, size_t ws_bytes,
+                           void *stream) {
+    if (!kv || n_q < 0 || max_pos < 0 || !block_ok(block)) return TQ_HIP_EINVAL;
+    if (keep <= 0 || sinks < 0 || recent < 1 || recent > keep || sinks > keep - recent) return TQ_HIP_EINVAL;
+    if (n_q == 0) return TQ_HIP_OK;
+    const tq_hip_kv_desc &D = kv->desc;
+    if (n_q > 65535 || D.n_kv_heads > 65535) return TQ_HIP_EINVAL;   // grid dimensions
+    if (max_pos >= (long)D.max_pages_per_seq * TQ_HIP_PAGE_TOKENS || stride < (size_t)(max_pos / block + 1))
+        return TQ_HIP_EINVAL;
+    if (!d_pos || !d_q || !d_bounds || !d_list || !d_ws || ((d_cos == nullptr) != (d_sin == nullptr))) return TQ_HIP_EINVAL;
+    if (((uintptr_t)d_q | (uintptr_t)d_cos | (uintptr_t)d_sin | (uintptr_t)d_bounds | (uintptr_t)d_ws) & 15)
+        return TQ_HIP_EINVAL;
+    if (((uintptr_t)d_seq | (uintptr_t)d_pos | (uintptr_t)d_list) & 3) return TQ_HIP_EINVAL;
+    if (!d_seq && n_q > D.max_seqs) return TQ_HIP_EINVAL;
+    if (!tq_decode3_supported(D.head_dim, D.n_q_heads / D.n_kv_heads)) return TQ_HIP_ETYPE;
+    if (ws_bytes < select_ws(kv, n_q, max_pos, block)) return TQ_HIP_EINVAL;
+    const OnDevice on(kv->device);
+    if (on.rc != TQ_HIP_OK) return on.rc;
+    TqSelectArgs a;
+    a.view = kv->view;
+    a.n_q = n_q;
+    a.n_q_heads = D.n_q_heads;
+    a.seq_of = d_seq;
+    a.pos_of = d_pos;
+    a.max_pos = max_pos;
+    a.block = block;
+    a.keep = keep;
+    a.sinks = sinks;
+    a.recent = recent;
+    a.q = d_q;
+    a.cos_t = d_cos;
+    a.sin_t = d_sin;
+    a.bounds = d_bounds;
+    a.stride = stride;
+    a.list = d_list;
+    a.key_stride = (size_t)(max_pos / block + 1);
+    a.chunk = tq_select_chunk(n_q, D.n_kv_heads, (int)a.key_stride);
+    a.keys = static_cast<uint64_t *>(d_ws);
+    return herr(tq_launch_select(a, pick(kv, stream)));
+}
+
+size_t tq_hip_decode_step_blocks_ws_bytes(const tq_hip_kv *kv, int n_q, int max_pos, int block, int keep) {
+    if (!kv || n_q <= 0 || n_q > 65535 || max_pos < 0 || !block_ok(block) || keep <= 0) return 0;
+    if ((long)keep * block > 1L << 19 || !use_decode3(kv)) return 0;
+    return blocks_ws(kv, n_q, max_pos, block, keep);
+}
+
+int tq_hip_decode_step_blocks_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq, const int32_t *d_pos, int max_pos,
+                                    int block, int keep, const int32_t *d_list, const float *d_q, const float *d_k,
+                                    const float *d_v, const float *d_cos, const float *d_sin, float *d_out,
+                                    uint16_t *d_bounds, size_t stride, void *d_ws, size_t ws_bytes, void *stream) {
+    if (!kv || n_q < 0 || max_pos < 0 || !block_ok(block) || keep <= 0) return TQ_HIP_EINVAL;
+    if ((long)keep * block > 1L << 19) return TQ_HIP_EINVAL;
+    if (n_q == 0) return TQ_HIP_OK;
+    const tq_hip_kv_desc &D = kv->desc;
+    if (n_q > 65535 || D.n_kv_heads > 65535) return TQ_HIP_EINVAL;   // grid dimensions
+    if (!d_pos || !d_list || !d_q || !d_k || !d_v || !d_out || !d_ws || ((d_cos == nullptr) != (d_sin == nullptr)))
+        return TQ_HIP_EINVAL;
+    if (d_bounds && stride < (size_t)(max_pos / block + 1)) return TQ_HIP_EINVAL;
+    if (((uintptr_t)d_q | (uintptr_t)d_k | (uintptr_t)d_v | (uintptr_t)d_cos | (uintptr_t)d_sin | (uintptr_t)d_out |
+         (uintptr_t)d_bounds | (uintptr_t)d_ws) & 15)
+        return TQ_HIP_EINVAL;
+    if (((uintptr_t)d_seq | (uintptr_t)d_pos | (uintptr_t)d_list) & 3) return TQ_HIP_EINVAL;
+    if (!d_seq && n_q > D.max_seqs) return TQ_HIP_EINVAL;
+    if (!use_decode3(kv)) return TQ_HIP_ETYPE;
+    if (ws_bytes < blocks_ws(kv, n_q, max_pos, block, keep)) return TQ_HIP_EINVAL;
+    const OnDevice on(kv->device);
+    if (on.rc != TQ_HIP_OK) return on.rc;
+    const hipStream_t s = pick(kv, stream);
+    TqDecodeArgs a = step_args(kv, n_q, d_seq, d_pos, d_q, d_k, d_v, d_cos, d_sin, d_out);
+    const int waves = plan_decode3(kv, n_q, (int)blocks_len(max_pos, block, keep), &a.split_tokens, &a.n_splits);
+    a.list = d_list;
+    a.keep = keep;
+    a.block_tokens = block;
+    a.bounds = d_bounds;
+    a.bounds_stride = stride;
+    a.partials = static_cast<float *>(d_ws);
+    TQ_TRY(tq_launch_decode3_parts(a, waves, s));
+    if (a.n_splits == 1) return TQ_HIP_OK;
+    TqMergeArgs m = merge_args(a);
+    m.slots = a.n_splits;
+    return herr(tq_launch_decode_merge(m, s));
 }
 
 // ---- prefill ---------------------------------------------------------------------

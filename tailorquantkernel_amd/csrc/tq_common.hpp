@@ -161,6 +161,18 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
 }
 
 // ---------------------------------------------------------------------------
+// bf16 by its bits: its value, and the nearest one not below or not above x (a number
+// or an infinity).  Rounding outward commutes with max and min, so bounds that grow
+// token by token are those of all tokens at once.
+__device__ __forceinline__ float bf16_value(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+__device__ __forceinline__ uint16_t bf16_away(float x, bool away) {
+    const uint32_t u = __float_as_uint(x);
+    return (uint16_t)((u >> 16) + (away && (u & 0xFFFFu) ? 1u : 0u));
+}
+__device__ __forceinline__ uint16_t bf16_above(float x) { return bf16_away(x, x > 0.0f); }
+__device__ __forceinline__ uint16_t bf16_below(float x) { return bf16_away(x, x < 0.0f); }
+
+// ---------------------------------------------------------------------------
 // RoPE, rotate-half pairing i <-> i + hd/2 (model/rope.c:14-22):
 //   lower half: x0*c - x1*s      upper half: x0*s + x1*c
 // with x0 = x[i], x1 = x[i + hd/2], c/s from the host table.
@@ -267,6 +279,15 @@ struct TqDecodeArgs {
     float *total;
     int32_t *where;
     size_t total_stride;
+    // The step over listed blocks (tq_launch_decode3_parts only), or null.
+    const int32_t *list;     // [n_q][n_kv_heads][keep]
+    int keep;
+    int block_tokens;
+    uint16_t *bounds;        // [max_seqs][n_kv_heads][bounds_stride][2][hd], or null
+    size_t bounds_stride;
+    // The step behind a group's common tokens (tq_launch_decode3_parts only), or null.
+    const int32_t *base_of;  // [n_q]
+    int part_slots;          // partial rows of a (query, kv head), at least n_splits
 };
 
 hipError_t tq_launch_quantize(const float *x, block_q8 *out, int n, hipStream_t s);
@@ -336,6 +357,26 @@ int tq_decode3_partial_floats(int head_dim, int group);
 // waves: 4 or 8 per work-group; split_tokens a multiple of 32*waves keeps the
 // waves' tile counts equal.
 hipError_t tq_launch_decode3(const TqDecodeArgs &a, int waves, hipStream_t s);
+// A step over listed blocks, or behind common tokens: head_dim 32/64/128 (with base_of
+// 64/128).  Every split of a (query, kv head) leaves its rows' means, then m and l, in
+// partials (a step over blocks in one split its output); tq_launch_decode_merge joins them.
+hipError_t tq_launch_decode3_parts(const TqDecodeArgs &a, int waves, hipStream_t s);
+
+// out from partials [query][kv head][slots][floats as tq_decode3_partial_floats]: of a
+// query at d_pos the slots of its splits (of its tokens, of listed blocks or from
+// base_of on) and the runs_of slots from n_splits on.  A query without slots, and one
+// in front of its base, is left.
+struct TqMergeArgs {
+    const int32_t *pos_of;
+    const int32_t *base_of;  // or null: 0
+    const int32_t *runs_of;  // or null: 0
+    int keep, block_tokens;  // listed blocks, or 0
+    int n_q, n_q_heads, n_kv_heads, head_dim;
+    const float *partials;
+    int n_splits, split_tokens, slots;
+    float *out;
+};
+hipError_t tq_launch_decode_merge(const TqMergeArgs &a, hipStream_t s);
 
 // After tq_launch_decode3 with scores on the same stream: out from the splits'
 // partials, and each token's softmax weight, summed over the group's heads,
@@ -418,6 +459,42 @@ struct TqEvictArgs {
 };
 size_t tq_evict_list_ints(int max_len, int keep);
 hipError_t tq_launch_evict(const TqEvictArgs &a, hipStream_t s);
+
+// tq_hip_kv_bounds_async (sparse.hip): n at most 65535.
+struct TqBoundsArgs {
+    tq::PagedView view;
+    int n;
+    const int32_t *seq_of;   // [n], or null: sequence i
+    const int32_t *from_of;  // [n], or null: 0
+    const int32_t *len_of;   // [n]
+    int max_len;
+    int block;
+    uint16_t *bounds;        // [max_seqs][n_kv_heads][stride][2][hd]
+    size_t stride;
+};
+hipError_t tq_launch_bounds(const TqBoundsArgs &a, hipStream_t s);
+
+// tq_hip_kv_select_async (sparse.hip).
+struct TqSelectArgs {
+    tq::PagedView view;
+    int n_q, n_q_heads;
+    const int32_t *seq_of;
+    const int32_t *pos_of;
+    int max_pos;
+    int block, keep, sinks, recent;
+    const float *q;
+    const float *cos_t, *sin_t;
+    const uint16_t *bounds;
+    size_t stride;
+    int32_t *list;
+    int chunk;               // tq_select_chunk
+    uint64_t *keys;          // chunk > 0: [n_q][n_kv_heads][key_stride], at least max_pos / block + 1
+    size_t key_stride;
+};
+// Blocks that a work-group scores in a launch of its own, or 0 where the selecting
+// work-group scores them all.
+int tq_select_chunk(int n_q, int n_kv_heads, int blocks);
+hipError_t tq_launch_select(const TqSelectArgs &a, hipStream_t s);
 
 // tq_hip_prefill_packed_async's dense form (prefill_packed.hip): the sequences of one
 // launch, none of them empty, longest first.

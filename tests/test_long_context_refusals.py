@@ -69,3 +69,13 @@ def test_norm_rope_arguments(nat):
     assert f(62, 1, P) == f(0, 1, P) == f(260, 1, P) == f(64, -1, P) == f(64, 2 ** 23 + 1, P) == nat.EINVAL
     assert f(64, 1, P + 1) == f(60, 1, P) == nat.EINVAL     # more values turn than a head has
     assert lib.tq_hip_norm_rope(C.byref(r), 64, 1, P, None, None, 1e-6, None) == nat.OK
+
+
+def test_blocks_without_a_cache(nat):
+    lib = nat.load()
+    assert lib.tq_hip_kv_bounds_async(None, 1, None, None, P, 64, 16, P, 4, None) == nat.EINVAL
+    assert lib.tq_hip_kv_select_ws_bytes(None, 1, 63, 16, 4) == 0
+    assert lib.tq_hip_kv_select_async(None, 1, None, P, 63, 16, 4, 1, 1, P, P, P, P, 4, P, P, 1 << 20, None) == nat.EINVAL
+    assert lib.tq_hip_decode_step_blocks_ws_bytes(None, 1, 63, 16, 4) == 0
+    assert lib.tq_hip_decode_step_blocks_async(None, 1, None, P, 63, 16, 4, P, P, P, P, P, P, P, P, 4, P, 1 << 20,
+                                               None) == nat.EINVAL
