@@ -305,6 +305,28 @@ int tq_hip_decode_step_weights_async(tq_hip_kv *kv, int n_q, const int32_t *d_se
                                      const float *d_sin, float *d_out, const int32_t *d_at, float *d_total,
                                      int32_t *d_where, size_t stride, void *d_ws, size_t ws_bytes, void *stream);
 
+/* The same step for a batch in which groups of queries share the tokens that their
+ * sequences begin with, a system prompt or a document (no counterpart in the
+ * reference): queries start[g] .. start[g + 1] - 1 are group g, and the first
+ * prefix[g] tokens of its sequences, a multiple of TQ_HIP_PAGE_TOKENS, lie in the same
+ * pages, which are read once for the group, through the page table of its first
+ * query's sequence.  Queries before start[0] and from start[n_groups] on share
+ * nothing.  start (n_groups + 1 entries, none less than the one before, the last at
+ * most n_q) and prefix are HOST arrays, read during the call: a captured call keeps
+ * its groups, while d_seq, d_pos and the pages may change.  A query whose d_pos[i] is
+ * below its prefix is left out: nothing is appended, and its output row stays.  A
+ * sequence appears at most once per call, and its new token's page is its own.
+ * Head dims 64/128 with groups of 1..8 heads, TQ_HIP_ETYPE otherwise; fp32 arrays
+ * 16-byte aligned.  d_ws: tq_hip_decode_step_shared_ws_bytes for the same n_q,
+ * max_pos and groups (0: a call that is refused), 16-byte aligned, nothing is kept
+ * in it between calls. */
+size_t tq_hip_decode_step_shared_ws_bytes(const tq_hip_kv *kv, int n_q, int max_pos, int n_groups, const int32_t *start,
+                                          const int32_t *prefix);
+int tq_hip_decode_step_shared_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq, const int32_t *d_pos, int max_pos,
+                                    int n_groups, const int32_t *start, const int32_t *prefix, const float *d_q,
+                                    const float *d_k, const float *d_v, const float *d_cos, const float *d_sin,
+                                    float *d_out, void *d_ws, size_t ws_bytes, void *stream);
+
 /* ---- a cache of bounded size: eviction by gathered attention weight -------
  * No counterpart in the reference.  Each (sequence, kv head) has a row of
  * `stride` totals and of text positions, one per cache slot, kept by the caller:

@@ -48,7 +48,7 @@ __global__ __launch_bounds__(kThreads) void decode_merge_kernel(TqMergeArgs a) {
         const float M = wave_max(fmaxf(m[0], m[1]));
         float f[2];
 #pragma unroll
-        for (int i = 0; i < 2; i++) f[i] = m[i] == -INFINITY ? 0.0f : l[i] * __builtin_amdgcn_exp2f(m[i] - M);
+        for (int i = 0; i < 2; i++) f[i] = l[i] == 0.0f ? 0.0f : l[i] * __builtin_amdgcn_exp2f(m[i] - M);
         const float inv = 1.0f / wave_sum(f[0] + f[1]);
         wt[h][lane] = f[0] * inv;
         wt[h][lane + 64] = f[1] * inv;

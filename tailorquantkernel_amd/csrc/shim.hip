@@ -1165,6 +1165,141 @@ static TqMergeArgs merge_args(const TqDecodeArgs &a) {
     return m;
 }
 
+// ---- steps with common tokens --------------------------------------------------------
+
+namespace {
+
+// Most runs of a group's common tokens, and splits of what lies behind them: the merge
+// holds 128 slots.
+constexpr int kSharedRuns = 64;
+
+// How a step with common tokens is cut: what each group shares, in runs of `chunk` key
+// tiles, and the splits behind.
+struct SharedPlan {
+    long chunk = 1;
+    int runs = 0;            // most runs of a group
+    int waves, split_tokens, n_splits, slots;
+    size_t partials, bytes;  // of the workspace: base_of, runs_of, partials
+};
+
+// What group g shares: tokens that are worth a launch of their own.
+int shared_tokens(const int32_t *start, const int32_t *prefix, int g) {
+    return start[g + 1] - start[g] >= 2 ? prefix[g] : 0;
+}
+
+bool shared_ok(const tq_hip_kv *kv, int n_q, int max_pos, int n_groups, const int32_t *start, const int32_t *prefix) {
+    if (n_groups < 0 || (n_groups > 0 && (!start || !prefix))) return false;
+    if (n_q > 65535 || kv->desc.n_kv_heads > 65535 || max_pos >= max_context(kv)) return false;
+    if (n_groups > 0 && (start[0] < 0 || start[n_groups] > n_q)) return false;
+    for (int g = 0; g < n_groups; g++) {
+        if (start[g + 1] < start[g] || prefix[g] < 0 || prefix[g] % TQ_HIP_PAGE_TOKENS) return false;
+        if (prefix[g] > max_pos) return false;   // a token is appended behind them
+    }
+    return true;
+}
+
+void plan_shared(const tq_hip_kv *kv, int n_q, int max_pos, int n_groups, const int32_t *start, const int32_t *prefix,
+                 SharedPlan &p) {
+    const tq_hip_kv_desc &D = kv->desc;
+    const int g = D.n_q_heads / D.n_kv_heads;
+    long steps = 0;
+    int least = n_groups > 0 && start[0] == 0 && start[n_groups] == n_q ? INT32_MAX : 0, most = 0;
+    for (int i = 0; i < n_groups; i++) {
+        if (start[i + 1] == start[i]) continue;
+        const int common = shared_tokens(start, prefix, i);
+        least = std::min(least, common);
+        most = std::max(most, common);
+        steps += tq_shared_steps(start[i + 1] - start[i], g, common);
+    }
+    // two work-groups per CU
+    p.chunk = std::max(1L, (steps * D.n_kv_heads + 511) / 512);
+    const long tiles = (most + 31) / 32;
+    p.chunk = std::max(std::min(p.chunk, (long)TQ_SHARED_RUN_TILES), (tiles + kSharedRuns - 1) / kSharedRuns);
+    p.runs = most ? tq_shared_runs(most, p.chunk) : 0;
+    p.waves = plan_decode3(kv, n_q, max_pos + 1 - (least == INT32_MAX ? 0 : least), &p.split_tokens, &p.n_splits);
+    p.slots = p.n_splits + p.runs;
+    const size_t list = ((size_t)n_q * sizeof(int32_t) + 255) & ~(size_t)255;
+    p.partials = 2 * list;
+    p.bytes = p.partials + (size_t)n_q * D.n_kv_heads * p.slots * tq_decode3_partial_floats(D.head_dim, g) * sizeof(float);
+}
+
+}  // namespace
+
+size_t tq_hip_decode_step_shared_ws_bytes(const tq_hip_kv *kv, int n_q, int max_pos, int n_groups, const int32_t *start,
+                                          const int32_t *prefix) {
+    if (!kv || n_q <= 0 || max_pos < 0 || !shared_ok(kv, n_q, max_pos, n_groups, start, prefix)) return 0;
+    if (!use_decode3(kv) || !tq_shared_supported(kv->desc.head_dim, kv->desc.n_q_heads / kv->desc.n_kv_heads)) return 0;
+    SharedPlan p;
+    plan_shared(kv, n_q, max_pos, n_groups, start, prefix, p);
+    return p.bytes;
+}
+
+int tq_hip_decode_step_shared_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq, const int32_t *d_pos, int max_pos,
+                                    int n_groups, const int32_t *start, const int32_t *prefix, const float *d_q,
+                                    const float *d_k, const float *d_v, const float *d_cos, const float *d_sin,
+                                    float *d_out, void *d_ws, size_t ws_bytes, void *stream) {
+    if (!kv || n_q < 0 || max_pos < 0 || !shared_ok(kv, n_q, max_pos, n_groups, start, prefix)) return TQ_HIP_EINVAL;
+    if (n_q == 0) return TQ_HIP_OK;
+    if (!d_pos || !d_q || !d_k || !d_v || !d_out || !d_ws || ((d_cos == nullptr) != (d_sin == nullptr))) return TQ_HIP_EINVAL;
+    if (((uintptr_t)d_q | (uintptr_t)d_k | (uintptr_t)d_v | (uintptr_t)d_cos | (uintptr_t)d_sin | (uintptr_t)d_out |
+         (uintptr_t)d_ws) & 15)
+        return TQ_HIP_EINVAL;
+    if (((uintptr_t)d_seq | (uintptr_t)d_pos) & 3) return TQ_HIP_EINVAL;
+    const tq_hip_kv_desc &D = kv->desc;
+    if (!d_seq && n_q > D.max_seqs) return TQ_HIP_EINVAL;
+    if (!use_decode3(kv) || !tq_shared_supported(D.head_dim, D.n_q_heads / D.n_kv_heads)) return TQ_HIP_ETYPE;
+    SharedPlan p;
+    plan_shared(kv, n_q, max_pos, n_groups, start, prefix, p);
+    if (ws_bytes < p.bytes) return TQ_HIP_EINVAL;
+    const OnDevice on(kv->device);
+    if (on.rc != TQ_HIP_OK) return on.rc;
+    const hipStream_t s = pick(kv, stream);
+    unsigned char *ws = static_cast<unsigned char *>(d_ws);
+    TqDecodeArgs a = step_args(kv, n_q, d_seq, d_pos, d_q, d_k, d_v, d_cos, d_sin, d_out);
+    a.split_tokens = p.split_tokens;
+    a.n_splits = p.n_splits;
+    a.part_slots = p.slots;
+    a.partials = reinterpret_cast<float *>(ws + p.partials);
+    int32_t *base_of = reinterpret_cast<int32_t *>(ws), *runs_of = reinterpret_cast<int32_t *>(ws + p.partials / 2);
+    a.base_of = base_of;
+    // the common tokens, TQ_MAX_PACK groups a launch
+    TqSharedTable t;
+    TqSharedArgs c;
+    c.view = kv->view;
+    c.table = &t;
+    c.seq_of = d_seq;
+    c.q = d_q;
+    c.cos_t = d_cos;
+    c.sin_t = d_sin;
+    c.n_q_heads = D.n_q_heads;
+    c.head_dim = D.head_dim;
+    c.scale = a.scale;
+    c.partials = a.partials;
+    c.first_slot = p.n_splits;
+    c.slots = p.slots;
+    c.base_of = base_of;
+    c.runs_of = runs_of;
+    int g0 = 0;
+    do {
+        t.n_groups = std::min(TQ_MAX_PACK, n_groups - g0);
+        t.query0 = g0 == 0 ? 0 : start[g0];
+        t.query1 = g0 + t.n_groups == n_groups ? n_q : start[g0 + t.n_groups];
+        for (int i = 0; i < t.n_groups; i++) {
+            t.first[i] = start[g0 + i];
+            t.members[i] = start[g0 + i + 1] - start[g0 + i];
+            t.prefix[i] = shared_tokens(start, prefix, g0 + i);
+            t.runs[i] = t.prefix[i] ? tq_shared_runs(t.prefix[i], p.chunk) : 0;
+        }
+        TQ_TRY(tq_launch_shared(c, s));
+        g0 += t.n_groups;
+    } while (g0 < n_groups);
+    TQ_TRY(tq_launch_decode3_parts(a, p.waves, s));
+    TqMergeArgs m = merge_args(a);
+    m.runs_of = runs_of;
+    m.slots = p.slots;
+    return herr(tq_launch_decode_merge(m, s));
+}
+
 // ---- eviction --------------------------------------------------------------------
 
 size_t tq_hip_kv_evict_ws_bytes(const tq_hip_kv *kv, int n, int max_len, int keep) {

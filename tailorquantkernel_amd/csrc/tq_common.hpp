@@ -535,3 +535,35 @@ struct TqPackRows {
     size_t n_counters;
 };
 hipError_t tq_launch_pack_rows(const TqPackRows &a, const TqPackTable &t, int first, bool clear, hipStream_t s);
+
+// tq_hip_decode_step_shared_async (shared.hip): the common tokens of a launch's groups,
+// one mean per row and run in the partials' slots first_slot + run, and base_of / runs_of
+// of the queries [query0, query1) for the launches that follow.
+#define TQ_SHARED_RUN_TILES 512     // key tiles of a run at most
+struct TqSharedTable {
+    int n_groups;
+    int query0, query1;
+    int first[TQ_MAX_PACK];         // first query
+    int members[TQ_MAX_PACK];
+    int prefix[TQ_MAX_PACK];        // common tokens, 0 where the group shares nothing
+    int runs[TQ_MAX_PACK];          // runs of their key tiles
+    int item0[TQ_MAX_PACK + 1];     // filled in by the launch
+};
+struct TqSharedArgs {
+    tq::PagedView view;
+    const TqSharedTable *table;
+    const int32_t *seq_of;          // or null: query i is sequence i
+    const float *q;                 // 16-byte aligned, as cos_t and sin_t
+    const float *cos_t, *sin_t;     // or null
+    int n_q_heads;
+    int head_dim;
+    float scale;
+    float *partials;                // [n_q][n_kv_heads][slots][tq_decode3_partial_floats]
+    int first_slot, slots;
+    int32_t *base_of, *runs_of;     // [n_q]
+};
+bool tq_shared_supported(int head_dim, int group);
+// Key tiles times blocks of rows of a group, and the runs that cut its tiles in `chunk`s.
+long tq_shared_steps(int members, int group, int prefix);
+int tq_shared_runs(int prefix, long chunk);
+hipError_t tq_launch_shared(const TqSharedArgs &a, hipStream_t s);

@@ -109,6 +109,9 @@ _PROTOS = {
     "tq_hip_kv_evict_async": (_i, [_vp, _i, _vp, _vp, _i, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp]),
     "tq_hip_rope_rows": (_i, [_vp, _i, _vp, _vp, _vp, _vp]),
     "tq_hip_norm_rope": (_i, [_vp, _i, _i, _vp, _vp, _vp, C.c_float, _vp]),
+    "tq_hip_decode_step_shared_ws_bytes": (_sz, [_vp, _i, _i, _i, _vp, _vp]),
+    "tq_hip_decode_step_shared_async": (_i, [_vp, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+                                            _vp]),
     "tq_hip_kv_bounds_async": (_i, [_vp, _i, _vp, _vp, _vp, _i, _i, _vp, _sz, _vp]),
     "tq_hip_kv_select_ws_bytes": (_sz, [_vp, _i, _i, _i, _i]),
     "tq_hip_kv_select_async": (_i, [_vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _sz, _vp]),

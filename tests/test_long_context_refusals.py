@@ -79,3 +79,10 @@ def test_blocks_without_a_cache(nat):
     assert lib.tq_hip_decode_step_blocks_ws_bytes(None, 1, 63, 16, 4) == 0
     assert lib.tq_hip_decode_step_blocks_async(None, 1, None, P, 63, 16, 4, P, P, P, P, P, P, P, P, 4, P, 1 << 20,
                                                None) == nat.EINVAL
+
+
+def test_shared_without_a_cache(nat):
+    lib, start, prefix = nat.load(), (C.c_int32 * 2)(0, 4), (C.c_int32 * 1)(16)
+    a = 1, C.addressof(start), C.addressof(prefix)
+    assert lib.tq_hip_decode_step_shared_ws_bytes(None, 4, 63, *a) == 0
+    assert lib.tq_hip_decode_step_shared_async(None, 4, None, P, 63, *a, P, P, P, P, P, P, P, 1 << 20, None) == nat.EINVAL
