@@ -2,6 +2,8 @@
 // of several prompts, the step that gathers weights.
 #include "decode3.hpp"
 
+using namespace d3;
+
 bool tq_decode3_supported(int head_dim, int group) {
     const bool hd_ok = head_dim == 32 || head_dim == 64 || head_dim == 128;
     return hd_ok && group >= 1 && group <= 8;

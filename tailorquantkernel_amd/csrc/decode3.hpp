@@ -62,6 +62,7 @@
 #include "tq_common.hpp"
 
 namespace {
+namespace d3 {   // (shared.hip has names of its own for the like)
 
 using namespace tq;
 
@@ -267,41 +268,40 @@ __device__ __forceinline__ void split3_bf16(const float (&x)[8], v8bf &hi, v8bf 
 // position is one in that order; only the page ids' way to the table differs.  The
 // work-group that appends also puts the new key into its block's bounds.
 // kShared, the part of a step behind a group's common tokens: positions begin at
-// base_of[query], a whole page.
+// `base`, a whole page, and query z is z (shared.hip's work-groups run it).
 // Of these two every split leaves its rows' means with m and l (a step over blocks in
 // one split its output), and decode_merge_kernel joins them.
 // RMSNorm and completion flags are kPlain's only; kRows appends nothing and takes its
 // pages from the table, as kBlocks and kShared do; these and kScores always append.
 constexpr int kPlain = 0, kRows = 1, kScores = 2, kBlocks = 3, kShared = 4;
+// split, kvh, z: the grid's place; base: kShared's; sm and the slots: the work-group's shared memory (two
+// tile slots per wave, separate objects so that the wait for one slot's copies does not
+// wait for the other's).
 template <int HD, int G, int W, int MODE>
-__global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
+__device__ __forceinline__ void decode3_run(const TqDecodeArgs &a, const int split, const int kvh, const int z,
+                                            Smem3<HD, G> &sm, unsigned char (&slot0)[W][L3<HD, G>::TILE],
+                                            unsigned char (&slot1)[W][L3<HD, G>::TILE], const int base = 0) {
     using L = L3<HD, G>;
     constexpr int kWaves = W;
     constexpr int kThreads = 64 * W;
     constexpr int NB = L::NB, ROW = L::ROW, NT = L::NT, CT = L::CT, CPL = L::CPL;
-    __shared__ __align__(16) Smem3<HD, G> sm;
-    // two tile slots per wave, separate objects so the wait for one slot's
-    // copies does not wait for the other's
-    __shared__ __align__(16) unsigned char slot0[kWaves][L::TILE];
-    __shared__ __align__(16) unsigned char slot1[kWaves][L::TILE];
 
     const int tid = threadIdx.x;
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lg = lane >> 4, l16 = lane & 15;
-    const int split = blockIdx.x, kvh = blockIdx.y;
     // The query this work-group serves.  A ragged batch goes longest first:
     // grid z is the rank of the query's length (ties by index), so the
     // work-groups of the longest sequences are dispatched first and the
     // short ones fill the gaps at the end (longest-processing-time order).
     // Each query's result does not depend on the order.
-    int qi = blockIdx.z;
+    int qi = z;
     // (the query's raw length and sequence, when the ranking below reads them)
     bool ranked = false;
     int len_rk = 0, seq_rk = 0;
-    if (a.n_q > 1) {
+    if (MODE != kShared && a.n_q > 1) {
         if (!a.len_of) {
-            qi = a.n_q - 1 - (int)blockIdx.z;   // query i attends pos0 + i + 1 keys
+            qi = a.n_q - 1 - z;   // query i attends pos0 + i + 1 keys
         } else if (a.n_q <= kSortQ) {
             // the batch's lengths (and sequences) through LDS, ranked by one
             // thread per query; the chosen query's length and sequence are
@@ -309,7 +309,7 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
             // both loads issued before either is waited for (a missing
             // sequence array reads the lengths again and stores 0)
             for (int i = tid; i < a.n_q; i += kThreads) {
-                const int li = MODE == kShared ? a.len_of[i] - a.base_of[i] : a.len_of[i];
+                const int li = a.len_of[i];
                 const int si = (a.seq_of ? a.seq_of : a.len_of)[i];
                 sm.qlen[i] = li;
                 sm.qseq[i] = a.seq_of ? si : 0;
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
                     const int lu = sm.qlen[u];
                     r += (lu > li) || (lu == li && u < i);
                 }
-                if (r == (int)blockIdx.z) sm.qsel = i;
+                if (r == z) sm.qsel = i;
             }
             __syncthreads();
             qi = sm.qsel;
@@ -346,7 +346,6 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
     // address when absent), used only after the copies below are issued, so
     // the copies do not wait for them.
     const int len_raw = ranked ? len_rk : *(a.len_of ? a.len_of + qi : reinterpret_cast<const int32_t *>(a.q));
-    const int base = MODE == kShared ? a.base_of[qi] : 0;
     const int seq_raw = ranked ? seq_rk : *(a.seq_of ? a.seq_of + qi : reinterpret_cast<const int32_t *>(a.q));
 
     // ---- 1. this wave's copy of the inputs it quantizes, into the tail-free
@@ -442,7 +441,7 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
     }
     __builtin_amdgcn_sched_barrier(0);
     int len = a.len_of ? len_raw + a.len_plus : a.pos0 + qi + 1;
-    if (MODE == kShared && !ranked) len -= base;
+    if (MODE == kShared) len -= base;
     [[maybe_unused]] const int at_new = len - 1;   // kBlocks: the new token's slot
     if (MODE == kBlocks && len > 0) {
         const int block = at_new / a.block_tokens;
@@ -1075,6 +1074,14 @@ __global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
     if (MODE == kPlain && a.done) signal_done();
 }
 
+template <int HD, int G, int W, int MODE>
+__global__ __launch_bounds__(64 * W) void decode3_kernel(TqDecodeArgs a) {
+    __shared__ __align__(16) Smem3<HD, G> sm;
+    __shared__ __align__(16) unsigned char slot0[W][L3<HD, G>::TILE];
+    __shared__ __align__(16) unsigned char slot1[W][L3<HD, G>::TILE];
+    decode3_run<HD, G, W, MODE>(a, blockIdx.x, blockIdx.y, blockIdx.z, sm, slot0, slot1);
+}
+
 template <int HD, int G, int MODE>
 hipError_t launch3_hd_g(const TqDecodeArgs &a, int waves, hipStream_t s) {
     const dim3 grid(a.n_splits, a.n_kv_heads, a.n_q);
@@ -1100,4 +1107,5 @@ hipError_t launch3_hd(const TqDecodeArgs &a, int g, int waves, hipStream_t s) {
     }
 }
 
+}  // namespace d3
 }  // namespace

@@ -46,10 +46,11 @@ struct Img {
 // The key in register i of lane half h of a 32 x 32 product.
 __host__ __device__ constexpr int key_of(int h, int i) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
-// x = hi + lo in fp16, four pairs.
-__device__ __forceinline__ void split_f16(const float (&x)[8], u32x4 &hi, u32x4 &lo) {
+// x = hi + lo in fp16, in pairs (hi and lo: N / 2 words).
+template <int N, class W>
+__device__ __forceinline__ void split_f16(const float (&x)[N], W &hi, W &lo) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < N / 2; i++) {
         const v2h v = {(_Float16)x[2 * i], (_Float16)x[2 * i + 1]};
         uint32_t h = __builtin_bit_cast(uint32_t, v);
         // lo is taken from the stored bits: left to see through them, the compiler

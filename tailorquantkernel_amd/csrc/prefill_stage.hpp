@@ -33,6 +33,17 @@ __device__ __forceinline__ void dma16(const void *src, unsigned char *dst) {
         : "v"(src), "s"(lds));
 }
 
+// The same copy from a scalar base address plus each lane's 32-bit offset.
+__device__ __forceinline__ void dma16s(const unsigned char *base, uint32_t off, unsigned char *dst) {
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8 *)dst;
+    uint32_t saved;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "v"(off), "s"(base), "s"(lds));
+}
+
 // Wait until at most N vector memory operations of this wave are outstanding
 // (the copies above are counted in issue order).
 template <int N>

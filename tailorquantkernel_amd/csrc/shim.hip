@@ -1151,7 +1151,6 @@ static TqDecodeArgs step_args(const tq_hip_kv *kv, int n_q, const int32_t *d_seq
 static TqMergeArgs merge_args(const TqDecodeArgs &a) {
     TqMergeArgs m{};
     m.pos_of = a.len_of;
-    m.base_of = a.base_of;
     m.keep = a.list ? a.keep : 0;
     m.block_tokens = a.block_tokens;
     m.n_q = a.n_q;
@@ -1178,7 +1177,7 @@ constexpr int kSharedRuns = 64;
 struct SharedPlan {
     long chunk = 1;
     int runs = 0;            // most runs of a group
-    int waves, split_tokens, n_splits, slots;
+    int split_tokens, n_splits, slots;
     size_t partials, bytes;  // of the workspace: base_of, runs_of, partials
 };
 
@@ -1211,12 +1210,16 @@ void plan_shared(const tq_hip_kv *kv, int n_q, int max_pos, int n_groups, const 
         most = std::max(most, common);
         steps += tq_shared_steps(start[i + 1] - start[i], g, common);
     }
-    // two work-groups per CU
-    p.chunk = std::max(1L, (steps * D.n_kv_heads + 511) / 512);
+    // one work-group per CU, the queries' own beside it, where the tiles are few: each
+    // writes its rows' means, and two a CU are slowed by one another (64 queries of 32 / 8
+    // heads, 128 and their own up to 512 tokens: behind 1,024 common ones 36.7 us and 45.2
+    // with two, 4,096 43 and 53; behind 16,384 94 and 92)
+    const long all = steps * D.n_kv_heads, wgs = all <= 40 * 256 ? 256 : 512;
+    p.chunk = std::max(1L, (all + wgs - 1) / wgs);
     const long tiles = (most + 31) / 32;
     p.chunk = std::max(std::min(p.chunk, (long)TQ_SHARED_RUN_TILES), (tiles + kSharedRuns - 1) / kSharedRuns);
     p.runs = most ? tq_shared_runs(most, p.chunk) : 0;
-    p.waves = plan_decode3(kv, n_q, max_pos + 1 - (least == INT32_MAX ? 0 : least), &p.split_tokens, &p.n_splits);
+    plan_splits3(kv, n_q, max_pos + 1 - (least == INT32_MAX ? 0 : least), kSharedWaves, &p.split_tokens, &p.n_splits);
     p.slots = p.n_splits + p.runs;
     const size_t list = ((size_t)n_q * sizeof(int32_t) + 255) & ~(size_t)255;
     p.partials = 2 * list;
@@ -1261,24 +1264,7 @@ int tq_hip_decode_step_shared_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq
     a.part_slots = p.slots;
     a.partials = reinterpret_cast<float *>(ws + p.partials);
     int32_t *base_of = reinterpret_cast<int32_t *>(ws), *runs_of = reinterpret_cast<int32_t *>(ws + p.partials / 2);
-    a.base_of = base_of;
-    // the common tokens, TQ_MAX_PACK groups a launch
-    TqSharedTable t;
-    TqSharedArgs c;
-    c.view = kv->view;
-    c.table = &t;
-    c.seq_of = d_seq;
-    c.q = d_q;
-    c.cos_t = d_cos;
-    c.sin_t = d_sin;
-    c.n_q_heads = D.n_q_heads;
-    c.head_dim = D.head_dim;
-    c.scale = a.scale;
-    c.partials = a.partials;
-    c.first_slot = p.n_splits;
-    c.slots = p.slots;
-    c.base_of = base_of;
-    c.runs_of = runs_of;
+    TqSharedTable t;   // TQ_MAX_PACK groups a launch
     int g0 = 0;
     do {
         t.n_groups = std::min(TQ_MAX_PACK, n_groups - g0);
@@ -1290,11 +1276,11 @@ int tq_hip_decode_step_shared_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq
             t.prefix[i] = shared_tokens(start, prefix, g0 + i);
             t.runs[i] = t.prefix[i] ? tq_shared_runs(t.prefix[i], p.chunk) : 0;
         }
-        TQ_TRY(tq_launch_shared(c, s));
+        TQ_TRY(tq_launch_shared(t, a, base_of, runs_of, s));
         g0 += t.n_groups;
     } while (g0 < n_groups);
-    TQ_TRY(tq_launch_decode3_parts(a, p.waves, s));
     TqMergeArgs m = merge_args(a);
+    m.base_of = base_of;
     m.runs_of = runs_of;
     m.slots = p.slots;
     return herr(tq_launch_decode_merge(m, s));
@@ -1476,7 +1462,7 @@ int tq_hip_decode_step_blocks_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq
     a.bounds = d_bounds;
     a.bounds_stride = stride;
     a.partials = static_cast<float *>(d_ws);
-    TQ_TRY(tq_launch_decode3_parts(a, waves, s));
+    TQ_TRY(tq_launch_decode3_blocks(a, waves, s));
     if (a.n_splits == 1) return TQ_HIP_OK;
     TqMergeArgs m = merge_args(a);
     m.slots = a.n_splits;

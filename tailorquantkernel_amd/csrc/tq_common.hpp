@@ -279,15 +279,14 @@ struct TqDecodeArgs {
     float *total;
     int32_t *where;
     size_t total_stride;
-    // The step over listed blocks (tq_launch_decode3_parts only), or null.
+    // The step over listed blocks (tq_launch_decode3_blocks only), or null.
     const int32_t *list;     // [n_q][n_kv_heads][keep]
     int keep;
     int block_tokens;
     uint16_t *bounds;        // [max_seqs][n_kv_heads][bounds_stride][2][hd], or null
     size_t bounds_stride;
-    // The step behind a group's common tokens (tq_launch_decode3_parts only), or null.
-    const int32_t *base_of;  // [n_q]
-    int part_slots;          // partial rows of a (query, kv head), at least n_splits
+    int part_slots;          // the step behind common tokens (shared.hip): partial rows of a
+                             // (query, kv head), at least n_splits
 };
 
 hipError_t tq_launch_quantize(const float *x, block_q8 *out, int n, hipStream_t s);
@@ -357,10 +356,9 @@ int tq_decode3_partial_floats(int head_dim, int group);
 // waves: 4 or 8 per work-group; split_tokens a multiple of 32*waves keeps the
 // waves' tile counts equal.
 hipError_t tq_launch_decode3(const TqDecodeArgs &a, int waves, hipStream_t s);
-// A step over listed blocks, or behind common tokens: head_dim 32/64/128 (with base_of
-// 64/128).  Every split of a (query, kv head) leaves its rows' means, then m and l, in
-// partials (a step over blocks in one split its output); tq_launch_decode_merge joins them.
-hipError_t tq_launch_decode3_parts(const TqDecodeArgs &a, int waves, hipStream_t s);
+// A step over listed blocks: in one split it leaves its output, of several each its rows'
+// means, then m and l, in partials for tq_launch_decode_merge.
+hipError_t tq_launch_decode3_blocks(const TqDecodeArgs &a, int waves, hipStream_t s);
 
 // out from partials [query][kv head][slots][floats as tq_decode3_partial_floats]: of a
 // query at d_pos the slots of its splits (of its tokens, of listed blocks or from
@@ -536,9 +534,10 @@ struct TqPackRows {
 };
 hipError_t tq_launch_pack_rows(const TqPackRows &a, const TqPackTable &t, int first, bool clear, hipStream_t s);
 
-// tq_hip_decode_step_shared_async (shared.hip): the common tokens of a launch's groups,
-// one mean per row and run in the partials' slots first_slot + run, and base_of / runs_of
-// of the queries [query0, query1) for the launches that follow.
+// tq_hip_decode_step_shared_async (shared.hip): groups of a launch and the queries
+// [query0, query1) whose steps behind the common tokens it makes.  Every split and run
+// leaves its rows' means, then m and l, in the step's partials: splits in the first
+// n_splits slots, runs from there on; base_of and runs_of go to tq_launch_decode_merge.
 #define TQ_SHARED_RUN_TILES 512     // key tiles of a run at most
 struct TqSharedTable {
     int n_groups;
@@ -546,24 +545,14 @@ struct TqSharedTable {
     int first[TQ_MAX_PACK];         // first query
     int members[TQ_MAX_PACK];
     int prefix[TQ_MAX_PACK];        // common tokens, 0 where the group shares nothing
-    int runs[TQ_MAX_PACK];          // runs of their key tiles
+    int runs[TQ_MAX_PACK];          // runs of their key tiles, at most as many
     int item0[TQ_MAX_PACK + 1];     // filled in by the launch
-};
-struct TqSharedArgs {
-    tq::PagedView view;
-    const TqSharedTable *table;
-    const int32_t *seq_of;          // or null: query i is sequence i
-    const float *q;                 // 16-byte aligned, as cos_t and sin_t
-    const float *cos_t, *sin_t;     // or null
-    int n_q_heads;
-    int head_dim;
-    float scale;
-    float *partials;                // [n_q][n_kv_heads][slots][tq_decode3_partial_floats]
-    int first_slot, slots;
-    int32_t *base_of, *runs_of;     // [n_q]
 };
 bool tq_shared_supported(int head_dim, int group);
 // Key tiles times blocks of rows of a group, and the runs that cut its tiles in `chunk`s.
 long tq_shared_steps(int members, int group, int prefix);
 int tq_shared_runs(int prefix, long chunk);
-hipError_t tq_launch_shared(const TqSharedArgs &a, hipStream_t s);
+// Waves of a work-group: the splits' units (plan_splits3).
+constexpr int kSharedWaves = 4;
+hipError_t tq_launch_shared(const TqSharedTable &t, const TqDecodeArgs &step, int32_t *base_of, int32_t *runs_of,
+                            hipStream_t s);
