@@ -16,11 +16,14 @@
 //   w % (hd / 4) of every (256 / hd)-th row and that dword's scale, the rows' lanes are
 //   joined at the end.  Bound by reading the keys.
 // score_kernel: eight lanes per block, 16 bytes of bounds each at a time (whole lines),
-//   scores as order-preserving 64-bit keys.
+//   scores as order-preserving 64-bit keys.  Bound by the conversions to 64 bits, as many
+//   as products and four times as slow: 16 x 8 heads over 512 blocks in 6.5 us of the
+//   kernel's 11.7 (33.6 MB), and by reading the bounds over more of them (16 x 8 over
+//   4,096 blocks, 268 MB in 69 us).  Reading four blocks ahead changed nothing.
 // select_kernel, one work-group per (query, kv head): the keep-th largest key by
 //   counting into bins over the range that the keys have, again within the bin at the
 //   edge until it is settled; then ranks in order by ballots, each wave on one run of
-//   blocks.
+//   blocks.  It scores the blocks itself where that fills the card (tq_select_chunk).
 #include <algorithm>
 
 #include "tq_common.hpp"
@@ -95,6 +98,8 @@ __global__ __launch_bounds__(kThreads) void bounds_kernel(TqBoundsArgs a) {
     }
 }
 
+constexpr int kMaxGroup = 8;
+
 // ---- scores --------------------------------------------------------------------
 
 // Order-preserving code of a score, at least 1 (NaN).
@@ -119,22 +124,31 @@ struct Sums {
     double up[P][8], down[P][8];
 };
 
+// What a work-group makes them from: the group's rotated rows, then the sums.
 template <int HD>
-__device__ __forceinline__ void load_sums(const TqSelectArgs &a, int qi, int kvh, double (&s_up)[HD],
-                                          double (&s_down)[HD], Sums<HD> &q) {
+struct SumsLds {
+    float x[kMaxGroup][HD];
+    double up[HD], down[HD];
+};
+
+template <int HD>
+__device__ __forceinline__ void load_sums(const TqSelectArgs &a, int qi, int kvh, SumsLds<HD> &lds, Sums<HD> &q) {
     const int g = a.n_q_heads / a.view.n_kv_heads;
+    const float *cs = a.cos_t ? a.cos_t + (size_t)qi * (HD / 2) : nullptr;
+    const float *sn = a.cos_t ? a.sin_t + (size_t)qi * (HD / 2) : nullptr;
+    const float *rows = a.q + ((size_t)qi * a.n_q_heads + (size_t)kvh * g) * HD;
+    for (int i = threadIdx.x; i < g * HD; i += blockDim.x) lds.x[i / HD][i % HD] = rope_elem(rows + i / HD * HD, i % HD, HD, cs, sn);
+    __syncthreads();
     for (int c = threadIdx.x; c < HD; c += blockDim.x) {
-        const float *cs = a.cos_t ? a.cos_t + (size_t)qi * (HD / 2) : nullptr;
-        const float *sn = a.cos_t ? a.sin_t + (size_t)qi * (HD / 2) : nullptr;
         double up = 0.0, down = 0.0;
         for (int h = 0; h < g; h++) {
-            const float x = rope_elem(a.q + ((size_t)qi * a.n_q_heads + (size_t)kvh * g + h) * HD, c, HD, cs, sn);
+            const float x = lds.x[h][c];
             // (a NaN goes into both: every score of the query is NaN)
             up += x <= 0.0f ? 0.0 : (double)x;
             down += x >= 0.0f ? 0.0 : (double)x;
         }
-        s_up[c] = up;
-        s_down[c] = down;
+        lds.up[c] = up;
+        lds.down[c] = down;
     }
     __syncthreads();
     const int l = threadIdx.x % 8;
@@ -143,39 +157,43 @@ __device__ __forceinline__ void load_sums(const TqSelectArgs &a, int qi, int kvh
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int c = 64 * p + 8 * l + j;
-            q.up[p][j] = c < HD ? s_up[min(c, HD - 1)] : 0.0;
-            q.down[p][j] = c < HD ? s_down[min(c, HD - 1)] : 0.0;
+            q.up[p][j] = c < HD ? lds.up[min(c, HD - 1)] : 0.0;
+            q.down[p][j] = c < HD ? lds.down[min(c, HD - 1)] : 0.0;
         }
 }
 
-// Blocks b0 + lane / 8 of a head's bounds: the score, the same in a block's eight lanes.
+// A block's bounds, this lane's share.
 template <int HD>
-__device__ __forceinline__ double score(const uint16_t *bounds, int b, const Sums<HD> &q) {
-    constexpr int P = Sums<HD>::P;
-    const int l = threadIdx.x % 8;
-    const uint16_t *at = bounds + (size_t)b * 2 * HD + 8 * (HD < 64 ? l & 3 : l);
+struct Share {
+    static constexpr int P = Sums<HD>::P;
     u32x4 hi[P], lo[P];
+    __device__ __forceinline__ void read(const uint16_t *bounds, int b) {
+        const int l = threadIdx.x % 8;
+        const uint16_t *at = bounds + (size_t)b * 2 * HD + 8 * (HD < 64 ? l & 3 : l);
 #pragma unroll
-    for (int p = 0; p < P; p++) {
-        hi[p] = *reinterpret_cast<const u32x4 *>(at + 64 * p);
-        lo[p] = *reinterpret_cast<const u32x4 *>(at + HD + 64 * p);
-    }
-    double s[2] = {0.0, 0.0};
-#pragma unroll
-    for (int p = 0; p < P; p++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint32_t h = hi[p][j / 2], w = lo[p][j / 2];
-            s[0] = fma((double)__uint_as_float(j & 1 ? h & 0xFFFF0000u : h << 16), q.up[p][j], s[0]);
-            s[1] = fma((double)__uint_as_float(j & 1 ? w & 0xFFFF0000u : w << 16), q.down[p][j], s[1]);
+        for (int p = 0; p < P; p++) {
+            hi[p] = *reinterpret_cast<const u32x4 *>(at + 64 * p);
+            lo[p] = *reinterpret_cast<const u32x4 *>(at + HD + 64 * p);
         }
-    double sum = s[0] + s[1];
-    if (HD < 64 && l >= 4) sum = 0.0;
-    sum += dpp_d<kDppQuadXor1>(sum);
-    sum += dpp_d<kDppQuadXor2>(sum);
-    sum += dpp_d<kDppRowHalfMirror>(sum);
-    return sum;
-}
+    }
+    // the score, the same in a block's eight lanes
+    __device__ __forceinline__ double score(const Sums<HD> &q) const {
+        double s[2] = {0.0, 0.0};
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const uint32_t h = hi[p][j / 2], w = lo[p][j / 2];
+                s[0] = fma((double)__uint_as_float(j & 1 ? h & 0xFFFF0000u : h << 16), q.up[p][j], s[0]);
+                s[1] = fma((double)__uint_as_float(j & 1 ? w & 0xFFFF0000u : w << 16), q.down[p][j], s[1]);
+            }
+        double sum = s[0] + s[1];
+        if (HD < 64 && threadIdx.x % 8 >= 4) sum = 0.0;
+        sum += dpp_d<kDppQuadXor1>(sum);
+        sum += dpp_d<kDppQuadXor2>(sum);
+        return sum + dpp_d<kDppRowHalfMirror>(sum);
+    }
+};
 
 // What the rules make of a query: its blocks, and whether there is a choice to make.
 struct Choice {
@@ -191,30 +209,38 @@ __device__ __forceinline__ Choice choice_of(const TqSelectArgs &a, int qi) {
     return c;
 }
 
-// Scores of the candidates (neither among the first `sinks` nor the last `recent`) into
-// keys, for `threads` threads from `first` on.
+// Keys of the blocks [begin, end) of a sequence's head, four blocks' bounds of each eight
+// lanes in flight at once.
 template <int HD>
-__device__ __forceinline__ void score_blocks(const TqSelectArgs &a, const Choice &c, int kvh, const Sums<HD> &q, int begin,
-                                             int end, uint64_t *keys) {
-    const uint16_t *bounds = a.bounds + ((size_t)c.seq * a.view.n_kv_heads + kvh) * a.stride * 2 * HD;
+__device__ __forceinline__ void score_blocks(const TqSelectArgs &a, int seq, int kvh, const Sums<HD> &q, int begin, int end,
+                                             uint64_t *keys) {
+    constexpr int A = 4;
+    const uint16_t *bounds = a.bounds + ((size_t)seq * a.view.n_kv_heads + kvh) * a.stride * 2 * HD;
     const int groups = blockDim.x / 8;
-    for (int b = begin + (int)threadIdx.x / 8; b < end; b += groups) {
-        const double s = score<HD>(bounds, b, q);
-        if (threadIdx.x % 8 == 0) keys[b] = score_key(s);
+    for (int b0 = begin + (int)threadIdx.x / 8; b0 < end; b0 += A * groups) {
+        Share<HD> s[A];
+#pragma unroll
+        for (int i = 0; i < A; i++) s[i].read(bounds, min(b0 + i * groups, end - 1));
+#pragma unroll
+        for (int i = 0; i < A; i++) {
+            const int b = b0 + i * groups;
+            const double x = s[i].score(q);
+            if (threadIdx.x % 8 == 0 && b < end) keys[b] = score_key(x);
+        }
     }
 }
 
 // Grid (chunk, kv head, query): keys of a chunk of blocks into the workspace.
 template <int HD>
 __global__ __launch_bounds__(kThreads) void score_kernel(TqSelectArgs a, int chunk) {
-    __shared__ double up[HD], down[HD];
+    __shared__ SumsLds<HD> sums;
     const int kvh = blockIdx.y, qi = blockIdx.z;
     const Choice c = choice_of(a, qi);
     const int begin = max((int)blockIdx.x * chunk, a.sinks), end = min(((int)blockIdx.x + 1) * chunk, c.count - a.recent);
     if (c.all || begin >= end) return;
     Sums<HD> q;
-    load_sums<HD>(a, qi, kvh, up, down, q);
-    score_blocks<HD>(a, c, kvh, q, begin, end, a.keys + ((size_t)qi * a.view.n_kv_heads + kvh) * a.key_stride);
+    load_sums<HD>(a, qi, kvh, sums, q);
+    score_blocks<HD>(a, c.seq, kvh, q, begin, end, a.keys + ((size_t)qi * a.view.n_kv_heads + kvh) * a.key_stride);
 }
 
 // ---- selection -----------------------------------------------------------------
@@ -222,15 +248,13 @@ __global__ __launch_bounds__(kThreads) void score_kernel(TqSelectArgs a, int chu
 constexpr int kBins = 2048;
 constexpr int kKeysInLds = 4096;
 
-// (HIP's min and max take two widths of 64-bit integers by way of another type)
-__device__ __forceinline__ uint64_t least(uint64_t x, uint64_t y) { return x < y ? x : y; }
-__device__ __forceinline__ uint64_t most(uint64_t x, uint64_t y) { return x > y ? x : y; }
-__device__ __forceinline__ uint64_t wave_max64(uint64_t x) {
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        x = most(x, (uint64_t)__shfl_xor((unsigned long long)x, o));
-    }
-    return x;
+__device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
+    x = max(x, dpp_u<kDppQuadXor1>(x));
+    x = max(x, dpp_u<kDppQuadXor2>(x));
+    x = max(x, dpp_u<kDppRowHalfMirror>(x));
+    x = max(x, dpp_u<kDppRowMirror>(x));
+    auto at = [&](int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)x, lane); };
+    return max(max(at(0), at(16)), max(at(32), at(48)));
 }
 __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
     // row_shr 1, 2, 4, 8 within the rows of 16, then the rows before
@@ -250,15 +274,19 @@ template <int HD, int WAVES, bool SCORED>
 __global__ __launch_bounds__(64 * WAVES) void select_kernel(TqSelectArgs a) {
     constexpr int THREADS = 64 * WAVES, BPT = kBins / THREADS;
     __shared__ uint64_t lds_keys[SCORED ? 1 : kKeysInLds];
-    __shared__ double up[SCORED ? 1 : HD], down[SCORED ? 1 : HD];
+    __shared__ SumsLds<SCORED ? 32 : HD> sums;
     __shared__ uint32_t hist[kBins];
-    __shared__ uint64_t w_lo[WAVES], w_hi[WAVES];
+    __shared__ uint32_t w_lo[WAVES], w_hi[WAVES];
     __shared__ uint32_t w_n[WAVES], w_m[WAVES];
     __shared__ uint32_t pick[3];             // the chosen bin, the keys wanted in it, the keys it has
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kvh = blockIdx.x, qi = blockIdx.y;
     const size_t pair = (size_t)qi * a.view.n_kv_heads + kvh;
     int32_t *list = a.list + pair * a.keep;
+    // (the sums wait for nothing; where every block is chosen they are made for nothing)
+    constexpr int H = SCORED ? 32 : HD;
+    Sums<H> q;
+    if constexpr (!SCORED) load_sums<HD>(a, qi, kvh, sums, q);
     const Choice c = choice_of(a, qi);
     if (c.all) {
         for (int j = tid; j < a.keep; j += THREADS) list[j] = j < c.count ? j : -1;
@@ -269,9 +297,7 @@ __global__ __launch_bounds__(64 * WAVES) void select_kernel(TqSelectArgs a) {
     if constexpr (SCORED) {
         keys = a.keys + pair * a.key_stride;
     } else {
-        Sums<HD> q;
-        load_sums<HD>(a, qi, kvh, up, down, q);
-        score_blocks<HD>(a, c, kvh, q, begin, end, lds_keys);
+        score_blocks<HD>(a, c.seq, kvh, q, begin, end, lds_keys);
         keys = lds_keys;
         __syncthreads();
     }
@@ -284,24 +310,25 @@ __global__ __launch_bounds__(64 * WAVES) void select_kernel(TqSelectArgs a) {
             f(b0, b < end ? keys[b] : 0ull);
         }
     };
-    uint64_t lo = ~0ull, hi = 0;
+    // the range of the keys' upper halves
+    uint32_t lo32 = 0xFFFFFFFFu, hi32 = 0;
     each([&](int, uint64_t k) {
-        lo = least(lo, k - 1);               // (none: the largest)
-        hi = most(hi, k);
+        lo32 = min(lo32, k == 0 ? 0xFFFFFFFFu : (uint32_t)(k >> 32));
+        hi32 = max(hi32, (uint32_t)(k >> 32));
     });
-    lo = ~wave_max64(~lo);
-    hi = wave_max64(hi);
+    lo32 = ~wave_umax(~lo32);
+    hi32 = wave_umax(hi32);
     if (lane == 0) {
-        w_lo[wave] = lo;
-        w_hi[wave] = hi;
+        w_lo[wave] = lo32;
+        w_hi[wave] = hi32;
     }
     __syncthreads();
 #pragma unroll
     for (int v = 0; v < WAVES; v++) {
-        lo = least(lo, w_lo[v]);
-        hi = most(hi, w_hi[v]);
+        lo32 = min(lo32, w_lo[v]);
+        hi32 = max(hi32, w_hi[v]);
     }
-    lo += 1;
+    uint64_t lo = (uint64_t)lo32 << 32, hi = (uint64_t)hi32 << 32 | 0xFFFFFFFFu;
     // the edge: the want-th largest key, of whose ties `want` are chosen at last
     uint32_t want = (uint32_t)(a.keep - a.sinks - a.recent);
     bool all_ties = want == 0;
@@ -309,7 +336,7 @@ __global__ __launch_bounds__(64 * WAVES) void select_kernel(TqSelectArgs a) {
         lo = ~0ull;                          // above every key
     } else {
 #pragma unroll 1
-        while (lo != hi) {                   // at most six rounds of 11 bits
+        for (int round = 0; round < 6 && lo != hi; round++) {   // 11 bits each
             const int bits = 64 - __clzll((long long)(hi - lo));
             const int shift = bits > 11 ? bits - 11 : 0;
             for (int b = tid; b < kBins; b += THREADS) hist[b] = 0;
@@ -343,7 +370,8 @@ __global__ __launch_bounds__(64 * WAVES) void select_kernel(TqSelectArgs a) {
             }
             __syncthreads();
             lo += (uint64_t)pick[0] << shift;
-            hi = least(hi, lo + (((uint64_t)1 << shift) - 1));
+            const uint64_t span = ((uint64_t)1 << shift) - 1;
+            if (hi - lo > span) hi = lo + span;   // (not the least of both: lo + span may pass 2^64)
             want = pick[1];
             if (want == pick[2]) {           // all of the bin are chosen
                 all_ties = true;
@@ -393,7 +421,7 @@ template <int HD>
 hipError_t launch_select(const TqSelectArgs &a, hipStream_t s) {
     const dim3 grid((unsigned)a.view.n_kv_heads, (unsigned)a.n_q);
     if (a.chunk == 0) {
-        hipLaunchKernelGGL((select_kernel<HD, 16, false>), grid, dim3(1024), 0, s, a);
+        hipLaunchKernelGGL((select_kernel<HD, 8, false>), grid, dim3(512), 0, s, a);
         return hipGetLastError();
     }
     const int blocks = a.max_pos / a.block + 1;
@@ -401,7 +429,7 @@ hipError_t launch_select(const TqSelectArgs &a, hipStream_t s) {
                        s, a, a.chunk);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((select_kernel<HD, 16, true>), grid, dim3(1024), 0, s, a);
+    hipLaunchKernelGGL((select_kernel<HD, 8, true>), grid, dim3(512), 0, s, a);
     return hipGetLastError();
 }
 
@@ -422,7 +450,16 @@ hipError_t tq_launch_bounds(const TqBoundsArgs &a, hipStream_t s) {
     return hipGetLastError();
 }
 
-int tq_select_chunk(int n_q, int n_kv_heads, int blocks) { return blocks <= kKeysInLds ? 0 : 512; }
+// A launch of its own for the scores takes about 3 us and pays where the selecting
+// work-groups, one per (query, kv head), leave most CUs idle over many blocks.  32 / 8
+// heads of 128, in one launch and in two: 1,024 blocks of 1 query 16.1 and 11.4 us, 8
+// queries 19.1 and 16.4, 16 queries 20.3 and 21.1; 4,096 blocks of 1 query 45 and 20, 16
+// queries 69 and 69; 256 blocks 8.9 .. 10.9 and 10.0 .. 13.0.
+int tq_select_chunk(int n_q, int n_kv_heads, int blocks) {
+    const long pairs = (long)n_q * n_kv_heads;
+    if (blocks <= 512 || (blocks <= kKeysInLds && pairs >= 128)) return 0;
+    return (int)std::min(256L, (pairs * blocks + 64 * 256 - 1) / (64 * 256) * 64);
+}
 
 hipError_t tq_launch_select(const TqSelectArgs &a, hipStream_t s) {
     switch (a.view.nb) {

@@ -468,3 +468,15 @@ def test_a_long_conversation(nat, oracle):
         pos = [p + 1 for p in pos]
     kept = bounds.dev.download(bounds.host.shape, np.uint16)
     assert np.array_equal(bounds.make(pos), kept)
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+def test_select_among_the_largest_scores(nat, oracle, sign):
+    """Infinite scores beside finite ones of either sign and of very different sizes: the bins' range ends near 2^64."""
+    s = Select(nat, oracle, 7, 1, 1, 64, [16 * 600 - 1], 16, 40, 0, 1, rope=False)
+    r = np.random.default_rng(8)
+    s.q = s.turned = np.abs(s.q) + 0.5
+    size = (sign * np.exp2(r.integers(-120, 120, s.stride))).astype(np.float32)
+    s.bounds[0, 0] = outward(size, True)[:, None, None]
+    s.bounds[0, 0, r.permutation(590)[:9], 0] = 0x7F80
+    assert np.array_equal(s.run(), s.expected())
