@@ -36,6 +36,18 @@ __global__ __launch_bounds__(kThreads) void decode_merge_kernel(TqMergeArgs a) {
     auto slot = [&](int s) { return s < own ? s : s - own + a.n_splits; };
     const int pstride = (G * (hd + 2) + 3) / 4 * 4;
     const float *part = a.partials + ((size_t)qi * a.n_kv_heads + kvh) * a.slots * pstride;
+    const int units = G * hd / 4;                                  // float4s of the rows
+    const int shares = units >= kThreads ? 1 : kThreads / units;   // slots s, s + shares, ..
+    constexpr int A = 8;
+    auto read = [&](int u, int s0, v4f (&o)[A]) {
+#pragma unroll
+        for (int i = 0; i < A; i++)
+            o[i] = *reinterpret_cast<const v4f *>(part + (size_t)slot(min(s0 + i * shares, used - 1)) * pstride + 4 * u);
+    };
+    // the first rows, on their way while the weights are made (of a thread without a share,
+    // any)
+    v4f ahead[A];
+    read(min(tid % min(units, kThreads), units - 1), tid / min(units, kThreads), ahead);
     for (int h = wave; h < G; h += kThreads / 64) {
         float m[2], l[2];
 #pragma unroll
@@ -54,8 +66,6 @@ __global__ __launch_bounds__(kThreads) void decode_merge_kernel(TqMergeArgs a) {
         wt[h][lane + 64] = f[1] * inv;
     }
     __syncthreads();
-    const int units = G * hd / 4;                                  // float4s of the rows
-    const int shares = units >= kThreads ? 1 : kThreads / units;   // slots s, s + shares, ..
     float *out = a.out + ((size_t)qi * a.n_q_heads + (size_t)kvh * G) * hd;
     for (int u0 = 0; u0 < units; u0 += kThreads) {
         const int u = u0 + tid % min(units, kThreads), share = tid / min(units, kThreads);
@@ -63,12 +73,14 @@ __global__ __launch_bounds__(kThreads) void decode_merge_kernel(TqMergeArgs a) {
         v4f acc = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         if (active) {
             const float *w = wt[4 * u / hd];
-            constexpr int A = 8;
             for (int s0 = share; s0 < used; s0 += A * shares) {
                 v4f o[A];
+                if (u0 == 0 && s0 == share) {
 #pragma unroll
-                for (int i = 0; i < A; i++)
-                    o[i] = *reinterpret_cast<const v4f *>(part + (size_t)slot(min(s0 + i * shares, used - 1)) * pstride + 4 * u);
+                    for (int i = 0; i < A; i++) o[i] = ahead[i];
+                } else {
+                    read(u, s0, o);
+                }
 #pragma unroll
                 for (int i = 0; i < A; i++) {
                     const int s = s0 + i * shares;

@@ -166,14 +166,14 @@ int decode3_waves_env() {
 }
 
 // MFMA decode: splits are whole units of 32*waves tokens (one tile per wave).
-// Aim at decode_wg_target() work-groups, at most decode3_split_cap() tokens per
+// Aim at `target` work-groups, at most decode3_split_cap() tokens per
 // split, and never more splits than the combine takes.
-void plan_splits3(const tq_hip_kv *kv, int n_q, int max_len, int waves, int *split_tokens, int *n_splits) {
+void plan_splits3(const tq_hip_kv *kv, int n_q, int max_len, int waves, int target, int *split_tokens, int *n_splits) {
     const int unit = 32 * waves;
     const long units = std::max(1, (max_len + unit - 1) / unit);
     const long pairs = (long)n_q * kv->desc.n_kv_heads;
     const long cap = tq_decode3_max_splits();
-    long want = (decode_wg_target(n_q) + pairs - 1) / pairs;
+    long want = (target + pairs - 1) / pairs;
     want = std::max(1L, std::min(std::min(want, cap), units));
     long per = (units + want - 1) / want;
     per = std::min<long>(per, std::max(1, decode3_split_cap() / unit));
@@ -199,7 +199,7 @@ int plan_decode3(const tq_hip_kv *kv, int n_q, int max_len, int *split_tokens, i
     // 8q/2kv/hd64 6.6 -> 5.3 us; from 384 keys on the splits win)
     if (n_q == 1 && max_len <= 8 * 32) waves = 8;
     if (decode3_waves_env()) waves = decode3_waves_env();
-    plan_splits3(kv, n_q, max_len, waves, split_tokens, n_splits);
+    plan_splits3(kv, n_q, max_len, waves, decode_wg_target(n_q), split_tokens, n_splits);
     return waves;
 }
 
@@ -1219,7 +1219,8 @@ void plan_shared(const tq_hip_kv *kv, int n_q, int max_pos, int n_groups, const 
     const long tiles = (most + 31) / 32;
     p.chunk = std::max(std::min(p.chunk, (long)TQ_SHARED_RUN_TILES), (tiles + kSharedRuns - 1) / kSharedRuns);
     p.runs = most ? tq_shared_runs(most, p.chunk) : 0;
-    plan_splits3(kv, n_q, max_pos + 1 - (least == INT32_MAX ? 0 : least), kSharedWaves, &p.split_tokens, &p.n_splits);
+    plan_splits3(kv, n_q, max_pos + 1 - (least == INT32_MAX ? 0 : least), kSharedWaves, decode_wg_target(n_q),
+                 &p.split_tokens, &p.n_splits);
     p.slots = p.n_splits + p.runs;
     const size_t list = ((size_t)n_q * sizeof(int32_t) + 255) & ~(size_t)255;
     p.partials = 2 * list;
@@ -1340,19 +1341,31 @@ bool block_ok(int block) {
     return block >= TQ_HIP_PAGE_TOKENS && block <= 1024 && block % TQ_HIP_PAGE_TOKENS == 0;
 }
 
+// (also where the scores need none: enough for fewer queries, which may)
 size_t select_ws(const tq_hip_kv *kv, int n_q, int max_pos, int block) {
     const int blocks = max_pos / block + 1;
-    if (tq_select_chunk(n_q, kv->desc.n_kv_heads, blocks) == 0) return 16;
+    if (tq_select_chunk(1, 1, blocks) == 0) return 16;
     return (size_t)n_q * kv->desc.n_kv_heads * blocks * sizeof(uint64_t);
 }
 
 // Most tokens that a step over listed blocks attends to.
 long blocks_len(int max_pos, int block, int keep) { return std::min((long)max_pos + 1, (long)keep * block); }
 
+// Waves per work-group, and the splits, of a step over listed blocks.  A batch aims at one
+// work-group of eight waves per CU: its lists are short, and a second split costs the
+// merge's launch too (32 queries of 32 / 8 heads of 128 over 2,048 tokens 31 us in one
+// split, 36 .. 40 in two; 16 of 64 / 8 over 4,096 in two splits of eight waves 39, in four
+// of four 41, in four of eight 46, in one 49).
+int plan_blocks(const tq_hip_kv *kv, int n_q, int max_len, int *split_tokens, int *n_splits) {
+    if (n_q == 1) return plan_decode3(kv, n_q, max_len, split_tokens, n_splits);
+    plan_splits3(kv, n_q, max_len, 8, 256, split_tokens, n_splits);
+    return 8;
+}
+
 size_t blocks_ws(const tq_hip_kv *kv, int n_q, int max_pos, int block, int keep) {
     const tq_hip_kv_desc &D = kv->desc;
     int split_tokens = 0, n_splits = 0;
-    plan_decode3(kv, n_q, (int)blocks_len(max_pos, block, keep), &split_tokens, &n_splits);
+    plan_blocks(kv, n_q, (int)blocks_len(max_pos, block, keep), &split_tokens, &n_splits);
     if (n_splits == 1) return 16;
     return (size_t)n_q * D.n_kv_heads * n_splits * tq_decode3_partial_floats(D.head_dim, D.n_q_heads / D.n_kv_heads) *
            sizeof(float);
@@ -1455,7 +1468,7 @@ int tq_hip_decode_step_blocks_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq
     if (on.rc != TQ_HIP_OK) return on.rc;
     const hipStream_t s = pick(kv, stream);
     TqDecodeArgs a = step_args(kv, n_q, d_seq, d_pos, d_q, d_k, d_v, d_cos, d_sin, d_out);
-    const int waves = plan_decode3(kv, n_q, (int)blocks_len(max_pos, block, keep), &a.split_tokens, &a.n_splits);
+    const int waves = plan_blocks(kv, n_q, (int)blocks_len(max_pos, block, keep), &a.split_tokens, &a.n_splits);
     a.list = d_list;
     a.keep = keep;
     a.block_tokens = block;

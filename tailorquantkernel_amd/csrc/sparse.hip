@@ -16,9 +16,9 @@
 //   w % (hd / 4) of every (256 / hd)-th row and that dword's scale, the rows' lanes are
 //   joined at the end.  Bound by reading the keys.
 // score_kernel: eight lanes per block, 16 bytes of bounds each at a time (whole lines),
-//   scores as order-preserving 64-bit keys.  Bound by the conversions to 64 bits, as many
-//   as products and four times as slow: 16 x 8 heads over 512 blocks in 6.5 us of the
-//   kernel's 11.7 (33.6 MB), and by reading the bounds over more of them (16 x 8 over
+//   scores as order-preserving 64-bit keys.  Bound by a bound's three instructions, of
+//   which the conversion to 64 bits runs at half the rate: 16 x 8 heads over 512 blocks in
+//   6.5 us of the kernel's 11.7 (33.6 MB), and by reading the bounds over more of them (16 x 8 over
 //   4,096 blocks, 268 MB in 69 us).  Reading four blocks ahead changed nothing.
 // select_kernel, one work-group per (query, kv head): the keep-th largest key by
 //   counting into bins over the range that the keys have, again within the bin at the
