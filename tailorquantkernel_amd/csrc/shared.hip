@@ -28,6 +28,7 @@ constexpr long kMostWgs = 1L << 23;
 struct SharedArgs {
     TqSharedTable t;
     TqDecodeArgs step;
+    int chunk;           // key tiles of a run
     int prefix_wgs;      // work-groups of the common tokens, in front of the others
     int z0;              // first query of the others
     int32_t *base_of, *runs_of;
@@ -233,20 +234,18 @@ __device__ __forceinline__ void prefix_run(const SharedArgs &sh, const int x, Pr
     const TqSharedTable &t_ = sh.t;
     const TqDecodeArgs &a = sh.step;
     const int n_kv = a.view.n_kv_heads;
-    const int kvh = x % n_kv, item = x / n_kv;
+    const int item = (int)((unsigned)x / (unsigned)n_kv), kvh = x - item * n_kv;
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = t_.n_groups == 1 ? 0 : find_sequence(t_.item0, t_.n_groups, item);
-    const int first = t_.first[g], prefix = t_.prefix[g], segs = t_.runs[g], rows = t_.members[g] * G;
-    const int blocks = (rows + kRows - 1) / kRows, mine = item - t_.item0[g];
-    const int run = mine / blocks, row0 = mine % blocks * kRows;
+    const int first = t_.first[g], prefix = t_.prefix[g], rows = t_.members[g] * G;
+    const unsigned blocks = (unsigned)(rows + kRows - 1) / kRows, mine = item - t_.item0[g];
+    const int run = (int)(mine / blocks), row0 = (int)(mine - run * blocks) * kRows;
+    // the run's tiles
+    const int kt0 = run * sh.chunk, nt = min(sh.chunk, (prefix + kKT - 1) / kKT - kt0);
     const int seq = a.seq_of ? a.seq_of[first] : first;
     const bool seq_ok = seq >= 0 && seq < a.view.max_seqs;
     const int32_t *table = a.view.page_table + (seq_ok ? (size_t)seq * a.view.max_pages : 0);
-    // the run's tiles, as even as they go
-    const int all = (prefix + kKT - 1) / kKT;
-    const int kt0 = (int)((long)all * run / segs), nt = (int)((long)all * (run + 1) / segs) - kt0;
-
     // Copies of a tile's K rows, or its V rows, by the work-group from its two pages' runs.
     // The pages' ids, lanes 0 and 1 of a vector load (a scalar one would hold up every LDS
     // read until it is back), are read a step before the copies that go by them.
@@ -430,10 +429,11 @@ int tq_shared_runs(int prefix, long chunk) {
     return (int)((tiles + chunk - 1) / chunk);
 }
 
-hipError_t tq_launch_shared(const TqSharedTable &t, const TqDecodeArgs &step, int32_t *base_of, int32_t *runs_of,
+hipError_t tq_launch_shared(const TqSharedTable &t, int chunk, const TqDecodeArgs &step, int32_t *base_of, int32_t *runs_of,
                             hipStream_t s) {
     const int g = step.n_q_heads / step.n_kv_heads;
-    if (!tq_shared_supported(step.head_dim, g) || t.n_groups < 0 || t.n_groups > TQ_MAX_PACK) return hipErrorInvalidValue;
+    if (!tq_shared_supported(step.head_dim, g) || t.n_groups < 0 || t.n_groups > TQ_MAX_PACK || chunk < 1)
+        return hipErrorInvalidValue;
     if (step.n_splits < 1 || step.n_splits > d3::kMaxSplits3 || step.split_tokens <= 0 || step.split_tokens % d3::kTK != 0 ||
         step.split_tokens > d3::kMaxSplitPages3 * kPage)
         return hipErrorInvalidValue;
@@ -446,12 +446,11 @@ hipError_t tq_launch_shared(const TqSharedTable &t, const TqDecodeArgs &step, in
     a.runs_of = runs_of;
     a.t.item0[0] = 0;
     long items = 0;
+    a.chunk = chunk;
     for (int i = 0; i < t.n_groups; i++) {
-        const long tiles = (t.prefix[i] + kKT - 1) / kKT, runs = t.runs[i];
-        if (runs < 0 || runs > tiles || runs + step.n_splits > step.part_slots ||
-            (tiles > 0 && (runs == 0 || (tiles + runs - 1) / runs > TQ_SHARED_RUN_TILES)))
-            return hipErrorInvalidValue;
-        items += (t.members[i] * (long)g + kRows - 1) / kRows * runs;
+        a.t.runs[i] = tq_shared_runs(t.prefix[i], chunk);
+        if (a.t.runs[i] + step.n_splits > step.part_slots) return hipErrorInvalidValue;
+        items += (t.members[i] * (long)g + kRows - 1) / kRows * a.t.runs[i];
         if (items * step.n_kv_heads >= kMostWgs) return hipErrorInvalidValue;
         a.t.item0[i + 1] = (int)items;
     }

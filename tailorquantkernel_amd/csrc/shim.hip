@@ -1217,8 +1217,8 @@ void plan_shared(const tq_hip_kv *kv, int n_q, int max_pos, int n_groups, const 
     const long all = steps * D.n_kv_heads, wgs = all <= 40 * 256 ? 256 : 512;
     p.chunk = std::max(1L, (all + wgs - 1) / wgs);
     const long tiles = (most + 31) / 32;
-    p.chunk = std::max(std::min(p.chunk, (long)TQ_SHARED_RUN_TILES), (tiles + kSharedRuns - 1) / kSharedRuns);
-    p.runs = most ? tq_shared_runs(most, p.chunk) : 0;
+    p.chunk = std::max(p.chunk, (tiles + kSharedRuns - 1) / kSharedRuns);
+    p.runs = tq_shared_runs(most, p.chunk);
     plan_splits3(kv, n_q, max_pos + 1 - (least == INT32_MAX ? 0 : least), kSharedWaves, decode_wg_target(n_q),
                  &p.split_tokens, &p.n_splits);
     p.slots = p.n_splits + p.runs;
@@ -1275,9 +1275,8 @@ int tq_hip_decode_step_shared_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq
             t.first[i] = start[g0 + i];
             t.members[i] = start[g0 + i + 1] - start[g0 + i];
             t.prefix[i] = shared_tokens(start, prefix, g0 + i);
-            t.runs[i] = t.prefix[i] ? tq_shared_runs(t.prefix[i], p.chunk) : 0;
         }
-        TQ_TRY(tq_launch_shared(t, a, base_of, runs_of, s));
+        TQ_TRY(tq_launch_shared(t, (int)p.chunk, a, base_of, runs_of, s));
         g0 += t.n_groups;
     } while (g0 < n_groups);
     TqMergeArgs m = merge_args(a);

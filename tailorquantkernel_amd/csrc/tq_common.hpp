@@ -538,15 +538,14 @@ hipError_t tq_launch_pack_rows(const TqPackRows &a, const TqPackTable &t, int fi
 // [query0, query1) whose steps behind the common tokens it makes.  Every split and run
 // leaves its rows' means, then m and l, in the step's partials: splits in the first
 // n_splits slots, runs from there on; base_of and runs_of go to tq_launch_decode_merge.
-#define TQ_SHARED_RUN_TILES 512     // key tiles of a run at most
 struct TqSharedTable {
     int n_groups;
     int query0, query1;
     int first[TQ_MAX_PACK];         // first query
     int members[TQ_MAX_PACK];
     int prefix[TQ_MAX_PACK];        // common tokens, 0 where the group shares nothing
-    int runs[TQ_MAX_PACK];          // runs of their key tiles, at most as many
-    int item0[TQ_MAX_PACK + 1];     // filled in by the launch
+    int runs[TQ_MAX_PACK];          // filled in by the launch: runs of their key tiles
+    int item0[TQ_MAX_PACK + 1];     //   and first item
 };
 bool tq_shared_supported(int head_dim, int group);
 // Key tiles times blocks of rows of a group, and the runs that cut its tiles in `chunk`s.
@@ -554,5 +553,5 @@ long tq_shared_steps(int members, int group, int prefix);
 int tq_shared_runs(int prefix, long chunk);
 // Waves of a work-group: the splits' units (plan_splits3).
 constexpr int kSharedWaves = 4;
-hipError_t tq_launch_shared(const TqSharedTable &t, const TqDecodeArgs &step, int32_t *base_of, int32_t *runs_of,
+hipError_t tq_launch_shared(const TqSharedTable &t, int chunk, const TqDecodeArgs &step, int32_t *base_of, int32_t *runs_of,
                             hipStream_t s);
