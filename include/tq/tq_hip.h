@@ -309,8 +309,13 @@ int tq_hip_decode_step_weights_async(tq_hip_kv *kv, int n_q, const int32_t *d_se
  * sequences begin with, a system prompt or a document (no counterpart in the
  * reference): queries start[g] .. start[g + 1] - 1 are group g, and the first
  * prefix[g] tokens of its sequences, a multiple of TQ_HIP_PAGE_TOKENS, lie in the same
- * pages, which are read once for the group, through the page table of its first
- * query's sequence.  Queries before start[0] and from start[n_groups] on share
+ * pages, which may be read once for the group, through the page table of its first
+ * query's sequence: the call does so, in groups of four and more queries, where that
+ * is faster for its groups as a whole, and else each query reads its own table (about
+ * 12 queries with 8,192 common tokens, or 32 with 2,048, are enough).  What is read
+ * together is kept as in the packed prefill, products to 2^-20 of themselves, terms
+ * below 2^-28 of the row's largest V scale not at all; the rest as in the step above.
+ * The choice goes by the shape, start and prefix only.  Queries before start[0] and from start[n_groups] on share
  * nothing.  start (n_groups + 1 entries, none less than the one before, the last at
  * most n_q) and prefix are HOST arrays, read during the call: a captured call keeps
  * its groups, while d_seq, d_pos and the pages may change.  A query whose d_pos[i] is

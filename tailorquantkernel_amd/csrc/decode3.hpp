@@ -268,19 +268,21 @@ __device__ __forceinline__ void split3_bf16(const float (&x)[8], v8bf &hi, v8bf 
 // position is one in that order; only the page ids' way to the table differs.  The
 // work-group that appends also puts the new key into its block's bounds.
 // kShared, the part of a step behind a group's common tokens: positions begin at
-// `base`, a whole page, and query z is z (shared.hip's work-groups run it).
+// `base`, a whole page, a query whose new token lies below `least` is left out, and query
+// z is z (shared.hip's work-groups run it).
 // Of these two every split leaves its rows' means with m and l (a step over blocks in
 // one split its output), and decode_merge_kernel joins them.
 // RMSNorm and completion flags are kPlain's only; kRows appends nothing and takes its
 // pages from the table, as kBlocks and kShared do; these and kScores always append.
 constexpr int kPlain = 0, kRows = 1, kScores = 2, kBlocks = 3, kShared = 4;
-// split, kvh, z: the grid's place; base: kShared's; sm and the slots: the work-group's shared memory (two
+// split, kvh, z: the grid's place; least, base: kShared's; sm and the slots: the work-group's shared memory (two
 // tile slots per wave, separate objects so that the wait for one slot's copies does not
 // wait for the other's).
 template <int HD, int G, int W, int MODE>
 __device__ __forceinline__ void decode3_run(const TqDecodeArgs &a, const int split, const int kvh, const int z,
                                             Smem3<HD, G> &sm, unsigned char (&slot0)[W][L3<HD, G>::TILE],
-                                            unsigned char (&slot1)[W][L3<HD, G>::TILE], const int base = 0) {
+                                            unsigned char (&slot1)[W][L3<HD, G>::TILE], const int least = 0,
+                                            const int base = 0) {
     using L = L3<HD, G>;
     constexpr int kWaves = W;
     constexpr int kThreads = 64 * W;
@@ -441,7 +443,7 @@ __device__ __forceinline__ void decode3_run(const TqDecodeArgs &a, const int spl
     }
     __builtin_amdgcn_sched_barrier(0);
     int len = a.len_of ? len_raw + a.len_plus : a.pos0 + qi + 1;
-    if (MODE == kShared) len -= base;
+    if (MODE == kShared) len = len <= least ? 0 : len - base;
     [[maybe_unused]] const int at_new = len - 1;   // kBlocks: the new token's slot
     if (MODE == kBlocks && len > 0) {
         const int block = at_new / a.block_tokens;

@@ -1,6 +1,6 @@
 // decode_merge.hip — the second launch of a decode step whose splits leave partial rows:
 // a step over listed blocks in several splits, and a step behind common tokens
-// (decode3_parts.hip, shared.hip).  No counterpart in the reference.
+// (decode3_blocks.hip, shared.hip).  No counterpart in the reference.
 //
 //   M = max over slots of m,  w = l 2^(m - M) / sum l 2^(m - M),  out = sum, in the
 //   slots' order, of w o
@@ -24,15 +24,17 @@ __global__ __launch_bounds__(kThreads) void decode_merge_kernel(TqMergeArgs a) {
     __shared__ __align__(16) v4f red[kThreads];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int kvh = blockIdx.x, qi = blockIdx.y, hd = a.head_dim;
-    int len = a.pos_of[qi] + 1 - (a.base_of ? a.base_of[qi] : 0);
-    if (len <= 0) return;
+    const int least = a.runs_of ? a.least_of[qi] : 0, runs = a.runs_of ? a.runs_of[qi] : 0;
+    int len = a.pos_of[qi] + 1;
+    if (len <= least) return;
+    if (runs) len -= least;
     if (a.keep) {
         const int block = (len - 1) / a.block_tokens;
         len += (min(block, a.keep - 1) - block) * a.block_tokens;
     }
     // slots 0 .. own - 1, then n_splits .. n_splits + runs - 1, numbered through
     const int own = min((len + a.split_tokens - 1) / a.split_tokens, a.n_splits);
-    const int used = own + (a.runs_of ? a.runs_of[qi] : 0);
+    const int used = own + runs;
     auto slot = [&](int s) { return s < own ? s : s - own + a.n_splits; };
     const int pstride = (G * (hd + 2) + 3) / 4 * 4;
     const float *part = a.partials + ((size_t)qi * a.n_kv_heads + kvh) * a.slots * pstride;

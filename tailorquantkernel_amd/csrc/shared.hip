@@ -6,10 +6,10 @@
 // read once and not once per member, and the work goes to the matrix cores 32 rows at a
 // time, as a prompt's does (pack_tile.hpp, whose scores, softmax and products these
 // are; what bounds them stands in prefill_packed.hip).  What lies behind the common
-// tokens each sequence attends to by itself (decode3_parts.hip), and
-// decode_merge_kernel joins the means of both.
+// tokens each sequence attends to by itself (decode3.hpp), in work-groups of the same
+// launch, and decode_merge_kernel joins the means of both.
 //
-// shared_prefix_kernel, 4 waves per (128 rows of a group, run of its key tiles, kv head):
+// prefix_run, 4 waves per (128 rows of a group, run of its key tiles, kv head):
 //   a tile's rows come from the pages by global_load_lds, two tiles ahead, and the
 //   work-group makes the tile's image from them in LDS: with few rows a key, an image
 //   in memory (2.8 times the cache's bytes, written and read again) would take longer
@@ -30,8 +30,8 @@ struct SharedArgs {
     TqDecodeArgs step;
     int chunk;           // key tiles of a run
     int prefix_wgs;      // work-groups of the common tokens, in front of the others
-    int z0;              // first query of the others
-    int32_t *base_of, *runs_of;
+    int z0, pairs;       // the others' first query, and (query, kv head) pairs
+    int32_t *least_of, *runs_of;
 };
 
 // The K (or V) rows of a tile: two pages' runs, one behind the other, [32][ROW].
@@ -382,20 +382,23 @@ __global__ __launch_bounds__(kThreads, 2) void shared_step_kernel(SharedArgs a) 
         prefix_run<HD, G>(a, (int)blockIdx.x, lds.prefix);
         return;
     }
-    const int n_kv = a.step.n_kv_heads, split = x % a.step.n_splits, pair = x / a.step.n_splits;
+    // every pair's first split in front of the second ones: those that lie behind a
+    // sequence's end come last, and on all XCDs alike (a pair's splits in a row put the
+    // same split of all on one where their number is 2, 4 or 8)
+    const int n_kv = a.step.n_kv_heads, split = (int)((unsigned)x / (unsigned)a.pairs), pair = x - split * a.pairs;
     const int kvh = pair % n_kv, z = a.z0 + pair / n_kv;
     // the query's group
     const int lane = threadIdx.x & 63;
     const bool in = lane < a.t.n_groups && a.t.first[lane] <= z && z < a.t.first[lane] + a.t.members[lane];
     const unsigned long long which = __builtin_amdgcn_ballot_w64(in);
     const int g = which ? __builtin_ctzll(which) : 0;
-    const int base = which ? a.t.prefix[g] : 0;
+    const int least = which ? a.t.prefix[g] : 0, runs = which ? a.t.runs[g] : 0;
     if (split == 0 && kvh == 0 && threadIdx.x == 0) {
-        a.base_of[z] = base;
-        a.runs_of[z] = which ? a.t.runs[g] : 0;
+        a.least_of[z] = least;
+        a.runs_of[z] = runs;
     }
     StepLds &s = *reinterpret_cast<StepLds *>(lds.step);
-    d3::decode3_run<HD, G, kSharedWaves, d3::kShared>(a.step, split, kvh, z, s.sm, s.slot0, s.slot1, base);
+    d3::decode3_run<HD, G, kSharedWaves, d3::kShared>(a.step, split, kvh, z, s.sm, s.slot0, s.slot1, least, runs ? least : 0);
 }
 
 template <int HD>
@@ -429,7 +432,7 @@ int tq_shared_runs(int prefix, long chunk) {
     return (int)((tiles + chunk - 1) / chunk);
 }
 
-hipError_t tq_launch_shared(const TqSharedTable &t, int chunk, const TqDecodeArgs &step, int32_t *base_of, int32_t *runs_of,
+hipError_t tq_launch_shared(const TqSharedTable &t, int chunk, const TqDecodeArgs &step, int32_t *least_of, int32_t *runs_of,
                             hipStream_t s) {
     const int g = step.n_q_heads / step.n_kv_heads;
     if (!tq_shared_supported(step.head_dim, g) || t.n_groups < 0 || t.n_groups > TQ_MAX_PACK || chunk < 1)
@@ -442,15 +445,15 @@ hipError_t tq_launch_shared(const TqSharedTable &t, int chunk, const TqDecodeArg
     SharedArgs a;
     a.t = t;
     a.step = step;
-    a.base_of = base_of;
+    a.least_of = least_of;
     a.runs_of = runs_of;
     a.t.item0[0] = 0;
     long items = 0;
     a.chunk = chunk;
     for (int i = 0; i < t.n_groups; i++) {
-        a.t.runs[i] = tq_shared_runs(t.prefix[i], chunk);
-        if (a.t.runs[i] + step.n_splits > step.part_slots) return hipErrorInvalidValue;
-        items += (t.members[i] * (long)g + kRows - 1) / kRows * a.t.runs[i];
+        if (t.runs[i] != 0 && (t.prefix[i] == 0 || t.runs[i] != tq_shared_runs(t.prefix[i], chunk))) return hipErrorInvalidValue;
+        if (t.runs[i] + step.n_splits > step.part_slots) return hipErrorInvalidValue;
+        items += (t.members[i] * (long)g + kRows - 1) / kRows * t.runs[i];
         if (items * step.n_kv_heads >= kMostWgs) return hipErrorInvalidValue;
         a.t.item0[i + 1] = (int)items;
     }
@@ -459,7 +462,8 @@ hipError_t tq_launch_shared(const TqSharedTable &t, int chunk, const TqDecodeArg
     const int most = (int)std::max(1L, kMostWgs / per_query);
     a.prefix_wgs = (int)items * step.n_kv_heads;
     for (a.z0 = t.query0; a.z0 < t.query1; a.z0 += most) {
-        const unsigned wgs = (unsigned)(a.prefix_wgs + std::min(most, t.query1 - a.z0) * per_query);
+        a.pairs = std::min(most, t.query1 - a.z0) * step.n_kv_heads;
+        const unsigned wgs = (unsigned)(a.prefix_wgs + (long)a.pairs * step.n_splits);
         const hipError_t e = step.head_dim == 64 ? launch_shared<64>(a, g, wgs, s) : launch_shared<128>(a, g, wgs, s);
         if (e != hipSuccess) return e;
         a.prefix_wgs = 0;

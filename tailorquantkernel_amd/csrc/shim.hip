@@ -1171,19 +1171,47 @@ namespace {
 // Most runs of a group's common tokens, and splits of what lies behind them: the merge
 // holds 128 slots.
 constexpr int kSharedRuns = 64;
+// Fewest queries of a group that attend to its tokens together.
+constexpr int kFewestMembers = 4;
 
 // How a step with common tokens is cut: what each group shares, in runs of `chunk` key
 // tiles, and the splits behind.
 struct SharedPlan {
+    bool together = false;
+    // What a group attends to together: all of its common tokens, or none.
+    int common(int members, int prefix) const { return together && members >= kFewestMembers ? prefix : 0; }
     long chunk = 1;
     int runs = 0;            // most runs of a group
     int split_tokens, n_splits, slots;
-    size_t partials, bytes;  // of the workspace: base_of, runs_of, partials
+    size_t partials, bytes;  // of the workspace: least_of, runs_of, partials
 };
 
-// What group g shares: tokens that are worth a launch of their own.
-int shared_tokens(const int32_t *start, const int32_t *prefix, int g) {
-    return start[g + 1] - start[g] >= 2 ? prefix[g] : 0;
+// Whether a call's groups attend to their common tokens together, or each query to its
+// own as in any step.  A token of a kv head costs a query one unit by itself (1.5 with
+// more than 4 heads a kv head), and a block of 128 rows six, whatever it holds; the
+// images, the rows' means and their merge want some 300,000 units saved.  Measured (us,
+// together / each by itself; own tokens 64-256 behind):
+//   queries  common   32 / 8 heads   64 / 8         16 / 16        24 / 8 of 64
+//   4         4,096   22.4 / 16.8    24.5 / 21.4    28.8 / 20.0    17.2 / 14.4   apart
+//   8         4,096   23.1 / 20.7    26.8 / 26.1    29.2 / 27.3    17.7 / 16.8   apart
+//   8        16,384   48.3 / 52.3    52.2 / 67.6*   79.4 / 73.0    38.5 / 31.7   apart (* together)
+//   12        2,048   19.7 / 23.1    24.2 / 27.7    21.3 / 30.8    14.6 / 16.4   apart
+//   12        8,192   33.0 / 46.6    37.5 / 59.0    46.1 / 75.3    25.7 / 30.1   together
+//   16        4,096   25.5 / 28.1    30.5 / 37.7    30.0 / 41.2    18.6 / 22.8   together
+//   32        1,024   28.6 / 21.0    33.7 / 26.3    25.2 / 29.0*   15.8 / 18.0   apart (* together)
+//   32        2,048   28.7 / 28.7    33.5 / 37.9    25.5 / 43.0    16.6 / 23.6   together
+//   64          256   23.9 / 20.0    32.1 / 24.2    28.7 / 30.6    17.4 / 16.9   apart
+//   64        1,024   32.5 / 31.8    39.1 / 40.3    35.8 / 52.6    19.2 / 25.4   together
+//   64        4,096   39.7 / 77.3    58.7 / 103     43.4 / 138     29.2 / 58.1   together
+bool worth_sharing(const tq_hip_kv *kv, int n_groups, const int32_t *start, const int32_t *prefix) {
+    const int g = kv->desc.n_q_heads / kv->desc.n_kv_heads;
+    double saved = 0.0;
+    for (int i = 0; i < n_groups; i++) {
+        const int members = start[i + 1] - start[i];
+        if (members >= kFewestMembers)
+            saved += (members * (g > 4 ? 1.5 : 1.0) - 6.0 * tq_shared_steps(members, g, 1)) * prefix[i];
+    }
+    return saved * kv->desc.n_kv_heads >= 300e3;
 }
 
 bool shared_ok(const tq_hip_kv *kv, int n_q, int max_pos, int n_groups, const int32_t *start, const int32_t *prefix) {
@@ -1201,15 +1229,22 @@ void plan_shared(const tq_hip_kv *kv, int n_q, int max_pos, int n_groups, const 
                  SharedPlan &p) {
     const tq_hip_kv_desc &D = kv->desc;
     const int g = D.n_q_heads / D.n_kv_heads;
-    long steps = 0;
-    int least = n_groups > 0 && start[0] == 0 && start[n_groups] == n_q ? INT32_MAX : 0, most = 0;
+    p.together = worth_sharing(kv, n_groups, start, prefix);
+    long steps = 0, grouped = 0, apart = 0, longest = 0;   // key tiles of rows; queries; tokens that a query attends to by itself
+    int least = INT32_MAX, deepest = 0, most = 0;
     for (int i = 0; i < n_groups; i++) {
-        if (start[i + 1] == start[i]) continue;
-        const int common = shared_tokens(start, prefix, i);
+        const int members = start[i + 1] - start[i];
+        if (members == 0) continue;
+        const int common = p.common(members, prefix[i]);
         least = std::min(least, common);
         most = std::max(most, common);
-        steps += tq_shared_steps(start[i + 1] - start[i], g, common);
+        deepest = std::max(deepest, (int)prefix[i]);
+        longest = std::max(longest, (long)prefix[i] - common);
+        steps += tq_shared_steps(members, g, common);
+        grouped += members;
+        apart += (long)members * (prefix[i] - common);
     }
+    if (grouped < n_q) least = 0;
     // one work-group per CU, the queries' own beside it, where the tiles are few: each
     // writes its rows' means, and two a CU are slowed by one another (64 queries of 32 / 8
     // heads, 128 and their own up to 512 tokens: behind 1,024 common ones 36.7 us and 45.2
@@ -1219,8 +1254,28 @@ void plan_shared(const tq_hip_kv *kv, int n_q, int max_pos, int n_groups, const 
     const long tiles = (most + 31) / 32;
     p.chunk = std::max(p.chunk, (tiles + kSharedRuns - 1) / kSharedRuns);
     p.runs = tq_shared_runs(most, p.chunk);
-    plan_splits3(kv, n_q, max_pos + 1 - (least == INT32_MAX ? 0 : least), kSharedWaves, decode_wg_target(n_q),
-                 &p.split_tokens, &p.n_splits);
+    // Splits of what a query attends to by itself: at first as of a step of max_len tokens.
+    // Where a few have much more than the others, common tokens of a small group, more
+    // splits shorten what the last of them takes (0.75 us for 128 tokens, if the 512
+    // work-groups that run at once do not have as much each), and those behind the
+    // others' ends cost their start (3.5 us for 512).  Groups of 12, 3 and 33 behind
+    // 16,384, 7,680 and 864 common tokens, 64 / 8 heads: 2 splits 143 us, 5 92.
+    const long whole = (long)max_pos + 1, own = whole - deepest, pairs = (long)n_q * D.n_kv_heads;
+    apart += grouped * own + (n_q - grouped) * whole;
+    longest = grouped < n_q ? whole : longest + own;
+    const int max_len = (int)(whole - least);
+    plan_splits3(kv, n_q, max_len, kSharedWaves, decode_wg_target(n_q), &p.split_tokens, &p.n_splits);
+    const int unit = 32 * kSharedWaves;
+    const double even = (double)apart * D.n_kv_heads / 512;
+    double best = 1e30;
+    for (int n = p.n_splits; n <= tq_decode3_max_splits(); n++) {
+        const int tokens = ((max_len + n - 1) / n + unit - 1) / unit * unit;
+        const double t = std::max(even, (double)std::min<long>(tokens, longest)) * (0.75 / unit) + n * pairs * (3.5 / 512);
+        if (t >= best) continue;
+        best = t;
+        p.split_tokens = tokens;
+        p.n_splits = (max_len + tokens - 1) / tokens;
+    }
     p.slots = p.n_splits + p.runs;
     const size_t list = ((size_t)n_q * sizeof(int32_t) + 255) & ~(size_t)255;
     p.partials = 2 * list;
@@ -1264,7 +1319,7 @@ int tq_hip_decode_step_shared_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq
     a.n_splits = p.n_splits;
     a.part_slots = p.slots;
     a.partials = reinterpret_cast<float *>(ws + p.partials);
-    int32_t *base_of = reinterpret_cast<int32_t *>(ws), *runs_of = reinterpret_cast<int32_t *>(ws + p.partials / 2);
+    int32_t *least_of = reinterpret_cast<int32_t *>(ws), *runs_of = reinterpret_cast<int32_t *>(ws + p.partials / 2);
     TqSharedTable t;   // TQ_MAX_PACK groups a launch
     int g0 = 0;
     do {
@@ -1274,13 +1329,14 @@ int tq_hip_decode_step_shared_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq
         for (int i = 0; i < t.n_groups; i++) {
             t.first[i] = start[g0 + i];
             t.members[i] = start[g0 + i + 1] - start[g0 + i];
-            t.prefix[i] = shared_tokens(start, prefix, g0 + i);
+            t.prefix[i] = prefix[g0 + i];
+            t.runs[i] = tq_shared_runs(p.common(t.members[i], t.prefix[i]), p.chunk);
         }
-        TQ_TRY(tq_launch_shared(t, (int)p.chunk, a, base_of, runs_of, s));
+        TQ_TRY(tq_launch_shared(t, (int)p.chunk, a, least_of, runs_of, s));
         g0 += t.n_groups;
     } while (g0 < n_groups);
     TqMergeArgs m = merge_args(a);
-    m.base_of = base_of;
+    m.least_of = least_of;
     m.runs_of = runs_of;
     m.slots = p.slots;
     return herr(tq_launch_decode_merge(m, s));

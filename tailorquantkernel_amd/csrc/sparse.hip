@@ -1,6 +1,6 @@
 // sparse.hip — which blocks of a long context a query attends to: the bounds of a block's
 // keys, and the choice by what they can score (tq_hip_kv_bounds_async,
-// tq_hip_kv_select_async; the step over the chosen blocks is decode3_parts.hip).  No
+// tq_hip_kv_select_async; the step over the chosen blocks is decode3_blocks.hip).  No
 // counterpart in the reference, which attends to everything.
 //
 //   M_c, m_c = max, min over a block's tokens of d_t code_tc, as bf16 rounded outward

@@ -361,12 +361,12 @@ hipError_t tq_launch_decode3(const TqDecodeArgs &a, int waves, hipStream_t s);
 hipError_t tq_launch_decode3_blocks(const TqDecodeArgs &a, int waves, hipStream_t s);
 
 // out from partials [query][kv head][slots][floats as tq_decode3_partial_floats]: of a
-// query at d_pos the slots of its splits (of its tokens, of listed blocks or from
-// base_of on) and the runs_of slots from n_splits on.  A query without slots, and one
-// in front of its base, is left.
+// query at d_pos the slots of its splits (of its tokens, of listed blocks or, with runs,
+// from least_of on) and the runs_of slots from n_splits on.  A query in front of its
+// least position is left.
 struct TqMergeArgs {
     const int32_t *pos_of;
-    const int32_t *base_of;  // or null: 0
+    const int32_t *least_of;  // or null: 0
     const int32_t *runs_of;  // or null: 0
     int keep, block_tokens;  // listed blocks, or 0
     int n_q, n_q_heads, n_kv_heads, head_dim;
@@ -537,15 +537,15 @@ hipError_t tq_launch_pack_rows(const TqPackRows &a, const TqPackTable &t, int fi
 // tq_hip_decode_step_shared_async (shared.hip): groups of a launch and the queries
 // [query0, query1) whose steps behind the common tokens it makes.  Every split and run
 // leaves its rows' means, then m and l, in the step's partials: splits in the first
-// n_splits slots, runs from there on; base_of and runs_of go to tq_launch_decode_merge.
+// n_splits slots, runs from there on; least_of and runs_of go to tq_launch_decode_merge.
 struct TqSharedTable {
     int n_groups;
     int query0, query1;
     int first[TQ_MAX_PACK];         // first query
     int members[TQ_MAX_PACK];
     int prefix[TQ_MAX_PACK];        // common tokens, 0 where the group shares nothing
-    int runs[TQ_MAX_PACK];          // filled in by the launch: runs of their key tiles
-    int item0[TQ_MAX_PACK + 1];     //   and first item
+    int runs[TQ_MAX_PACK];          // runs of their key tiles; 0: each attends to them by itself
+    int item0[TQ_MAX_PACK + 1];     // filled in by the launch
 };
 bool tq_shared_supported(int head_dim, int group);
 // Key tiles times blocks of rows of a group, and the runs that cut its tiles in `chunk`s.
@@ -553,5 +553,5 @@ long tq_shared_steps(int members, int group, int prefix);
 int tq_shared_runs(int prefix, long chunk);
 // Waves of a work-group: the splits' units (plan_splits3).
 constexpr int kSharedWaves = 4;
-hipError_t tq_launch_shared(const TqSharedTable &t, int chunk, const TqDecodeArgs &step, int32_t *base_of, int32_t *runs_of,
+hipError_t tq_launch_shared(const TqSharedTable &t, int chunk, const TqDecodeArgs &step, int32_t *least_of, int32_t *runs_of,
                             hipStream_t s);

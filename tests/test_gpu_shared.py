@@ -18,28 +18,52 @@ def nat():
     return native
 
 
+def members(n):
+    """Own tokens of n members of a group."""
+    return [(7 * i) % 50 for i in range(n)]
+
+
+def large_group(nq, nkv):
+    """A group that makes a call attend to the common tokens of its groups of 4 and more together."""
+    group = nq // nkv
+    n = 120 // group
+    saved = n * (1.5 if group > 4 else 1) - 6
+    return PAGE * (int(400e3 / (saved * nkv)) // PAGE + 1), members(n)
+
+
 class Shared:
     """Groups of (common tokens, [own tokens of each member]), `before` and `behind` lists of queries that share nothing.
-    A query appends the token behind its own."""
+    A query appends the token behind its own.  large: behind the others a group that makes the call attend to common
+    tokens together."""
 
     def __init__(self, nat, oracle, seed, nq, nkv, hd, groups, before=(), behind=(), rope=True, order=None, room=1,
-                 max_pos=None):
+                 max_pos=None, large=True):
+        self.checked = len(before) + sum(len(m) for _, m in groups)      # and the large group's last, and what is behind it
+        if large:
+            groups = [*groups, large_group(nq, nkv)]
+        self.behind = len(behind)
         own = [*before, *(m for _, members in groups for m in members), *behind]
         base = [0] * len(before) + [p for p, members in groups for _ in members] + [0] * len(behind)
         lens = [b + m for b, m in zip(base, own)]
-        self.order = list(range(len(own))) if order is None else order      # query i reads sequence order[i]
+        self.order = list(range(len(own)))                                  # query i reads sequence order[i]
+        self.order[:len(order or ())] = order or ()
         by_seq = [0] * len(own)
         for i, s in enumerate(self.order):
-            by_seq[s] = lens[i]
+            by_seq[s] = own[i]                  # a group's first sequence holds its common tokens, and room for any own
+        at = len(before)
+        for p, rest in groups:
+            if rest:
+                by_seq[self.order[at]] = p + max(rest)
+            at += len(rest)
         c = self.c = Cache(nat, oracle, seed, nq, nkv, hd, by_seq, room=room)
         at = len(before)
         self.start, self.prefix = [at], []
-        for p, members in groups:
-            for i in range(at, at + len(members)):
+        for p, rest in groups:
+            for i in range(at + 1, at + len(rest)):
                 first, mine = self.order[at], self.order[i]
-                c.pages[mine] = np.concatenate([c.pages[first][:p // PAGE], c.pages[mine][p // PAGE:]])
+                c.pages[mine] = np.concatenate([c.pages[first][:p // PAGE], c.pages[mine]])
                 c.kv.set_pages(mine, c.pages[mine])
-            at += len(members)
+            at += len(rest)
             self.start.append(at)
             self.prefix.append(p)
         self.host = np.asarray(self.start, np.int32), np.asarray(self.prefix, np.int32)
@@ -52,7 +76,7 @@ class Shared:
         self.dev = {"q": c.up(self.q), "k": c.up(self.k), "v": c.up(self.v), "seq": None,
                     "out": c.up(np.full(self.q.shape, 3.0, np.float32))}
         if order is not None:
-            self.dev["seq"] = c.up(np.asarray(order, np.int32))
+            self.dev["seq"] = c.up(np.asarray(self.order, np.int32))
         self.at(lens)
         self.ws_bytes = c.lib.tq_hip_decode_step_shared_ws_bytes(c.kv.h, self.n, self.max_pos, len(self.prefix),
                                                                  self.host[0].ctypes.data, self.host[1].ctypes.data)
@@ -98,7 +122,7 @@ class Shared:
                 assert (out[i] == 3.0).all()
                 continue
             c.put(s, [p], np.stack([kq[i], vq[i]], 1)[None])
-            if not finite:
+            if not finite or self.checked <= i < len(self.pos) - self.behind - 1:
                 continue
             rows = c.rows(s, p + 1)
             ref, bound, _, _ = attention(c, qq[i:i + 1], rows, [p], 2.0 ** -20 + 80 * 2.0 ** -24)
@@ -112,68 +136,89 @@ class Shared:
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("group", [1, 2, 3, 4, 5, 6, 7, 8])
 def test_shapes(nat, oracle, hd, group):
-    st = Shared(nat, oracle, hd + group, 2 * group, 2, hd, [(48, [0, 5, 40]), (32, [7]), (320, [1, 2, 300, 16, 15])],
+    st = Shared(nat, oracle, hd + group, 2 * group, 2, hd, [(48, [0, 5, 40, 9]), (32, [7]), (320, [1, 2, 300, 16, 15])],
                 before=[20], behind=[0, 33])
     st.check(st.run())
 
 
 @pytest.mark.parametrize("prefix", [0, 16, 32, 48, 64, 496, 512, 528, 2000, 4096])
-@pytest.mark.parametrize("members", [2, 9, 33])
-def test_lengths(nat, oracle, prefix, members):
-    """Runs of one tile and of many, a last tile that is half empty, rows in one block and in two."""
-    own = [(7 * i) % 50 for i in range(members)]
-    st = Shared(nat, oracle, prefix + members, 8, 2, 64, [(prefix, own)])
+@pytest.mark.parametrize("n", [3, 4, 9, 33])
+@pytest.mark.parametrize("nq", [2, 8])
+def test_lengths(nat, oracle, prefix, n, nq):
+    """Runs of one tile (1 head a kv head) and of several, a last tile that is half empty, rows in one block and in two."""
+    st = Shared(nat, oracle, prefix + n, nq, 2, 64, [(prefix, members(n))])
     st.check(st.run())
 
 
-@pytest.mark.parametrize("members", [1, 16, 17, 32, 64, 65])
-def test_rows(nat, oracle, members):
+@pytest.mark.parametrize("prefix", [0, 16, 64, 496, 2000])
+@pytest.mark.parametrize("n", [2, 9])
+def test_each_by_itself(nat, oracle, prefix, n):
+    """Too few tokens to be attended to together."""
+    st = Shared(nat, oracle, prefix + n, 8, 2, 64, [(prefix, members(n)), (16, [0, 3, 5, 7])], behind=[1200], large=False)
+    st.check(st.run())
+
+
+@pytest.mark.parametrize("nq,nkv,n", [(8, 8, 12), (32, 8, 12), (16, 2, 9)])
+def test_worth_it_alone(nat, oracle, nq, nkv, n):
+    """One group, with fewer common tokens than are attended to together, and with as many."""
+    saved = n * (1.5 if nq > 4 * nkv else 1) - 6
+    few = PAGE * (int(300e3 / (saved * nkv)) // PAGE)
+    for prefix in (few, few + PAGE):
+        st = Shared(nat, oracle, prefix, nq, nkv, 64, [(prefix, members(n))], large=False)
+        st.check(st.run())
+
+
+@pytest.mark.parametrize("n", [1, 4, 16, 17, 32, 64, 65])
+def test_rows(nat, oracle, n):
     """Waves and blocks that the members' heads fill and do not."""
-    st = Shared(nat, oracle, members, 16, 2, 128, [(208, [i % 20 for i in range(members)])])
+    st = Shared(nat, oracle, n, 16, 2, 128, [(208, [i % 20 for i in range(n)])])
     st.check(st.run())
 
 
 def test_long_own_parts(nat, oracle):
     """What lies behind the common tokens in several splits, beside members that have none."""
-    st = Shared(nat, oracle, 1, 8, 2, 64, [(160, [3000, 0, 1500, 1]), (64, [0, 0])], behind=[2500])
+    st = Shared(nat, oracle, 1, 8, 2, 64, [(160, [3000, 0, 1500, 1]), (64, [0, 0, 0, 0])], behind=[2500])
     st.check(st.run())
 
 
 def test_a_long_prefix(nat, oracle):
     """As many runs as the merge takes."""
-    st = Shared(nat, oracle, 2, 4, 1, 64, [(70000, [3, 40])])
+    st = Shared(nat, oracle, 2, 4, 1, 64, [(70000, members(12))], large=False)
     st.check(st.run())
 
 
 def test_nothing_is_shared(nat, oracle):
-    st = Shared(nat, oracle, 3, 8, 2, 64, [], before=[100, 0, 37])
+    st = Shared(nat, oracle, 3, 8, 2, 64, [], before=[100, 0, 37], large=False)
     st.check(st.run())
-    st = Shared(nat, oracle, 3, 8, 2, 64, [(0, [100, 5]), (32, [4])])
-    st.check(st.run())
-    st = Shared(nat, oracle, 3, 8, 2, 64, [(48, []), (32, [4, 5])], behind=[9])      # an empty group
-    st.check(st.run())
+    for large in (False, True):
+        st = Shared(nat, oracle, 3, 8, 2, 64, [(0, [100, 5, 6, 7]), (32, [4])], large=large)
+        st.check(st.run())
+        st = Shared(nat, oracle, 3, 8, 2, 64, [(48, []), (32, [4, 5, 6, 7])], behind=[9], large=large)      # an empty group
+        st.check(st.run())
 
 
 def test_many_groups(nat, oracle):
     """More groups than one launch takes, and more queries than are ranked."""
-    st = Shared(nat, oracle, 4, 2, 1, 64, [(16 * (1 + g % 5), [g % 7, g % 11]) for g in range(70)], before=[3], behind=[4, 5])
+    st = Shared(nat, oracle, 4, 2, 1, 64, [(16 * (1 + g % 5), [g % 7, g % 11, 2, 3][:2 + g % 3]) for g in range(70)],
+                before=[3], behind=[4, 5])
     st.check(st.run())
 
 
 def test_sequences_in_any_order_without_rope(nat, oracle):
-    st = Shared(nat, oracle, 5, 8, 2, 128, [(96, [5, 6, 7]), (32, [40, 1])], before=[3], rope=False,
-                order=[4, 0, 5, 2, 1, 3], max_pos=500)
+    st = Shared(nat, oracle, 5, 8, 2, 128, [(96, [5, 6, 7, 8]), (32, [40, 1, 2, 3, 4])], before=[3], rope=False,
+                order=[4, 0, 5, 9, 2, 1, 8, 3, 7, 6], max_pos=9500)
     st.check(st.run())
 
 
 def test_queries_in_front_of_their_common_tokens_are_left_out(nat, oracle):
-    st = Shared(nat, oracle, 6, 8, 2, 64, [(96, [5, 6, 7, 8])], behind=[10, 20])
-    st.at([101, 95, -1, 104, -1, 20])
-    st.check(st.run())
+    for large in (False, True):
+        st = Shared(nat, oracle, 6, 8, 2, 64, [(96, [5, 6, 7, 8, 9]), (32, [4])], behind=[10, 20], large=large)
+        st.at([101, 95, -1, 96, 0, 31, *st.pos[6:-2], -1, 20])
+        st.check(st.run())
 
 
 def test_equal_results_every_time(nat, oracle):
-    st = Shared(nat, oracle, 7, 32, 8, 128, [(1024, [i for i in range(40)])])
+    st = Shared(nat, oracle, 7, 32, 8, 128, [(1152, [i for i in range(40)])], large=False)
     first = st.run()
     assert np.array_equal(first, st.run())
     st.check(first)
@@ -181,7 +226,7 @@ def test_equal_results_every_time(nat, oracle):
 
 def test_values_of_very_different_sizes(nat, oracle):
     """Scales of common tokens from 2^-60 to 2^60, in one tile and across tiles: each term keeps its bits."""
-    st = Shared(nat, oracle, 8, 8, 2, 64, [(256, [3, 30])])
+    st = Shared(nat, oracle, 8, 8, 2, 64, [(256, [3, 30, 0, 9])])
     c, page = st.c, st.c.pages[0]
     r = np.random.default_rng(1)
     sizes = np.float32(2.0) ** r.integers(-60, 60, (8, c.nkv, PAGE, c.nb)).astype(np.float32)
@@ -193,7 +238,7 @@ def test_values_of_very_different_sizes(nat, oracle):
 
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 def test_a_block_that_is_no_number_stays_in_its_columns(nat, oracle, bad):
-    st = Shared(nat, oracle, 9, 8, 2, 64, [(256, [3, 30, 7])], behind=[40])
+    st = Shared(nat, oracle, 9, 8, 2, 64, [(256, [3, 30, 7, 0])], behind=[40])
     clean = st.run()
     c = st.c
     c.pool["d"][c.pages[0][3], 1, 1, 5, 1] = bad       # token 53's value, kv head 1, second block
@@ -201,7 +246,7 @@ def test_a_block_that_is_no_number_stays_in_its_columns(nat, oracle, bad):
     out = st.run()
     st.check(out, finite=False)
     hit = np.zeros(out.shape, bool)
-    hit[:3, 4:, 32:] = True
+    hit[:4, 4:, 32:] = True
     if np.isnan(bad):
         assert np.isnan(out[hit]).all()
     else:
@@ -210,18 +255,18 @@ def test_a_block_that_is_no_number_stays_in_its_columns(nat, oracle, bad):
 
 
 def test_a_key_that_is_no_number_is_seen(nat, oracle):
-    st = Shared(nat, oracle, 10, 8, 2, 64, [(64, [3, 30])], behind=[40])
+    st = Shared(nat, oracle, 10, 8, 2, 64, [(64, [3, 30, 7, 0])], behind=[40])
     clean = st.run()
     st.c.pool["d"][st.c.pages[0][1], 0, 0, 2, 0] = np.nan
     out = st.run()
-    assert np.isnan(out[:2, :4]).all()
-    assert np.array_equal(out[:, 4:], clean[:, 4:]) and np.array_equal(out[2], clean[2])
+    assert np.isnan(out[:4, :4]).all()
+    assert np.array_equal(out[:, 4:], clean[:, 4:]) and np.array_equal(out[4:], clean[4:])
 
 
 def test_captured_and_two_at_once(nat, oracle):
     g, other = Graphs(), Graphs()
-    a = Shared(nat, oracle, 11, 8, 2, 64, [(160, [5, 6, 60])], room=20, max_pos=250)
-    b = Shared(nat, oracle, 12, 8, 2, 128, [(320, [i for i in range(20)])], room=20, max_pos=400)
+    a = Shared(nat, oracle, 11, 8, 2, 64, [(160, [5, 6, 60, 0])], room=20, max_pos=8500)
+    b = Shared(nat, oracle, 12, 8, 2, 128, [(320, [i for i in range(20)])], room=20, max_pos=8500)
     for st in (a, b):
         st.c.upload()
     ga, gb = g.capture(a.launch), other.capture(b.launch)
@@ -232,16 +277,15 @@ def test_captured_and_two_at_once(nat, oracle):
         for st in (a, b):
             st.check(st.results())
             st.at([p + 1 + turn for p in st.pos])
-            st.c.put(0, (), ())
             # (a turn leaves gaps of rows that no step wrote: what the cache holds there counts)
 
 
 def test_a_conversation_under_a_prompt(nat, oracle):
     """A prompt prefilled once, its pages mapped into every sequence, questions packed behind it, then steps together."""
-    nq, nkv, hd, prompt, turns = 8, 2, 64, 96, [5, 17, 1]
-    st = Shared(nat, oracle, 13, nq, nkv, hd, [(prompt, turns)], room=8, max_pos=200)
+    nq, nkv, hd, prompt, turns = 8, 2, 64, 96, [5, 17, 1, 9]
+    st = Shared(nat, oracle, 13, nq, nkv, hd, [(prompt, turns)], room=8, max_pos=8500)
     c, r = st.c, st.c.r
-    for pos0, lens, seqs in (([0], [prompt], [0]), ([prompt] * 3, turns, [0, 1, 2])):
+    for pos0, lens, seqs in (([0], [prompt], [0]), ([prompt] * len(turns), turns, range(len(turns)))):
         rows = sum(lens)
         q, k, v = (r.standard_normal((rows, h, hd), dtype=np.float32) for h in (nq, nkv, nkv))
         at = [b + j for b, m in zip(pos0, lens) for j in range(m)]
