@@ -1171,7 +1171,7 @@ namespace {
 // Most runs of a group's common tokens, and splits of what lies behind them: the merge
 // holds 128 slots.
 constexpr int kSharedRuns = 64;
-// Fewest queries of a group that attend to its tokens together.
+// Fewest queries of a group that attend to its tokens together (or SharedPlan::far).
 constexpr int kFewestMembers = 4;
 
 // How a step with common tokens is cut: what each group shares, in runs of `chunk` key
@@ -1179,7 +1179,10 @@ constexpr int kFewestMembers = 4;
 struct SharedPlan {
     bool together = false;
     // What a group attends to together: all of its common tokens, or none.
-    int common(int members, int prefix) const { return together && members >= kFewestMembers ? prefix : 0; }
+    int common(int members, int prefix) const {
+        return together && (members >= kFewestMembers || (members >= 2 && prefix > far)) ? prefix : 0;
+    }
+    double far = 0.0;        // a prefix that is long for two queries, too
     long chunk = 1;
     int runs = 0;            // most runs of a group
     int split_tokens, n_splits, slots;
@@ -1230,19 +1233,34 @@ void plan_shared(const tq_hip_kv *kv, int n_q, int max_pos, int n_groups, const 
     const tq_hip_kv_desc &D = kv->desc;
     const int g = D.n_q_heads / D.n_kv_heads;
     p.together = worth_sharing(kv, n_groups, start, prefix);
-    long steps = 0, grouped = 0, apart = 0, longest = 0;   // key tiles of rows; queries; tokens that a query attends to by itself
-    int least = INT32_MAX, deepest = 0, most = 0;
+    const long whole = (long)max_pos + 1;
+    long grouped = 0, apart = 0;   // queries; tokens that queries attend to by themselves
+    int deepest = 0;
+    for (int i = 0; i < n_groups; i++) {
+        const int members = start[i + 1] - start[i];
+        grouped += members;
+        if (members > 0) deepest = std::max(deepest, (int)prefix[i]);
+        if (!p.together || members < kFewestMembers) apart += (long)members * prefix[i];
+    }
+    apart += grouped * (whole - deepest) + (n_q - grouped) * whole;
+    // what each of the 512 work-groups that run at once has of them
+    double even = (double)apart * D.n_kv_heads / 512;
+    // Two or three queries would keep a few work-groups busy for long behind far more
+    // common tokens than that (groups of 12, 3 and 33 behind 16,384, 7,680 and 864, 64 / 8
+    // heads: by themselves 92 us, together 80), but not where many are like them
+    // (20 groups, five of 3 queries behind up to 4,096: 78 and 87)
+    p.far = 4.0 * even;
+    long steps = 0, longest = 0;   // key tiles of rows; most common tokens that a query attends to by itself
+    int least = INT32_MAX, most = 0;
     for (int i = 0; i < n_groups; i++) {
         const int members = start[i + 1] - start[i];
         if (members == 0) continue;
         const int common = p.common(members, prefix[i]);
         least = std::min(least, common);
         most = std::max(most, common);
-        deepest = std::max(deepest, (int)prefix[i]);
         longest = std::max(longest, (long)prefix[i] - common);
         steps += tq_shared_steps(members, g, common);
-        grouped += members;
-        apart += (long)members * (prefix[i] - common);
+        if (members < kFewestMembers) even -= (double)members * common * D.n_kv_heads / 512;
     }
     if (grouped < n_q) least = 0;
     // one work-group per CU, the queries' own beside it, where the tiles are few: each
@@ -1258,15 +1276,13 @@ void plan_shared(const tq_hip_kv *kv, int n_q, int max_pos, int n_groups, const 
     // Where a few have much more than the others, common tokens of a small group, more
     // splits shorten what the last of them takes (0.75 us for 128 tokens, if the 512
     // work-groups that run at once do not have as much each), and those behind the
-    // others' ends cost their start (3.5 us for 512).  Groups of 12, 3 and 33 behind
-    // 16,384, 7,680 and 864 common tokens, 64 / 8 heads: 2 splits 143 us, 5 92.
-    const long whole = (long)max_pos + 1, own = whole - deepest, pairs = (long)n_q * D.n_kv_heads;
-    apart += grouped * own + (n_q - grouped) * whole;
-    longest = grouped < n_q ? whole : longest + own;
+    // others' ends cost their start (3.5 us for 512).  24 queries in groups of 7, 8, 3 and
+    // 4 behind 2,000-12,600 tokens and two alone, 32 / 8 heads: 3 splits 83 us, 10 65.
+    const long pairs = (long)n_q * D.n_kv_heads;
+    longest = grouped < n_q ? whole : longest + whole - deepest;
     const int max_len = (int)(whole - least);
     plan_splits3(kv, n_q, max_len, kSharedWaves, decode_wg_target(n_q), &p.split_tokens, &p.n_splits);
     const int unit = 32 * kSharedWaves;
-    const double even = (double)apart * D.n_kv_heads / 512;
     double best = 1e30;
     for (int n = p.n_splits; n <= tq_decode3_max_splits(); n++) {
         const int tokens = ((max_len + n - 1) / n + unit - 1) / unit * unit;
