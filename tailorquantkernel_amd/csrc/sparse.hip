@@ -67,15 +67,21 @@ __global__ __launch_bounds__(kThreads) void bounds_kernel(TqBoundsArgs a) {
                 d[s] = *reinterpret_cast<const float *>(p);
                 c[s] = *reinterpret_cast<const uint32_t *>(p + 4 + word % 8 * 4);
             }
+            // (the max and min of a number and NaN are the number: a row behind the
+            // end counts as one whose scale is NaN)
 #pragma unroll
-            for (int s = 0; s < STEPS; s++) {
-                const bool there = t0 + s * RPI + sub < t1;
+            for (int s = 0; s < STEPS; s++) d[s] = t0 + s * RPI + sub < t1 ? d[s] : __builtin_nanf("");
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
+            for (int j = 0; j < 4; j++) {
+                float up = (float)(int8_t)(c[0] >> (8 * j)) * d[0], down = up;
+#pragma unroll
+                for (int s = 1; s < STEPS; s++) {
                     const float key = (float)(int8_t)(c[s] >> (8 * j)) * d[s];
-                    most[j] = there ? fmaxf(most[j], key) : most[j];
-                    least[j] = there ? fminf(least[j], key) : least[j];
+                    up = fmaxf(up, key);
+                    down = fminf(down, key);
                 }
+                most[j] = fmaxf(most[j], up);
+                least[j] = fminf(least[j], down);
             }
         }
         // over the lanes of the other rows
