@@ -30,8 +30,6 @@ struct Frequencies {
     int pairs;
 };
 
-typedef float v2f_any __attribute__((ext_vector_type(2), aligned(4)));
-
 struct CosSin {
     float c, s;
 };
@@ -122,11 +120,15 @@ __device__ __forceinline__ float lanes_sum(float x) {
     return x;
 }
 
-// Grid (row, chunk of U * 256 / LANES heads): LANES lanes have a head, four values each.
-// Bound by reading and writing the heads.  With whole pairs in a lane (rot a multiple
-// of 4) lane l < rot / 4 has pairs 2 l and 2 l + 1; otherwise values 4 l .. 4 l + 3,
-// and it reads their partners too, which is rare enough.  A head lies in one wave,
-// whose loads all come before its stores: in place is safe either way.
+// Grid (row, chunk of U * 256 / LANES heads): LANES lanes have a head, values 4 l .. 4 l + 3
+// each.  The partners of neighbouring pairs are in the lane (rot a multiple of 4), those
+// of halves in another lane of the wave (a multiple of 8); otherwise a lane reads its
+// partners too, which is rare enough.  A head lies in one wave, whose loads all come before
+// its stores: in place is safe either way.
+//   Bound by reading and writing the heads: 4,096 rows of 64 and 8 heads of 128 (302 MB) in
+// 67 us, 8,192 in 124 (4.9 TB/s, where a copy of as much reaches 5.3), 64 rows of 32 and 8
+// in 6.5, the launch and the angles.  Stores past the caches (nontemporal) took 2,048 rows
+// from 36 to 24 us and 4,096 from 72; loads past them undo that (34).
 enum { kHalves, kNeighbours, kAny };
 template <int LANES, int U, int FORM>
 __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int interleaved) {
@@ -136,9 +138,9 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int inte
     const size_t row = blockIdx.x;
     const int hd = a.head_dim, rot = a.rot;
     const bool in = 4 * l < hd;
-    const bool turns = FORM == kAny ? 4 * l < rot : l < rot / 4;
-    // places of this lane's values: 0, 1 and 2, 3 neighbours
-    const int e0 = FORM == kHalves && turns ? 2 * l : 4 * l, e2 = FORM == kHalves && turns ? rot / 2 + 2 * l : 4 * l + 2;
+    const bool turns = 4 * l < rot, upper = 8 * l >= rot;
+    // (FORM kHalves) the lane of this lane's partners
+    const int other = (tid & 63) + (!turns ? 0 : upper ? -rot / 8 : rot / 8);
     // (FORM kAny) the partner of value 4 l + j
     int mate[4];
     if constexpr (FORM == kAny) {
@@ -163,13 +165,8 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int inte
         for (int j = 0; j < 4; j++) x[u][j] = y[u][j] = 0.0f;
         if (out[u]) {
             const float *src = t.x + row * t.stride + (size_t)h * hd;
-            if constexpr (FORM == kHalves) {
-                const v2f_any lo = *reinterpret_cast<const v2f_any *>(src + e0), up = *reinterpret_cast<const v2f_any *>(src + e2);
-                x[u][0] = lo.x, x[u][1] = lo.y, x[u][2] = up.x, x[u][3] = up.y;
-            } else {
-                const v4f_any v = *reinterpret_cast<const v4f_any *>(src + e0);
-                x[u][0] = v.x, x[u][1] = v.y, x[u][2] = v.z, x[u][3] = v.w;
-            }
+            const v4f_any v = *reinterpret_cast<const v4f_any *>(src + 4 * l);
+            x[u][0] = v.x, x[u][1] = v.y, x[u][2] = v.z, x[u][3] = v.w;
             if constexpr (FORM == kAny) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) y[u][j] = src[mate[j]];
@@ -187,19 +184,21 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int inte
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const float sum = lanes_sum<LANES>((x[u][0] * x[u][0] + x[u][1] * x[u][1]) + (x[u][2] * x[u][2] + x[u][3] * x[u][3]));
-        if (!out[u]) continue;
-        if (weight[u]) {
+        if (weight[u] && out[u]) {
             const float inv = 1.0f / sqrtf(a.eps + sum / (float)hd);
             const float *w = weight[u];
-            const int e[4] = {e0, e0 + 1, e2, e2 + 1};
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                x[u][j] = x[u][j] * inv * w[e[j]];
+                x[u][j] = x[u][j] * inv * w[4 * l + j];
                 if constexpr (FORM == kAny) y[u][j] = y[u][j] * inv * w[mate[j]];
             }
         }
-        float *dst = out[u];
         float *v = x[u];
+        if constexpr (FORM == kHalves) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[u][j] = __shfl(v[j], other);
+        }
+        if (!out[u]) continue;
         if constexpr (FORM == kAny) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -209,22 +208,20 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int inte
                 const bool lower = interleaved ? !(e & 1) : e < rot / 2;
                 v[j] = lower ? v[j] * cs[i] - y[u][j] * sn[i] : y[u][j] * sn[i] + v[j] * cs[i];
             }
+        } else if (turns && FORM == kHalves) {
+            const int i = 4 * l - (upper ? rot / 2 : 0);
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = v[j] * cs[i + j] + y[u][j] * (upper ? sn[i + j] : -sn[i + j]);
         } else if (turns) {
-            const float c0 = cs[2 * l], s0 = sn[2 * l], c1 = cs[2 * l + 1], s1 = sn[2 * l + 1];
-            // (first, second) of pair 0 and of pair 1
-            const int b0 = FORM == kHalves ? 2 : 1, a1 = FORM == kHalves ? 1 : 2;
-            const float p0 = v[0], p1 = v[b0], q0 = v[a1], q1 = v[3];
-            v[0] = p0 * c0 - p1 * s0;
-            v[b0] = p0 * s0 + p1 * c0;
-            v[a1] = q0 * c1 - q1 * s1;
-            v[3] = q0 * s1 + q1 * c1;
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
+                const float c = cs[2 * l + j / 2], s = sn[2 * l + j / 2], p0 = v[j], p1 = v[j + 1];
+                v[j] = p0 * c - p1 * s;
+                v[j + 1] = p0 * s + p1 * c;
+            }
         }
-        if constexpr (FORM == kHalves) {
-            *reinterpret_cast<v2f_any *>(dst + e0) = v2f_any{v[0], v[1]};
-            *reinterpret_cast<v2f_any *>(dst + e2) = v2f_any{v[2], v[3]};
-        } else {
-            *reinterpret_cast<v4f_any *>(dst + e0) = v4f_any{v[0], v[1], v[2], v[3]};
-        }
+        const v4f_any r{v[0], v[1], v[2], v[3]};
+        __builtin_nontemporal_store(r, reinterpret_cast<v4f_any *>(out[u] + 4 * l));
     }
 }
 
@@ -285,7 +282,7 @@ template <int LANES, int U>
 void launch_norm_rope(const NormRopeArgs &a, int interleaved, int n, hipStream_t s) {
     constexpr int PER = 256 / LANES * U;
     const dim3 grid((unsigned)n, (unsigned)((a.heads + PER - 1) / PER));
-    if (a.rot % 4)
+    if (a.rot % (interleaved ? 4 : 8))
         hipLaunchKernelGGL((norm_rope_kernel<LANES, U, kAny>), grid, dim3(256), 0, s, a, interleaved);
     else if (interleaved)
         hipLaunchKernelGGL((norm_rope_kernel<LANES, U, kNeighbours>), grid, dim3(256), 0, s, a, interleaved);
@@ -295,12 +292,16 @@ void launch_norm_rope(const NormRopeArgs &a, int interleaved, int n, hipStream_t
 
 template <int LANES>
 void launch_norm_rope(const NormRopeArgs &a, int interleaved, int n, hipStream_t s) {
-    // four heads in flight per lane where that leaves work-groups enough for the CUs
-    const long wgs = (long)n * ((a.heads + 256 / LANES * 4 - 1) / (256 / LANES * 4));
-    if (wgs >= 1024)
-        launch_norm_rope<LANES, 4>(a, interleaved, n, s);
-    else
-        launch_norm_rope<LANES, 1>(a, interleaved, n, s);
+    // up to four heads in flight per lane where that leaves work-groups enough for the
+    // CUs, and a row's work-groups with equally many (8,192 rows of 72 heads of 128: three
+    // 124 us, four 125 with lanes that have none, two 130, one 146)
+    const int sets = (a.heads + 256 / LANES - 1) / (256 / LANES), wgs = (sets + 3) / 4;
+    switch ((long)n * wgs >= 1024 ? (sets + wgs - 1) / wgs : 1) {
+        case 1: return launch_norm_rope<LANES, 1>(a, interleaved, n, s);
+        case 2: return launch_norm_rope<LANES, 2>(a, interleaved, n, s);
+        case 3: return launch_norm_rope<LANES, 3>(a, interleaved, n, s);
+        default: return launch_norm_rope<LANES, 4>(a, interleaved, n, s);
+    }
 }
 
 int herr(hipError_t e) { return e == hipSuccess ? TQ_HIP_OK : TQ_HIP_EHIP_BASE - (int)e; }
