@@ -183,11 +183,12 @@ def test_in_place_and_unaligned_give_the_same(nat, hd, nq, nk, rot, layout):
             assert np.array_equal(whole[:, (nq + nk) * hd:], x[:, (nq + nk) * hd:])
 
 
-@pytest.mark.parametrize("n", [1, 511, 513, 3001])
-def test_many_rows(nat, n):
-    """Both numbers of heads a lane takes, and rows either side of where they change."""
+@pytest.mark.parametrize("n,nq,nk", [(1, 32, 8), (511, 32, 8), (513, 32, 8), (3001, 32, 8), (1030, 6, 1), (1030, 9, 2),
+                                     (1030, 20, 1), (1030, 28, 4), (400, 64, 8)])
+def test_many_rows(nat, n, nq, nk):
+    """Every number of heads that a lane takes, and rows either side of where it changes."""
     r = np.random.default_rng(n)
-    hd, nq, nk = 128, 32, 8
+    hd = 128
     x = r.standard_normal((n, (nq + nk) * hd)).astype(np.float32)
     weights = [r.standard_normal(hd).astype(np.float32) for _ in range(2)]
     pos = r.integers(0, 100000, n).astype(np.int32)
