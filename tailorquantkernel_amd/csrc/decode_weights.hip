@@ -1,5 +1,5 @@
 // decode_weights.hip — the second half of a decode step that gathers attention
-// weights over several splits (decode3.hip with scores): their partials become the
+// weights over several splits (decode3.hpp with scores): their partials become the
 // output rows, and the scores become weights, which are added to the totals
 // that eviction goes by.  No counterpart in the reference.
 //

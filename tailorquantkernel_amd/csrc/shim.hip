@@ -132,7 +132,7 @@ void plan_splits(const tq_hip_kv *kv, int n_q, int max_len, int *split_tokens, i
     *n_splits = (chunks + per - 1) / per;
 }
 
-// Which decode kernel serves a call: the MFMA kernel (decode3.hip) wherever it
+// Which decode kernel serves a call: the MFMA kernel (decode3.hpp) wherever it
 // covers the shape, else the VALU kernel (decode.hip).  TQ_HIP_DECODE_KERNEL=1
 // forces the VALU kernel (for comparisons).
 bool use_decode3(const tq_hip_kv *kv) {
