@@ -59,7 +59,7 @@ __device__ __forceinline__ CosSin cos_sin(int pos, double f, double magnitude) {
 }
 
 // Four consecutive values of the flat [n][pairs] arrays per thread.  Bound by the launch
-// (64 rows of 64 pairs in 2.8 us) and by the angles and the stores alike (33,000 rows, 17 MB,
+// (64 rows of 64 pairs in 2.8 us) and by the angles and the stores alike (32,768 rows, 17 MB,
 // in 7.3).
 __global__ __launch_bounds__(256) void rope_rows_kernel(Frequencies a, const int32_t *pos, size_t total, float *cos_t,
                                                         float *sin_t) {

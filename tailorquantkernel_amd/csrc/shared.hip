@@ -18,8 +18,8 @@
 //   products and the next scores, 0.15 the barrier; with a wave per SIMD the vector pipe
 //   is busy 44% of the time, the matrix pipe 18%.  In front of the first 8 us pass (the
 //   page table, the queries' quantization, the first tile from memory), and the merge
-//   takes 6.6.  64 queries of 32 / 8 heads of 128 behind 4,096 common tokens 44 us (75 each
-//   by itself), behind 16,384 92 (270).  Work-groups of eight waves and 256 rows, half of
+//   takes 6.6.  64 queries of 32 / 8 heads of 128 behind 4,096 common tokens 44 us (77 each
+//   by itself), behind 16,384 92.  Work-groups of eight waves and 256 rows, half of
 //   them on either image, were slower but for the longest prefixes (58 and 89 us): their
 //   LDS leaves no room for the queries' own work-groups beside them.
 #include <algorithm>
@@ -251,16 +251,22 @@ __device__ __forceinline__ void prefix_run(const SharedArgs &sh, const int x, Pr
     const int run = (int)(mine / blocks), row0 = (int)(mine - run * blocks) * kRows;
     // the run's tiles
     const int kt0 = run * sh.chunk, nt = min(sh.chunk, (prefix + kKT - 1) / kKT - kt0);
-    const int seq = a.seq_of ? a.seq_of[first] : first;
-    const bool seq_ok = seq >= 0 && seq < a.view.max_seqs;
-    const int32_t *table = a.view.page_table + (seq_ok ? (size_t)seq * a.view.max_pages : 0);
+    // the pages by the table of the first query that is not left out
+    int seq = -1;
+    for (int m0 = 0; seq < 0 && m0 < t_.members[g]; m0 += 64) {
+        const int m = first + min(m0 + lane, t_.members[g] - 1), s = a.seq_of ? a.seq_of[m] : m;
+        const unsigned long long there = __builtin_amdgcn_ballot_w64(a.len_of[m] >= prefix && s >= 0 && s < a.view.max_seqs);
+        if (there) seq = __builtin_amdgcn_readlane(s, __builtin_ctzll(there));
+    }
+    if (seq < 0) return;
+    const int32_t *table = a.view.page_table + (size_t)seq * a.view.max_pages;
     // Copies of a tile's K rows, or its V rows, by the work-group from its two pages' runs.
     // The pages' ids, lanes 0 and 1 of a vector load (a scalar one would hold up every LDS
     // read until it is back), are read a step before the copies that go by them.
     const unsigned char *head0 = a.view.pool + (size_t)kvh * a.view.head_run;
     auto ids_of = [&](int t) {
         const int lp = 2 * (kt0 + t) + (thread_now() & 1);
-        return seq_ok && lp < a.view.max_pages ? table[lp] : 0;
+        return lp < a.view.max_pages ? table[lp] : 0;
     };
     auto fetch = [&](int ids, size_t part, unsigned char *to) {
         const uint32_t off = 16 * (thread_now() & 63);

@@ -217,6 +217,24 @@ def test_queries_in_front_of_their_common_tokens_are_left_out(nat, oracle):
         st.check(st.run())
 
 
+@pytest.mark.parametrize("idle", [1, 3, 70])
+def test_the_first_of_a_group_may_be_idle(nat, oracle, idle):
+    """No sequence, or one that has not come to its common tokens: their pages are those of the first that has."""
+    n = idle + 5
+    st = Shared(nat, oracle, idle, 8, 2, 64, [(2064, members(n))], behind=[4], order=list(range(n)))
+    st.at([-1] * idle + st.pos[idle:])
+    seqs = np.asarray(st.order, np.int32)
+    seqs[:idle] = -1
+    if idle == 3:
+        st.at([700, -1, 5000] + st.pos[idle:])
+        seqs[:3] = 0, 10 ** 6, -7
+    st.dev["seq"].upload(seqs)
+    out = st.run()
+    if idle == 3:
+        st.pos[2], out[2] = -1, 3.0     # (a query of no sequence appends nothing, and its row says nothing)
+    st.check(out)
+
+
 def test_equal_results_every_time(nat, oracle):
     st = Shared(nat, oracle, 7, 32, 8, 128, [(1152, [i for i in range(40)])], large=False)
     first = st.run()
