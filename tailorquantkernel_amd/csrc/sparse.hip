@@ -278,13 +278,16 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
     return x + (row > 0 ? r0 : 0u) + (row > 1 ? r1 : 0u) + (row > 2 ? r2 : 0u);
 }
 
-// Grid (kv head, query).  SCORED: the keys are in the workspace; else this work-group
-// makes them, in LDS.
-template <int HD, int WAVES, bool SCORED>
+// Grid (kv head, query).  This work-group makes the keys, in LDS (kMade), or score_kernel
+// did, in the workspace: up to kKeysInLds of them are copied from there (kCopied: each of
+// some six looks at them would wait for the L2; 4,096 blocks of 1 query 17.5 us and 20.9,
+// of 8 36.8 and 40.1, 1,024 of 1 11.9 and 12.3).
+enum { kMade, kCopied, kKept };
+template <int HD, int WAVES, int KEYS>
 __global__ __launch_bounds__(64 * WAVES) void select_kernel(TqSelectArgs a) {
     constexpr int THREADS = 64 * WAVES, BPT = kBins / THREADS;
-    __shared__ uint64_t lds_keys[SCORED ? 1 : kKeysInLds];
-    __shared__ SumsLds<SCORED ? 32 : HD> sums;
+    __shared__ uint64_t lds_keys[KEYS == kKept ? 1 : kKeysInLds];
+    __shared__ SumsLds<KEYS == kMade ? HD : 32> sums;
     __shared__ uint32_t hist[kBins];
     __shared__ uint32_t w_lo[WAVES], w_hi[WAVES];
     __shared__ uint32_t w_n[WAVES], w_m[WAVES];
@@ -294,23 +297,23 @@ __global__ __launch_bounds__(64 * WAVES) void select_kernel(TqSelectArgs a) {
     const size_t pair = (size_t)qi * a.view.n_kv_heads + kvh;
     int32_t *list = a.list + pair * a.keep;
     // (the sums wait for nothing; where every block is chosen they are made for nothing)
-    constexpr int H = SCORED ? 32 : HD;
+    constexpr int H = KEYS == kMade ? HD : 32;
     Sums<H> q;
-    if constexpr (!SCORED) load_sums<HD>(a, qi, kvh, sums, q);
+    if constexpr (KEYS == kMade) load_sums<HD>(a, qi, kvh, sums, q);
     const Choice c = choice_of(a, qi);
     if (c.all) {
         for (int j = tid; j < a.keep; j += THREADS) list[j] = j < c.count ? j : -1;
         return;
     }
     const int begin = a.sinks, end = c.count - a.recent;     // the candidates
-    const uint64_t *keys;
-    if constexpr (SCORED) {
-        keys = a.keys + pair * a.key_stride;
-    } else {
-        score_blocks<HD>(a, c.seq, kvh, q, begin, end, lds_keys);
-        keys = lds_keys;
-        __syncthreads();
+    const uint64_t *kept = a.keys + pair * a.key_stride;
+    const uint64_t *keys = KEYS == kKept ? kept : lds_keys;
+    if constexpr (KEYS == kMade) score_blocks<HD>(a, c.seq, kvh, q, begin, end, lds_keys);
+    if constexpr (KEYS == kCopied) {
+#pragma unroll 4
+        for (int b = begin + tid; b < end; b += THREADS) lds_keys[b] = kept[b];
     }
+    if constexpr (KEYS != kKept) __syncthreads();
     // f(first block of 64, this lane's key, 0 for no candidate) over this wave's run
     const int per = ((end - begin + 63) / 64 + WAVES - 1) / WAVES;
     auto each = [&](auto f) {
@@ -431,7 +434,7 @@ template <int HD>
 hipError_t launch_select(const TqSelectArgs &a, hipStream_t s) {
     const dim3 grid((unsigned)a.view.n_kv_heads, (unsigned)a.n_q);
     if (a.chunk == 0) {
-        hipLaunchKernelGGL((select_kernel<HD, 8, false>), grid, dim3(512), 0, s, a);
+        hipLaunchKernelGGL((select_kernel<HD, 8, kMade>), grid, dim3(512), 0, s, a);
         return hipGetLastError();
     }
     const int blocks = a.max_pos / a.block + 1;
@@ -439,7 +442,10 @@ hipError_t launch_select(const TqSelectArgs &a, hipStream_t s) {
                        s, a, a.chunk);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((select_kernel<HD, 8, true>), grid, dim3(512), 0, s, a);
+    if (blocks <= kKeysInLds)
+        hipLaunchKernelGGL((select_kernel<HD, 8, kCopied>), grid, dim3(512), 0, s, a);
+    else
+        hipLaunchKernelGGL((select_kernel<HD, 8, kKept>), grid, dim3(512), 0, s, a);
     return hipGetLastError();
 }
 
@@ -463,7 +469,7 @@ hipError_t tq_launch_bounds(const TqBoundsArgs &a, hipStream_t s) {
 // A launch of its own for the scores takes about 3 us and pays where the selecting
 // work-groups, one per (query, kv head), leave most CUs idle over many blocks.  32 / 8
 // heads of 128, in one launch and in two: 1,024 blocks of 1 query 16.1 and 11.4 us, 8
-// queries 19.1 and 16.4, 16 queries 20.3 and 21.1; 4,096 blocks of 1 query 45 and 20, 16
+// queries 19.1 and 16.4, 16 queries 20.3 and 21.1; 4,096 blocks of 1 query 45 and 17.5, 16
 // queries 69 and 69; 256 blocks 8.9 .. 10.9 and 10.0 .. 13.0.
 int tq_select_chunk(int n_q, int n_kv_heads, int blocks) {
     const long pairs = (long)n_q * n_kv_heads;
