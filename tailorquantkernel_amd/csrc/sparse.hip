@@ -430,14 +430,22 @@ __global__ __launch_bounds__(64 * WAVES) void select_kernel(TqSelectArgs a) {
     });
 }
 
+// Four waves for up to 512 blocks, eight for more (four and eight, 32 / 8 heads of 128: 250
+// blocks of 64 queries 17.0 and 22.2 us, of 1 8.9 and 9.0, 500 of 64 27.3 and 31.2, of 1
+// 12.0 and 11.9; 2,000 of 16 34.9 and 34.0, 4,062 of 64 205 and 193).
+constexpr int kFewBlocks = 512;
+
 template <int HD>
 hipError_t launch_select(const TqSelectArgs &a, hipStream_t s) {
     const dim3 grid((unsigned)a.view.n_kv_heads, (unsigned)a.n_q);
+    const int blocks = a.max_pos / a.block + 1;
     if (a.chunk == 0) {
-        hipLaunchKernelGGL((select_kernel<HD, 8, kMade>), grid, dim3(512), 0, s, a);
+        if (blocks <= kFewBlocks)
+            hipLaunchKernelGGL((select_kernel<HD, 4, kMade>), grid, dim3(256), 0, s, a);
+        else
+            hipLaunchKernelGGL((select_kernel<HD, 8, kMade>), grid, dim3(512), 0, s, a);
         return hipGetLastError();
     }
-    const int blocks = a.max_pos / a.block + 1;
     hipLaunchKernelGGL(score_kernel<HD>, dim3((unsigned)((blocks + a.chunk - 1) / a.chunk), grid.x, grid.y), dim3(kThreads), 0,
                        s, a, a.chunk);
     const hipError_t e = hipGetLastError();
@@ -473,7 +481,7 @@ hipError_t tq_launch_bounds(const TqBoundsArgs &a, hipStream_t s) {
 // queries 69 and 69; 256 blocks 8.9 .. 10.9 and 10.0 .. 13.0.
 int tq_select_chunk(int n_q, int n_kv_heads, int blocks) {
     const long pairs = (long)n_q * n_kv_heads;
-    if (blocks <= 512 || (blocks <= kKeysInLds && pairs >= 128)) return 0;
+    if (blocks <= kFewBlocks || (blocks <= kKeysInLds && pairs >= 128)) return 0;
     return (int)std::min(256L, (pairs * blocks + 64 * 256 - 1) / (64 * 256) * 64);
 }
 

@@ -227,6 +227,15 @@ def test_select_lengths(nat, oracle, blocks, keep):
     assert np.array_equal(s.run(), s.expected())
 
 
+@pytest.mark.parametrize("blocks", [511, 512, 513, 1030, 4096, 4097])
+@pytest.mark.parametrize("hd", [32, 128])
+def test_select_for_a_batch(nat, oracle, blocks, hd):
+    """Heads enough that scores get no launch of their own, up to the length where they do."""
+    pos = [16 * blocks - 1, *(int(p) for p in np.random.default_rng(blocks).integers(0, 16 * blocks, 15))]
+    s = Select(nat, oracle, blocks, 8, 8, hd, pos, 16, 70, 2, 3, rope=False)
+    assert np.array_equal(s.run(), s.expected())
+
+
 def test_select_among_equals(nat, oracle):
     """Equal scores go to the lower block, also where many share the edge and where all do."""
     s = Select(nat, oracle, 1, 4, 2, 64, [6400, 6400, 6400, 6400], 16, 40, 1, 2, rope=False)
