@@ -308,23 +308,23 @@ int tq_hip_decode_step_weights_async(tq_hip_kv *kv, int n_q, const int32_t *d_se
 /* The same step for a batch in which groups of queries share the tokens that their
  * sequences begin with, a system prompt or a document (no counterpart in the
  * reference): queries start[g] .. start[g + 1] - 1 are group g, and the first
- * prefix[g] tokens of its sequences, a multiple of TQ_HIP_PAGE_TOKENS, lie in the same
- * pages, which may be read once for the group, through the page table of the first of
- * its queries that is not left out: the call does so where that is faster (12 queries
- * with 8,192 common tokens or 32 with 2,048 are enough), by a choice that n_q, max_pos,
- * start and prefix make, and else each query goes by its own table.  Of what is read
- * together products are kept to 2^-20 of themselves, as in the packed prefill, and no
- * terms below 2^-28 of a row's largest V scale; the rest is as in the steps above.  Queries
- * before start[0] and from start[n_groups] on share nothing.  start (n_groups + 1
- * entries, none less than the one before, the last at most n_q) and prefix are HOST
- * arrays, read during the call: a captured call keeps its groups, while d_seq, d_pos
- * and the pages may change.  A query whose d_pos[i] is below its prefix is left out:
- * nothing is appended, and its output row stays.  A sequence appears at most once per
- * call, and its new token's page is its own.
- * Head dims 64/128 with groups of 1..8 heads, TQ_HIP_ETYPE otherwise; fp32 arrays
- * 16-byte aligned.  d_ws: tq_hip_decode_step_shared_ws_bytes for the same n_q,
- * max_pos and groups (0: a call that is refused), 16-byte aligned, nothing is kept
- * in it between calls. */
+ * prefix[g] tokens of its sequences, a multiple of TQ_HIP_PAGE_TOKENS and at most
+ * max_pos, lie in the same pages, which may be read once for the group, through the
+ * page table of the first of its queries that is not left out: the call does so where
+ * that is faster (12 queries with 8,192 common tokens or 32 with 2,048 are enough),
+ * by a choice that n_q, max_pos, start and prefix make, and else each query goes by
+ * its own table.  Of what is read together products are kept to 2^-20 of themselves,
+ * as in the packed prefill, and no terms below 2^-28 of a row's largest V scale; the
+ * rest is as in the steps above.  Queries before start[0] and from start[n_groups] on
+ * share nothing.  start (n_groups + 1 entries, none less than the one before, the
+ * last at most n_q) and prefix are HOST arrays, read during the call: a captured call
+ * keeps its groups, while d_seq, d_pos and the pages may change.  A query whose
+ * d_pos[i] is below its prefix is left out: nothing is appended, and its output row
+ * stays.  A sequence appears at most once per call, and its new token's page is its
+ * own. Head dims 64/128 with groups of 1..8 heads, TQ_HIP_ETYPE otherwise; fp32
+ * arrays 16-byte aligned.  d_ws: tq_hip_decode_step_shared_ws_bytes for the same n_q,
+ * max_pos and groups (0: a call that is refused), 16-byte aligned, nothing is kept in
+ * it between calls. */
 size_t tq_hip_decode_step_shared_ws_bytes(const tq_hip_kv *kv, int n_q, int max_pos, int n_groups, const int32_t *start,
                                           const int32_t *prefix);
 int tq_hip_decode_step_shared_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq, const int32_t *d_pos, int max_pos,
