@@ -383,10 +383,16 @@ int tq_hip_kv_bounds_async(tq_hip_kv *kv, int n, const int32_t *d_seq, const int
  * the first `sinks` blocks, the last `recent` (at least 1: the block of the query's own
  * token is always among them, and its bounds need not be there yet), and of the others
  * those with the largest score
- *   sum over the group's heads g and channels c of max(q_gc M_c, q_gc m_c),
- * M and m the block's bounds: no key of the block scores more.  Scores are in 64 bits,
- * NaN lowest; equal ones go to the lower block.  Entries past min(keep, d_pos[i] / block
- * + 1) are -1, all of them for a negative d_pos[i] or a sequence outside the cache.  d_q
+ *   sum over channels c of (sum over g of max(q_gc, 0)) M_c + (sum over g of min(q_gc, 0)) m_c,
+ * g the group's heads, M and m the block's bounds, in 64 bits.  While the bounds are
+ * finite that is the sum over g and c of max(q_gc M_c, q_gc m_c), and no cached key's
+ * products with these q add up to more (a step's q are rounded to Q8, which the scores
+ * leave out).  With an infinite bound the score is what these products and sums make of
+ * it: NaN where infinity meets a sum of zero or infinity of the other sign, and NaN ranks
+ * lowest.  So a block of which a channel holds no number, or that has no pages, comes
+ * behind all blocks with finite bounds; one with an overflowed key may come first or
+ * last.  Equal scores go to the lower block.  Entries past min(keep, d_pos[i] / block + 1)
+ * are -1, all of them for a negative d_pos[i] or a sequence outside the cache.  d_q
  * [n_q][n_q_heads * head_dim], before RoPE with d_cos / d_sin, rotated with NULL.
  * sinks + recent at most keep; n_q at most 65535; fp32 arrays and d_bounds 16-byte
  * aligned; head dims 32/64/128 with groups 1..8, TQ_HIP_ETYPE otherwise.  d_ws:

@@ -4,13 +4,17 @@
 // counterpart in the reference, which attends to everything.
 //
 //   M_c, m_c = max, min over a block's tokens of d_t code_tc, as bf16 rounded outward
-//   s(block) = sum over the group's heads g and channels c of max(q_gc M_c, q_gc m_c)
-//            = sum over c of (sum_g max(q_gc, 0)) M_c + (sum_g min(q_gc, 0)) m_c
+//   s(block) = sum over c of (sum_g max(q_gc, 0)) M_c + (sum_g min(q_gc, 0)) m_c
 //
-// The second form needs two products per channel whatever the group: with both sums
-// over the heads made once, a block costs its 4 hd bytes and 2 hd products.  These are
-// in 64 bits, so that which of two blocks scores higher does not depend on how a sum
-// was ordered (fp64 runs at fp32's rate here, and the bytes bound it).
+// over channels c, with the group's heads g.  For finite bounds it is the sum over g and c
+// of max(q_gc M_c, q_gc m_c), and needs two products per channel whatever the group: with
+// both sums over the heads made once, a block costs its 4 hd bytes and 2 hd products.
+// For infinite ones the two differ, 0 times infinity, and this is the one to rank by: a
+// channel without a number (M = -inf, m = inf: scales that are NaN, pages that are not
+// there) makes its block the last choice, where the maximum, +inf, would put it in
+// front of every block that has keys.  The products are in 64 bits, so that which of two
+// blocks scores higher does not depend on how a sum was ordered (fp64 runs at fp32's rate
+// here, and the bytes bound it).
 //
 // bounds_kernel, a wave per block: a page's key rows are one run; lane w has code dword
 //   w % (hd / 4) of every (256 / hd)-th row and that dword's scale, the rows' lanes are
