@@ -313,9 +313,9 @@ int tq_hip_decode_step_weights_async(tq_hip_kv *kv, int n_q, const int32_t *d_se
  * page table of the first of its queries that is not left out: the call does so where
  * that is faster (12 queries with 8,192 common tokens or 32 with 2,048 are enough),
  * by a choice that n_q, max_pos, start and prefix make, and else each query goes by
- * its own table.  Of what is read together products are kept to 2^-20 of themselves,
- * as in the packed prefill, and no terms below 2^-28 of a row's largest V scale; the
- * rest is as in the steps above.  Queries before start[0] and from start[n_groups] on
+ * its own table.  Of what is read together each product of a weight and a value is kept
+ * to 2^-20 of itself and 2^-28 of the row's largest V scale, as in the packed prefill;
+ * the rest is as in the steps above.  Queries before start[0] and from start[n_groups] on
  * share nothing.  start (n_groups + 1 entries, none less than the one before, the
  * last at most n_q) and prefix are HOST arrays, read during the call: a captured call
  * keeps its groups, while d_seq, d_pos and the pages may change.  A query whose
@@ -439,8 +439,8 @@ int tq_hip_prefill_async(tq_hip_kv *kv, int seq, int pos0, int n, const float *d
  * before any launch, for a sequence that appears twice or that has no page for one
  * of its tokens; a page that takes a token of one sequence is no other's.  Head
  * dims 64/128 with groups 1..8 take the dense kernel (arrays 16-byte aligned), which
- * keeps P and V to 2^-22 where tq_hip_prefill_async keeps 2^-16 (and no term below
- * 2^-29 of the largest V scale so far).  Sequences with few new tokens, those of
+ * keeps P and V to 2^-22 where tq_hip_prefill_async keeps 2^-16 (each of their products
+ * to 2^-20 of itself and 2^-28 of the largest V scale so far).  Sequences with few new tokens, those of
  * more than 65,536 tokens, and every sequence of other shapes, attend row by row as
  * decode steps do, with products as exact: prompts, short turns and single tokens
  * can share a call.  (A whole prompt row by row takes many times as long, and there,

@@ -19,6 +19,8 @@ constexpr int kRows = 128;               // rows of a work-group, 32 per wave
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kHead = 4.0f;            // log2 headroom before the running max moves
 constexpr float kShift = 11.0f;          // log2 of what P is multiplied by
+constexpr int kVShift = 8;               // and V', whose codes reach 2^7, over its largest scale
+constexpr float kWildBelow = 0x1p-1f;    // units: a key with no larger scale has a unit of its own
 constexpr int kCounterInts = 64;         // one 256-byte line per counter
 constexpr int kCoherent = 16;            // cache policy sc1: agent-coherent access
 constexpr int kBufs = 3;                 // tile buffers
@@ -63,6 +65,12 @@ __device__ __forceinline__ void split_f16(const float (&x)[N], W &hi, W &lo) {
         hi[i] = h;
         lo[i] = __builtin_bit_cast(uint32_t, w);
     }
+}
+
+// log2 of the unit of values whose largest scale is d: 2^-kVShift of the power of two just
+// above d (bits of non-negative floats order as integers).
+__device__ __forceinline__ int unit_exponent(float d) {
+    return min(max((int)(__float_as_uint(d) >> 23) - 126 - kVShift, -126), 126);
 }
 
 // Over lanes l and l ^ 32, the same value in both.

@@ -55,9 +55,12 @@
 //
 // Precision: two fp16 parts keep 22 bits where bf16's keep 16, but not its range.
 // P is taken 2^kShift times as large, so that the parts of all but negligible
-// weights are normal numbers.  A tile's V' are in units of the power of two just
-// above its largest scale; o is kept per row in the largest unit of the keys that
-// the row has seen.  A wild tile, one with a key whose scales are all below 2^-9
+// weights are normal numbers.  A tile's V' are in units of 2^-8 of the power of two just
+// above its largest scale, up to 2^15 of them: lower parts end at 2^-25 units, 2^-32 of
+// that scale, so that a block of small values beside a large one keeps its bits (with
+// units 2^8 as large, at no less time, values 2^-12 times as large as others of their
+// key were kept to 2^-12 of themselves); o is kept per row in the largest unit of the
+// keys that the row has seen.  A wild tile, one with a key whose scales are all below 2^-9
 // of its largest or with one that is no number, has a unit per key instead,
 // which goes to P.  What a scale that is no number makes of a block is added to that
 // block's columns apart from the products, in the rows that see its key.  So what the
@@ -117,12 +120,11 @@ __global__ __launch_bounds__(kThreads) void pack_stage_kernel(PackArgs a) {
     const unsigned char *rv = reinterpret_cast<const unsigned char *>(raw[1]);
     unsigned char *out = s.img + ((size_t)kvh * a.n_tiles + x) * I::BYTES;
 
-    // the units of V' (bits of non-negative floats order as integers)
+    // the units of V'
     __shared__ float per_key[kKT];
     __shared__ float shared_per_unit;
     __shared__ int shared_wild;
     if (tid < 64) {
-        auto exponent = [](float d) { return min(max((int)(__float_as_uint(d) >> 23) - 126, -126), 126); };
         float d = 0.0f;   // the largest that is a number
         uint32_t odd = 0;
         for (int b = 0; b < NB; b++) {
@@ -134,11 +136,11 @@ __global__ __launch_bounds__(kThreads) void pack_stage_kernel(PackArgs a) {
             odd |= up | down;
             if (tid == 0) *reinterpret_cast<uint2 *>(out + I::VO + 8 * b) = make_uint2(up, down);
         }
-        const int e = exponent(wave_max(d));
+        const int e = unit_exponent(wave_max(d));
         const float unit = ldexpf(1.0f, e);
-        const bool any = odd != 0 || __builtin_amdgcn_ballot_w64(d > 0.0f && d < unit * 0x1p-9f) != 0;
+        const bool any = odd != 0 || __builtin_amdgcn_ballot_w64(d > 0.0f && d < unit * kWildBelow) != 0;
         if (tid < kKT) {
-            const int ek = exponent(d), h = (tid >> 2) & 1, at = (tid >> 3) * 4 + (tid & 3);   // key_of's inverse
+            const int ek = unit_exponent(d), h = (tid >> 2) & 1, at = (tid >> 3) * 4 + (tid & 3);   // key_of's inverse
             *reinterpret_cast<float *>(out + I::VK + (h * 16 + at) * 4) = ldexpf(1.0f, ek);
             per_key[tid] = ldexpf(1.0f, -ek);
         }
@@ -282,7 +284,7 @@ __global__ __launch_bounds__(kThreads, 2) void pack_block_kernel(PackArgs a) {
 
     float M = st.mrow, L = pair_sum(st.lsum);
     // columns 32c + 8g + 4h .. + 3 of the row are o[c][4g ..].  o / l is a mean of V',
-    // at most 127, and only that is taken out of its unit: o, a sum of P of 2^11 and
+    // at most 2^15, and only that is taken out of its unit: o, a sum of P of 2^11 and
     // more, would overflow where the mean does not, and unit / l underflow.
     auto store = [&](const v16f (&o)[C], float l, float unit) {
         if (!real) return;

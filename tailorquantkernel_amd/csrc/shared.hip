@@ -61,8 +61,6 @@ __device__ __forceinline__ int thread_now() {
     return tid;
 }
 
-__device__ __forceinline__ int scale_exponent(float d) { return min(max((int)(__float_as_uint(d) >> 23) - 126, -126), 126); }
-
 // Offsets of an image's two halves: K's codes and scales, V' with its units.  They are
 // made and read a step apart, so each has two buffers of its own.
 template <int HD>
@@ -92,7 +90,7 @@ __device__ __forceinline__ void make_wild(const unsigned char *raw, int keys, un
         odd |= up | down;
         if (tid == 0) *reinterpret_cast<uint2 *>(out + I::VO + 8 * b) = make_uint2(up, down);
     }
-    const int e = scale_exponent(d), top = scale_exponent(wave_max(d));
+    const int e = unit_exponent(d), top = unit_exponent(wave_max(d));
     if (tid < kKT) {
         const int h = (tid >> 2) & 1, at = (tid >> 3) * 4 + (tid & 3);   // key_of's inverse
         *reinterpret_cast<float *>(out + I::VK + (h * 16 + at) * 4) = ldexpf(1.0f, e);
@@ -196,9 +194,9 @@ __device__ __forceinline__ void make_v(const RawV<HD> &r, int tid, const unsigne
 #pragma unroll
         for (int x = 0; x < 4; x++) s[x] = RawV<HD>::first(lane) + x < keys ? s[x] : 0.0f;
     }
-    const int e = scale_exponent(wave_max(d));
+    const int e = unit_exponent(wave_max(d));
     const float unit = __uint_as_float((uint32_t)(e + 127) << 23), per_unit = __uint_as_float((uint32_t)(127 - e) << 23);
-    if (__builtin_amdgcn_ballot_w64(!number || (d > 0.0f && d < unit * 0x1p-9f)) != 0) {
+    if (__builtin_amdgcn_ballot_w64(!number || (d > 0.0f && d < unit * kWildBelow)) != 0) {
         make_wild<HD>(raw, keys, out);
         return;
     }
