@@ -1171,29 +1171,37 @@ namespace {
 // Most runs of a group's common tokens, and splits of what lies behind them: the merge
 // holds 128 slots.
 constexpr int kSharedRuns = 64;
-// Fewest queries of a group that attend to its tokens together (or SharedPlan::far).
-constexpr int kFewestMembers = 4;
+
+// What a common token of a kv head saves a group whose queries attend to it together: one
+// unit for each query that does not by itself (1.5 with more than 4 heads a kv head), less
+// six for a block of 128 rows, whatever it holds.  Groups that lose by it, beside 64 queries
+// behind 2,048 (us, 32 / 8 heads, together / by themselves): 6 of 4 behind 4,096 94 / 66, 8
+// of 5 behind 2,048 (and the 64 behind 4,096) 83 / 70; that neither lose nor gain: 3 of 6
+// behind 4,096 50 / 64, 8 of 6 behind 2,048 (32 behind 8,192) 84 / 70, 64 / 8 heads 12 of 4
+// behind 8,192 172 / 190.
+double saved_per_token(int members, int g) { return members * (g > 4 ? 1.5 : 1.0) - 6.0 * tq_shared_steps(members, g, 1); }
 
 // How a step with common tokens is cut: what each group shares, in runs of `chunk` key
 // tiles, and the splits behind.
 struct SharedPlan {
     bool together = false;
+    int g = 1;               // query heads of a kv head
+    bool loses(int members) const { return saved_per_token(members, g) < 0.0; }
     // What a group attends to together: all of its common tokens, or none.
     int common(int members, int prefix) const {
-        return together && (members >= kFewestMembers || (members >= 2 && prefix > far)) ? prefix : 0;
+        return together && (!loses(members) || (members >= 2 && prefix > far)) ? prefix : 0;
     }
-    double far = 0.0;        // a prefix that is long for two queries, too
+    double far = 0.0;        // a prefix that is long for a group that loses, too
     long chunk = 1;
     int runs = 0;            // most runs of a group
     int split_tokens, n_splits, slots;
     size_t partials, bytes;  // of the workspace: least_of, runs_of, partials
 };
 
-// Whether a call's groups attend to their common tokens together, or each query to its
-// own as in any step.  A token of a kv head costs a query one unit by itself (1.5 with
-// more than 4 heads a kv head), and a block of 128 rows six, whatever it holds; the
-// images, the rows' means and their merge want some 300,000 units saved.  Measured (us,
-// together / each by itself; own tokens 64-256 behind):
+// Whether groups of a call attend to their common tokens together, or each query to its
+// own as in any step: the images, the rows' means and their merge want some 300,000 units
+// saved, by the groups that save any, and the others go by themselves whatever those do
+// (but SharedPlan::far).  Measured (us, together / each by itself; own tokens 64-256 behind):
 //   queries  common   32 / 8 heads   64 / 8         16 / 16        24 / 8 of 64
 //   4         4,096   22.4 / 16.8    24.5 / 21.4    28.8 / 20.0    17.2 / 14.4   apart
 //   8         4,096   23.1 / 20.7    26.8 / 26.1    29.2 / 27.3    17.7 / 16.8   apart
@@ -1211,8 +1219,7 @@ bool worth_sharing(const tq_hip_kv *kv, int n_groups, const int32_t *start, cons
     double saved = 0.0;
     for (int i = 0; i < n_groups; i++) {
         const int members = start[i + 1] - start[i];
-        if (members >= kFewestMembers)
-            saved += (members * (g > 4 ? 1.5 : 1.0) - 6.0 * tq_shared_steps(members, g, 1)) * prefix[i];
+        saved += std::max(saved_per_token(members, g), 0.0) * prefix[i];
     }
     return saved * kv->desc.n_kv_heads >= 300e3;
 }
@@ -1231,7 +1238,7 @@ bool shared_ok(const tq_hip_kv *kv, int n_q, int max_pos, int n_groups, const in
 void plan_shared(const tq_hip_kv *kv, int n_q, int max_pos, int n_groups, const int32_t *start, const int32_t *prefix,
                  SharedPlan &p) {
     const tq_hip_kv_desc &D = kv->desc;
-    const int g = D.n_q_heads / D.n_kv_heads;
+    const int g = p.g = D.n_q_heads / D.n_kv_heads;
     p.together = worth_sharing(kv, n_groups, start, prefix);
     const long whole = (long)max_pos + 1;
     long grouped = 0, apart = 0;   // queries; tokens that queries attend to by themselves
@@ -1240,15 +1247,16 @@ void plan_shared(const tq_hip_kv *kv, int n_q, int max_pos, int n_groups, const 
         const int members = start[i + 1] - start[i];
         grouped += members;
         if (members > 0) deepest = std::max(deepest, (int)prefix[i]);
-        if (!p.together || members < kFewestMembers) apart += (long)members * prefix[i];
+        if (!p.together || p.loses(members)) apart += (long)members * prefix[i];
     }
     apart += grouped * (whole - deepest) + (n_q - grouped) * whole;
     // what each of the 512 work-groups that run at once has of them
     double even = (double)apart * D.n_kv_heads / 512;
-    // Two or three queries would keep a few work-groups busy for long behind far more
-    // common tokens than that (groups of 12, 3 and 33 behind 16,384, 7,680 and 864, 64 / 8
-    // heads: by themselves 92 us, together 80), but not where many are like them
-    // (20 groups, five of 3 queries behind up to 4,096: 78 and 87)
+    // A few queries would keep a few work-groups busy for long behind far more common
+    // tokens than that (4 behind 49,152 beside 64 behind 2,048, 32 / 8 heads: by themselves
+    // 135 us, together 108; 3 groups of 4 behind 16,384 121 and 106; groups of 12, 3 and
+    // 33 behind 16,384, 7,680 and 864, 64 / 8 heads: 92 and 80), but not where many are
+    // like them (20 groups, five of 3 queries behind up to 4,096: 78 and 87)
     p.far = 4.0 * even;
     long steps = 0, longest = 0;   // key tiles of rows; most common tokens that a query attends to by itself
     int least = INT32_MAX, most = 0;
@@ -1260,7 +1268,7 @@ void plan_shared(const tq_hip_kv *kv, int n_q, int max_pos, int n_groups, const 
         most = std::max(most, common);
         longest = std::max(longest, (long)prefix[i] - common);
         steps += tq_shared_steps(members, g, common);
-        if (members < kFewestMembers) even -= (double)members * common * D.n_kv_heads / 512;
+        if (p.loses(members)) even -= (double)members * common * D.n_kv_heads / 512;
     }
     if (grouped < n_q) least = 0;
     // one work-group per CU, the queries' own beside it, where the tiles are few: each
