@@ -409,7 +409,8 @@ int tq_hip_kv_select_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq, const i
  * below d_pos[i], and the new token, whose block d_pos[i] / block is the last of them.
  * The entries are those of tq_hip_kv_select_async or the caller's own: each once, on
  * mapped pages.  The new key also enters the bounds of its block (d_bounds NULL: none
- * are kept), which begin with the block's first token.  A sequence appears at most once
+ * are kept), which begin with the block's first token; one whose slot has no page is not
+ * cached and counts for nothing.  A sequence appears at most once
  * per call.  Head dims 32/64/128 with groups 1..8, TQ_HIP_ETYPE otherwise; fp32 arrays
  * and d_bounds 16-byte aligned; keep * block at most 2^19.  d_ws:
  * tq_hip_decode_step_blocks_ws_bytes for the same n_q, max_pos, block and keep (0: a call
@@ -440,11 +441,11 @@ int tq_hip_prefill_async(tq_hip_kv *kv, int seq, int pos0, int n, const float *d
  * of its tokens; a page that takes a token of one sequence is no other's.  Head
  * dims 64/128 with groups 1..8 take the dense kernel (arrays 16-byte aligned), which
  * keeps P and V to 2^-22 where tq_hip_prefill_async keeps 2^-16 (each of their products
- * to 2^-20 of itself and 2^-28 of the largest V scale so far).  Sequences with few new tokens, those of
- * more than 65,536 tokens, and every sequence of other shapes, attend row by row as
- * decode steps do, with products as exact: prompts, short turns and single tokens
- * can share a call.  (A whole prompt row by row takes many times as long, and there,
- * as in a decode step, values past 2^120 divided by the tokens may overflow.)  The
+ * to 2^-20 of itself and 2^-28 of the largest V scale so far).  Sequences with few new
+ * tokens, those of more than 65,536 tokens, and every sequence of other shapes, attend row
+ * by row as decode steps do, with products as exact: prompts, short turns and single
+ * tokens can share a call.  (A whole prompt row by row takes many times as long, and
+ * there, as in a decode step, values past 2^120 divided by the tokens may overflow.)  The
  * form of a sequence and the cuts of its blocks go by the cost of the whole call: its
  * precision does not depend on the others, its last bits may.  d_ws:
  * tq_hip_prefill_packed_ws_bytes for the same pos0 and start (0: a call that is

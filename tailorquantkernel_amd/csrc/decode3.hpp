@@ -616,7 +616,9 @@ __device__ __forceinline__ void decode3_run(const TqDecodeArgs &a, const int spl
             const int block = at_new / a.block_tokens;
             if (a.bounds && tid < HD && (unsigned)seq < (unsigned)view.max_seqs && (size_t)block < a.bounds_stride) {
                 const unsigned char *blk = sm.newrow + (tid / kQK) * kBlockBytes;
-                const float key = (float)(int8_t)blk[4 + tid % kQK] * *reinterpret_cast<const float *>(blk);
+                // (a key that no page took counts for nothing: NaN, past max and min)
+                const float key = phys < 0 ? __builtin_nanf("")
+                                           : (float)(int8_t)blk[4 + tid % kQK] * *reinterpret_cast<const float *>(blk);
                 uint16_t *b = a.bounds + (((size_t)seq * a.n_kv_heads + kvh) * a.bounds_stride + block) * 2 * HD + tid;
                 const bool first = at_new == block * a.block_tokens;
                 float most = first ? -INFINITY : bf16_value(b[0]), least = first ? INFINITY : bf16_value(b[HD]);
