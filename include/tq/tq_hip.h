@@ -319,8 +319,8 @@ int tq_hip_decode_step_weights_async(tq_hip_kv *kv, int n_q, const int32_t *d_se
  * share nothing.  start (n_groups + 1 entries, none less than the one before, the
  * last at most n_q) and prefix are HOST arrays, read during the call: a captured call
  * keeps its groups, while d_seq, d_pos and the pages may change.  A query whose
- * d_pos[i] is below its prefix is left out: nothing is appended, and its output row
- * stays.  A sequence appears at most once per call, and its new token's page is its
+ * d_pos[i] is below its prefix, or whose sequence is outside the cache, is left out:
+ * nothing is appended, and its output row stays.  A sequence appears at most once per call, and its new token's page is its
  * own. Head dims 64/128 with groups of 1..8 heads, TQ_HIP_ETYPE otherwise; fp32
  * arrays 16-byte aligned.  d_ws: tq_hip_decode_step_shared_ws_bytes for the same n_q,
  * max_pos and groups (0: a call that is refused), 16-byte aligned, nothing is kept in
@@ -410,7 +410,8 @@ int tq_hip_kv_select_async(tq_hip_kv *kv, int n_q, const int32_t *d_seq, const i
  * The entries are those of tq_hip_kv_select_async or the caller's own: each once, on
  * mapped pages.  The new key also enters the bounds of its block (d_bounds NULL: none
  * are kept), which begin with the block's first token; one whose slot has no page is not
- * cached and counts for nothing.  A sequence appears at most once
+ * cached and counts for nothing.  A query with a negative d_pos[i] or a sequence outside
+ * the cache is left out: its output row stays.  A sequence appears at most once
  * per call.  Head dims 32/64/128 with groups 1..8, TQ_HIP_ETYPE otherwise; fp32 arrays
  * and d_bounds 16-byte aligned; keep * block at most 2^19.  d_ws:
  * tq_hip_decode_step_blocks_ws_bytes for the same n_q, max_pos, block and keep (0: a call

@@ -271,7 +271,8 @@ __device__ __forceinline__ void split3_bf16(const float (&x)[8], v8bf &hi, v8bf 
 // `base`, a whole page, a query whose new token lies below `least` is left out, and query
 // z is z (shared.hip's work-groups run it).
 // Of these two every split leaves its rows' means with m and l (a step over blocks in
-// one split its output), and decode_merge_kernel joins them.
+// one split its output), and decode_merge_kernel joins them; both leave queries of
+// sequences outside the cache out.
 // RMSNorm and completion flags are kPlain's only; kRows appends nothing and takes its
 // pages from the table, as kBlocks and kShared do; these and kScores always append.
 constexpr int kPlain = 0, kRows = 1, kScores = 2, kBlocks = 3, kShared = 4;
@@ -450,6 +451,7 @@ __device__ __forceinline__ void decode3_run(const TqDecodeArgs &a, const int spl
         len = min(block, a.keep - 1) * a.block_tokens + at_new - block * a.block_tokens + 1;
     }
     const int seq = a.seq_of ? seq_raw : a.seq_const + a.seq_stride * qi;
+    if (MODE >= kBlocks && (unsigned)seq >= (unsigned)view.max_seqs) len = 0;
     int t_end;
     if (contig) {
         if (len <= 0 || t_begin >= len) return;
@@ -614,7 +616,7 @@ __device__ __forceinline__ void decode3_run(const TqDecodeArgs &a, const int spl
         }
         if constexpr (MODE == kBlocks) {
             const int block = at_new / a.block_tokens;
-            if (a.bounds && tid < HD && (unsigned)seq < (unsigned)view.max_seqs && (size_t)block < a.bounds_stride) {
+            if (a.bounds && tid < HD && (size_t)block < a.bounds_stride) {
                 const unsigned char *blk = sm.newrow + (tid / kQK) * kBlockBytes;
                 // (a key that no page took counts for nothing: NaN, past max and min)
                 const float key = phys < 0 ? __builtin_nanf("")

@@ -28,7 +28,8 @@ __global__ __launch_bounds__(kThreads) void decode_merge_kernel(TqMergeArgs a) {
     const int kvh = blockIdx.x, qi = blockIdx.y, hd = a.head_dim;
     const int least = a.runs_of ? a.least_of[qi] : 0, runs = a.runs_of ? a.runs_of[qi] : 0;
     int len = a.pos_of[qi] + 1;
-    if (len <= least) return;
+    const int seq = a.seq_of ? a.seq_of[qi] : qi;
+    if (len <= least || (unsigned)seq >= (unsigned)a.max_seqs) return;
     if (runs) len -= least;
     if (a.keep) {
         const int block = (len - 1) / a.block_tokens;

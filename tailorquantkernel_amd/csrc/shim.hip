@@ -1151,6 +1151,8 @@ static TqDecodeArgs step_args(const tq_hip_kv *kv, int n_q, const int32_t *d_seq
 static TqMergeArgs merge_args(const TqDecodeArgs &a) {
     TqMergeArgs m{};
     m.pos_of = a.len_of;
+    m.seq_of = a.seq_of;
+    m.max_seqs = a.view.max_seqs;
     m.keep = a.list ? a.keep : 0;
     m.block_tokens = a.block_tokens;
     m.n_q = a.n_q;

@@ -363,9 +363,11 @@ hipError_t tq_launch_decode3_blocks(const TqDecodeArgs &a, int waves, hipStream_
 // out from partials [query][kv head][slots][floats as tq_decode3_partial_floats]: of a
 // query at d_pos the slots of its splits (of its tokens, of listed blocks or, with runs,
 // from least_of on) and the runs_of slots from n_splits on.  A query in front of its
-// least position is left.
+// least position is left, and one of a sequence outside the cache.
 struct TqMergeArgs {
     const int32_t *pos_of;
+    const int32_t *seq_of;    // or null: sequence i
+    int max_seqs;
     const int32_t *least_of;  // or null: 0
     const int32_t *runs_of;  // or null: 0
     int keep, block_tokens;  // listed blocks, or 0
