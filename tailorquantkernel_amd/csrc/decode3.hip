@@ -38,5 +38,5 @@ hipError_t tq_launch_decode3(const TqDecodeArgs &a, int waves, hipStream_t s) {
         }
     };
     if (a.scores) return launch(std::integral_constant<int, kScores>{});
-    return a.exact ? launch(std::integral_constant<int, kRows>{}) : launch(std::integral_constant<int, kPlain>{});
+    return a.exact ? launch(std::integral_constant<int, kPromptRows>{}) : launch(std::integral_constant<int, kPlain>{});
 }

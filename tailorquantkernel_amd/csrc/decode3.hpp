@@ -59,7 +59,7 @@
 
 #include <type_traits>
 
-#include "tq_common.hpp"
+#include "lds_copy.hpp"
 
 namespace {
 namespace d3 {   // (shared.hip has names of its own for the like)
@@ -69,7 +69,6 @@ using namespace tq;
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 
 constexpr int kTK = 32;                  // keys per tile
 constexpr int kMaxSplits3 = 64;
@@ -153,10 +152,6 @@ __device__ __forceinline__ float xrow_sum(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
-    v2bf v = {(__bf16)a, (__bf16)b};
-    return __builtin_bit_cast(uint32_t, v);
-}
 // x = hi + lo with hi = bf16(x), lo = bf16(x - hi), four pairs.
 __device__ __forceinline__ void split_bf16(const float (&x)[8], v8bf &hi, v8bf &lo) {
     u32x4 h, l;
@@ -169,58 +164,6 @@ __device__ __forceinline__ void split_bf16(const float (&x)[8], v8bf &hi, v8bf &
     hi = __builtin_bit_cast(v8bf, h);
     lo = __builtin_bit_cast(v8bf, l);
 }
-
-typedef __attribute__((address_space(3))) unsigned char lds_u8;
-
-// 16 bytes from each lane's global address into LDS at dst + 16*lane
-// (global_load_lds_dwordx4; M0 holds the LDS byte address and is restored; a
-// scalar write of M0 needs one wait state before the copy, the s_nop).
-// Issued as inline assembly so that the compiler does not follow every such
-// copy with a full vmcnt(0) wait before LDS accesses: the kernel waits for
-// exactly the copies it needs (wait_copies), counting them in issue order.
-// No memory clobber: LDS reads of a slot are ordered before a refill by
-// wait_lds() (a compiler barrier plus lgkmcnt(0)) and after its copies by
-// wait_copies(); leaving memory unclobbered keeps the uniform loads that
-// precede the copies scalar.
-__device__ __forceinline__ void dma16(const void *src, unsigned char *dst) {
-    const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8 *)dst;
-    uint32_t saved;
-    asm volatile(
-        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\t"
-        "global_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-        : "=&s"(saved)
-        : "v"(src), "s"(lds));
-}
-// The same copy from a scalar base address plus each lane's 32-bit offset
-// (the saddr form): a uniform base costs no vector address arithmetic.
-__device__ __forceinline__ void dma16s(const unsigned char *base, uint32_t off, unsigned char *dst) {
-    const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8 *)dst;
-    uint32_t saved;
-    asm volatile(
-        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\t"
-        "global_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-        : "=&s"(saved)
-        : "v"(off), "s"(base), "s"(lds));
-}
-// 4 bytes per lane, the same way (into LDS at dst + 4*lane).
-__device__ __forceinline__ void dma4s(const unsigned char *base, uint32_t off, unsigned char *dst) {
-    const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8 *)dst;
-    uint32_t saved;
-    asm volatile(
-        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\t"
-        "global_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
-        : "=&s"(saved)
-        : "v"(off), "s"(base), "s"(lds));
-}
-// Wait until at most N vector memory operations of this wave are outstanding.
-template <int N>
-__device__ __forceinline__ void wait_copies() {
-    static_assert(N >= 0 && N < 64, "vmcnt immediate");
-    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
-}
-// Every LDS access issued so far has completed (before a copy may land on
-// memory those accesses touch).
-__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
 
 // RMSNorm's last step, out = (x * inverse) * weight, rounded as
 // model/rmsnorm.c:17 rounds it.
@@ -255,7 +198,7 @@ __device__ __forceinline__ void split3_bf16(const float (&x)[8], v8bf &hi, v8bf 
 // MODE, but for kPlain: W is split in three bf16 parts instead of two, so that out is
 // exact to 2^-25 instead of 2^-18 per term (the third product and its split take no
 // time beside the stream).
-// kRows, rows of several sequences' prompts: query i may stand in row row_of[i].
+// kPromptRows, rows of several sequences' prompts: query i may stand in row row_of[i].
 // kScores, the step that gathers weights: every score goes to a.scores, and with
 // more than one split the combine is left to decode_weights_kernel, which follows;
 // a single split knows its rows' sums and adds the weights itself (256 keys of 8 /
@@ -273,9 +216,9 @@ __device__ __forceinline__ void split3_bf16(const float (&x)[8], v8bf &hi, v8bf 
 // Of these two every split leaves its rows' means with m and l (a step over blocks in
 // one split its output), and decode_merge_kernel joins them; both leave queries of
 // sequences outside the cache out.
-// RMSNorm and completion flags are kPlain's only; kRows appends nothing and takes its
+// RMSNorm and completion flags are kPlain's only; kPromptRows appends nothing and takes its
 // pages from the table, as kBlocks and kShared do; these and kScores always append.
-constexpr int kPlain = 0, kRows = 1, kScores = 2, kBlocks = 3, kShared = 4;
+constexpr int kPlain = 0, kPromptRows = 1, kScores = 2, kBlocks = 3, kShared = 4;
 // split, kvh, z: the grid's place; least, base: kShared's; sm and the slots: the work-group's shared memory (two
 // tile slots per wave, separate objects so that the wait for one slot's copies does not
 // wait for the other's).
@@ -371,7 +314,7 @@ __device__ __forceinline__ void decode3_run(const TqDecodeArgs &a, const int spl
         // norm weights the K and V slots are too (without a step they repeat q)
         constexpr int QC = G * HD / 4, RC = HD / 8, NC = HD / 4;
         const int nch = QC + 2 * RC + (nrm ? 4 * NC : (step ? 2 * NC : 0));
-        const int at = MODE == kRows && a.row_of ? a.row_of[qi] : qi;
+        const int at = MODE == kPromptRows && a.row_of ? a.row_of[qi] : qi;
         const float *qg = a.q + ((size_t)at * a.n_q_heads + (size_t)kvh * G) * HD;
         const size_t nrow = ((size_t)qi * a.n_kv_heads + kvh) * HD;
         for (int c0 = 0; c0 < nch; c0 += 64) {
@@ -490,9 +433,9 @@ __device__ __forceinline__ void decode3_run(const TqDecodeArgs &a, const int spl
     }
     // the staged inputs have landed; the first tile may still be in flight
     if (first_issued)
-        wait_copies<CPL>();
+        wait_vm<CPL>();
     else
-        wait_copies<0>();
+        wait_vm<0>();
     if (nrm) {
         // 1/rms of each q head (lanes 0..G-1) and of the new K row (lane G):
         // the squares summed serially in element order, as model/rmsnorm.c:4-12
@@ -826,9 +769,9 @@ __device__ __forceinline__ void decode3_run(const TqDecodeArgs &a, const int spl
     // is one of ours, already issued after tile j's) may stay in flight.
     auto wait_tile = [&](int j) {
         if (j + 1 < my_tiles)
-            wait_copies<CPL>();
+            wait_vm<CPL>();
         else
-            wait_copies<0>();
+            wait_vm<0>();
     };
     for (int it = 0; it < my_tiles; it += 2) {
         {
@@ -881,7 +824,7 @@ __device__ __forceinline__ void decode3_run(const TqDecodeArgs &a, const int spl
     }
     __syncthreads();
 
-    const size_t out_row = (size_t)(MODE == kRows && a.row_of ? a.row_of[qi] : qi) * a.n_q_heads + (size_t)kvh * G;
+    const size_t out_row = (size_t)(MODE == kPromptRows && a.row_of ? a.row_of[qi] : qi) * a.n_q_heads + (size_t)kvh * G;
     const size_t pbase = ((size_t)qi * a.n_kv_heads + kvh) * (MODE == kShared ? a.part_slots : a.n_splits);
     const bool single = MODE != kShared && a.n_splits == 1;
     // Float4 f4 / 4 of this (query, kv head)'s G output rows.  With completion

@@ -1,56 +1,13 @@
-// prefill_stage.hpp — what the prefill kernels share: copies into LDS, and the
-// staging of a key tile's rows (old ones from the cache, new ones quantized and
-// appended).
+// prefill_stage.hpp — what the prefill kernels share: the staging of a key tile's rows
+// (old ones from the cache, new ones quantized and appended).
 #pragma once
 
+#include "lds_copy.hpp"
 #include "prefill_runs.hpp"
-#include "tq_common.hpp"
 
 namespace tq {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
-typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
-
-__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
-    v2bf v = {(__bf16)a, (__bf16)b};
-    return __builtin_bit_cast(uint32_t, v);
-}
-
-typedef __attribute__((address_space(3))) unsigned char lds_u8;
-
-// 16 bytes from each lane's global address into LDS at dst + 16*lane
-// (global_load_lds_dwordx4, M0 = LDS byte address, restored after; a scalar
-// write of M0 needs one wait state before the copy, the s_nop).  Inline
-// assembly keeps the compiler from following the copy with a full vmcnt(0)
-// wait before every LDS access; the kernel waits for its copies itself.
-__device__ __forceinline__ void dma16(const void *src, unsigned char *dst) {
-    const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8 *)dst;
-    uint32_t saved;
-    asm volatile(
-        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\t"
-        "global_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-        : "=&s"(saved)
-        : "v"(src), "s"(lds));
-}
-
-// The same copy from a scalar base address plus each lane's 32-bit offset.
-__device__ __forceinline__ void dma16s(const unsigned char *base, uint32_t off, unsigned char *dst) {
-    const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8 *)dst;
-    uint32_t saved;
-    asm volatile(
-        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\t"
-        "global_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-        : "=&s"(saved)
-        : "v"(off), "s"(base), "s"(lds));
-}
-
-// Wait until at most N vector memory operations of this wave are outstanding
-// (the copies above are counted in issue order).
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-    static_assert(N >= 0 && N < 64, "vmcnt immediate");
-    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
-}
 
 struct StageArgs {
     PagedView view;
