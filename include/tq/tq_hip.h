@@ -311,9 +311,10 @@ int tq_hip_decode_step_weights_async(tq_hip_kv *kv, int n_q, const int32_t *d_se
  * prefix[g] tokens of its sequences, a multiple of TQ_HIP_PAGE_TOKENS and at most
  * max_pos, lie in the same pages, which may be read once for the group, through the
  * page table of the first of its queries that is not left out: the call does so for the
- * groups where that is faster (12 queries with 8,192 common tokens or 32 with 2,048 are
- * enough, whatever other groups there are), by a choice that n_q, max_pos, start and
- * prefix make, and else each query goes by its own table.  Of what is read together each product of a weight and a value is kept
+ * groups where that is faster, by a choice that the numbers of heads, n_q, max_pos, start
+ * and prefix make, and else each query goes by its own table.  With 8 kv heads and more,
+ * 12 queries with 8,192 common tokens or 32 with 2,048 are enough, whatever other groups
+ * there are; with fewer kv heads it takes as many times more common tokens.  Of what is read together each product of a weight and a value is kept
  * to 2^-20 of itself and 2^-28 of the row's largest V scale, as in the packed prefill;
  * the rest is as in the steps above.  Queries before start[0] and from start[n_groups] on
  * share nothing.  start (n_groups + 1 entries, none less than the one before, the

@@ -58,3 +58,14 @@ def test_too_little_to_gain(nat, oracle):
     st = Shared(nat, oracle, 3, 8, 8, 64, [(640, members(64))], large=False, max_pos=7000)
     other_pages(st, 0, False)
     st.check(st.run())
+
+
+@pytest.mark.parametrize("nq,nkv", [(8, 8), (24, 8), (32, 8), (64, 8), (16, 16), (4, 1)])
+@pytest.mark.parametrize("n,prefix", [(12, 8192), (32, 2048)])
+def test_as_many_as_the_header_says(nat, oracle, nq, nkv, n, prefix):
+    """With fewer kv heads as many times more common tokens; a small group beside them changes nothing."""
+    prefix *= max(1, 8 // nkv)
+    st = Shared(nat, oracle, n, nq, nkv, 64, [(64, members(4)), (prefix, [0] * n)], large=False)
+    other_pages(st, 1, True)
+    st.checked = 0                   # the last query alone: the one whose table is another
+    st.check(st.run())
