@@ -1,7 +1,7 @@
 // decode3_blocks.hip — the MFMA decode step (decode3.hpp) over listed blocks.  Bound by
 // reading the blocks as the plain step is by its cache, in shorter runs: 16 queries of
-// 64 / 8 heads of 128 over 64 blocks of 64 tokens (151 MB) in 35 us and the merge's 4.8; one
-// of 32 / 8 over 128 blocks of 16 in 7.2 and 3.5, the latency of one tile a wave.
+// 64 / 8 heads of 128 over 64 blocks of 64 tokens (151 MB) in 36 us and the merge's 4.9; one
+// of 32 / 8 over 128 blocks of 16 in 7.6 and 4.0, the latency of one tile a wave.
 #include "decode3.hpp"
 
 using namespace d3;

@@ -8,8 +8,8 @@
 // One work-group per (query, kv head): a wave per head derives the weights, then every
 // thread has a float4 of the rows for a share of the slots, eight in flight.  Bound by the
 // latency of its dependent reads (the query's length, m and l, the rows) and, with many
-// slots, by reading the partials from the MALL: 1 query of 32 / 8 heads in 16 splits 3.5 us,
-// 16 of 64 / 8 in two 4.8, 64 of 32 / 8 in up to 20 (21 MB) 6.8.
+// slots, by reading the partials from the MALL: 1 query of 32 / 8 heads in 16 splits 4.0 us,
+// 16 of 64 / 8 in two 4.9, 64 of 32 / 8 in up to 20 (21 MB) 7.0.
 #include "tq_common.hpp"
 
 namespace {

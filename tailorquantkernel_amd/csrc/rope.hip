@@ -129,8 +129,10 @@ __device__ __forceinline__ float lanes_sum(float x) {
 // its stores: in place is safe either way.
 //   Bound by reading and writing the heads: 4,096 rows of 64 and 8 heads of 128 (302 MB) in
 // 67 us, 8,192 in 124 (4.9 TB/s, where a copy of as much reaches 5.3), 64 rows of 32 and 8
-// in 6.5, the launch and the angles.  Stores past the caches (nontemporal) took 2,048 rows
-// from 36 to 24 us and 4,096 from 72; loads past them undo that (34).
+// in 6.5, the launch and the angles.  Rotary dims that are no such multiples take 111-115
+// us for 4,096 rows, a lane's four partners one by one.  Stores past the caches
+// (nontemporal) took 2,048 rows from 36 to 24 us and 4,096 from 72; loads past them undo
+// that (34).
 enum { kHalves, kNeighbours, kAny };
 template <int LANES, int U, int FORM>
 __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int interleaved) {

@@ -18,10 +18,11 @@
 //   products and the next scores, 0.15 the barrier; with a wave per SIMD the vector pipe
 //   is busy 44% of the time, the matrix pipe 18%.  In front of the first 8 us pass (the
 //   page table, the queries' quantization, the first tile from memory), and the merge
-//   takes 6.6.  64 queries of 32 / 8 heads of 128 behind 4,096 common tokens 44 us (77 each
-//   by itself), behind 16,384 92.  Work-groups of eight waves and 256 rows, half of
-//   them on either image, were slower but for the longest prefixes (58 and 89 us): their
-//   LDS leaves no room for the queries' own work-groups beside them.
+//   takes 6.6.  64 queries of 32 / 8 heads of 128 behind 4,096 common tokens and 16-512 of
+//   their own 41 us (73 each by itself, 70 in the plain step), behind 16,384 87.
+//   Work-groups of eight waves and 256 rows, half of them on either image, were slower but
+//   for the longest prefixes (58 and 89 us where four waves took 43 and 92): their LDS
+//   leaves no room for the queries' own work-groups beside them.
 #include <algorithm>
 
 #include "decode3.hpp"

@@ -1205,17 +1205,19 @@ struct SharedPlan {
 // saved, by the groups that save any, and the others go by themselves whatever those do
 // (but SharedPlan::far).  Measured (us, together / each by itself; own tokens 64-256 behind):
 //   queries  common   32 / 8 heads   64 / 8         16 / 16        24 / 8 of 64
-//   4         4,096   22.4 / 16.8    24.5 / 21.4    28.8 / 20.0    17.2 / 14.4   apart
-//   8         4,096   23.1 / 20.7    26.8 / 26.1    29.2 / 27.3    17.7 / 16.8   apart
-//   8        16,384   48.3 / 52.3    52.2 / 67.6*   79.4 / 73.0    38.5 / 31.7   apart (* together)
-//   12        2,048   19.7 / 23.1    24.2 / 27.7    21.3 / 30.8    14.6 / 16.4   apart
-//   12        8,192   33.0 / 46.6    37.5 / 59.0    46.1 / 75.3    25.7 / 30.1   together
-//   16        4,096   25.5 / 28.1    30.5 / 37.7    30.0 / 41.2    18.6 / 22.8   together
-//   32        1,024   28.6 / 21.0    33.7 / 26.3    25.2 / 29.0*   15.8 / 18.0   apart (* together)
-//   32        2,048   28.7 / 28.7    33.5 / 37.9    25.5 / 43.0    16.6 / 23.6   together
-//   64          256   23.9 / 20.0    32.1 / 24.2    28.7 / 30.6    17.4 / 16.9   apart
-//   64        1,024   32.5 / 31.8    39.1 / 40.3    35.8 / 52.6    19.2 / 25.4   together
-//   64        4,096   39.7 / 77.3    58.7 / 103     43.4 / 138     29.2 / 58.1   together
+//   4         4,096   20.9 / 16.3    22.7 / 20.9    27.1 / 19.5    17.8 / 14.5   apart
+//   8         4,096   21.4 / 19.9    24.4 / 24.6    27.4 / 26.5    18.1 / 17.0   apart
+//   8        16,384   45.9 / 49.7    50.9 / 65.7*   76.4 / 71.6*   37.3 / 31.0   apart (* together)
+//   12        2,048   18.2 / 22.9    22.2 / 28.0    20.2 / 30.1    13.7 / 16.3   apart
+//   12        8,192   31.0 / 45.1    35.2 / 57.5    44.0 / 74.1    24.9 / 29.1   together
+//   16        4,096   23.3 / 27.4    28.5 / 34.6    28.2 / 40.7    17.1 / 22.2   together
+//   32        1,024   26.6 / 20.5    31.2 / 25.8    24.9 / 29.1*   15.0 / 17.4   apart (* together)
+//   32        2,048   27.6 / 27.4    31.0 / 35.4    25.7 / 42.5    15.5 / 22.6   together
+//   64          256   22.8 / 19.2    29.9 / 24.0    28.0 / 30.9    16.8 / 16.5   apart
+//   64        1,024   31.4 / 29.4    37.3 / 38.4    35.8 / 50.9    17.7 / 24.0   together
+//   64        4,096   36.8 / 69.5    53.8 / 95.7    40.7 / 129     26.3 / 53.2   together
+// (calls on one batch, one behind the other, as all the figures of this plan; the plain
+// step of these tokens takes 18.5 us at 4 x 4,096 with 32 / 8 heads, 16.1 with 64 / 8.)
 bool worth_sharing(const tq_hip_kv *kv, int n_groups, const int32_t *start, const int32_t *prefix) {
     const int g = kv->desc.n_q_heads / kv->desc.n_kv_heads;
     double saved = 0.0;
@@ -1275,8 +1277,8 @@ void plan_shared(const tq_hip_kv *kv, int n_q, int max_pos, int n_groups, const 
     if (grouped < n_q) least = 0;
     // one work-group per CU, the queries' own beside it, where the tiles are few: each
     // writes its rows' means, and two a CU are slowed by one another (64 queries of 32 / 8
-    // heads, 128 and their own up to 512 tokens: behind 1,024 common ones 36.7 us and 45.2
-    // with two, 4,096 43 and 53; behind 16,384 94 and 92)
+    // heads, 128-512 tokens of their own: behind 1,024 common ones 37.9 us and 44.4 with
+    // two, 4,096 41 and 52; behind 16,384 86 and 84)
     const long all = steps * D.n_kv_heads, wgs = all <= 40 * 256 ? 256 : 512;
     p.chunk = std::max(1L, (all + wgs - 1) / wgs);
     const long tiles = (most + 31) / 32;
@@ -1434,9 +1436,10 @@ long blocks_len(int max_pos, int block, int keep) { return std::min((long)max_po
 
 // Waves per work-group, and the splits, of a step over listed blocks.  A batch aims at one
 // work-group of eight waves per CU: its lists are short, and a second split costs the
-// merge's launch too (32 queries of 32 / 8 heads of 128 over 2,048 tokens 31 us in one
-// split, 36 .. 40 in two; 16 of 64 / 8 over 4,096 in two splits of eight waves 39, in four
-// of four 41, in four of eight 46, in one 49).
+// merge's launch too (calls on one batch, one behind the other: 32 queries of 32 / 8 heads
+// of 128 over 2,048 tokens 29 us in one split, 39 in two, 33 in two of four waves; 16 of 64
+// / 8 over 4,096 in two splits of eight waves 35.4, in four of four 35.3, in two of four 38,
+// in four of eight 43, in one 46).
 int plan_blocks(const tq_hip_kv *kv, int n_q, int max_len, int *split_tokens, int *n_splits) {
     if (n_q == 1) return plan_decode3(kv, n_q, max_len, split_tokens, n_splits);
     plan_splits3(kv, n_q, max_len, 8, 256, split_tokens, n_splits);

@@ -25,13 +25,15 @@
 //   grid changed nothing (67, 72, 67).
 // score_kernel: eight lanes per block, 16 bytes of bounds each at a time (whole lines),
 //   scores as order-preserving 64-bit keys.  Bound by a bound's three instructions, of
-//   which the conversion to 64 bits runs at half the rate: 16 x 8 heads over 512 blocks in
-//   6.5 us of the kernel's 11.7 (33.6 MB), and by reading the bounds over more of them (16 x 8 over
-//   4,096 blocks, 268 MB in 69 us).  Reading four blocks ahead changed nothing.
+//   which the conversion to 64 bits runs at half the rate, and over many blocks by reading
+//   the bounds (16 x 8 heads over 4,096 blocks, 268 MB in 55 us).  Reading four blocks ahead
+//   changed nothing.
 // select_kernel, one work-group per (query, kv head): the keep-th largest key by
 //   counting into bins over the range that the keys have, again within the bin at the
 //   edge until it is settled; then ranks in order by ballots, each wave on one run of
-//   blocks.  It scores the blocks itself where that fills the card (tq_select_chunk).
+//   blocks.  It scores the blocks itself where that fills the card (tq_select_chunk): 16 x 8
+//   heads over 512 blocks (33.6 MB) in 15 us, where two kernels take 11.6 for the scores
+//   and 5.5 for the choice.
 #include <algorithm>
 
 #include "tq_common.hpp"
@@ -284,8 +286,8 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 
 // Grid (kv head, query).  This work-group makes the keys, in LDS (kMade), or score_kernel
 // did, in the workspace: up to kKeysInLds of them are copied from there (kCopied: each of
-// some six looks at them would wait for the L2; 4,096 blocks of 1 query 17.5 us and 20.9,
-// of 8 36.8 and 40.1, 1,024 of 1 11.9 and 12.3).
+// some six looks at them would wait for the L2; 4,090 blocks of 1 query 16.9 us and 20.5,
+// of 8 35.1 and 39.0, 1,024 of 1 11.6 and 12.0).
 enum { kMade, kCopied, kKept };
 template <int HD, int WAVES, int KEYS>
 __global__ __launch_bounds__(64 * WAVES) void select_kernel(TqSelectArgs a) {
@@ -435,8 +437,8 @@ __global__ __launch_bounds__(64 * WAVES) void select_kernel(TqSelectArgs a) {
 }
 
 // Four waves for up to 512 blocks, eight for more (four and eight, 32 / 8 heads of 128: 250
-// blocks of 64 queries 17.0 and 22.2 us, of 1 8.9 and 9.0, 500 of 64 27.3 and 31.2, of 1
-// 12.0 and 11.9; 2,000 of 16 34.9 and 34.0, 4,062 of 64 205 and 193).
+// blocks of 64 queries 17.1 and 22.4 us, of 1 9.2 and 9.4, 500 of 64 27.2 and 31.0, of 1
+// 11.2 and 10.9; 2,000 of 16 32.7 and 31.6, 4,090 of 16 59.0 and 56.3).
 constexpr int kFewBlocks = 512;
 
 template <int HD>
@@ -480,9 +482,10 @@ hipError_t tq_launch_bounds(const TqBoundsArgs &a, hipStream_t s) {
 
 // A launch of its own for the scores takes about 3 us and pays where the selecting
 // work-groups, one per (query, kv head), leave most CUs idle over many blocks.  32 / 8
-// heads of 128, in one launch and in two: 1,024 blocks of 1 query 16.1 and 11.4 us, 8
-// queries 19.1 and 16.4, 16 queries 20.3 and 21.1; 4,096 blocks of 1 query 45 and 17.5, 16
-// queries 69 and 69; 256 blocks 8.9 .. 10.9 and 10.0 .. 13.0.
+// heads of 128, in one launch and in two: 1,024 blocks of 1 query 16.7 and 11.6 us, 8
+// queries 18.4 and 16.7, 16 queries 20.3 and 21.6; 4,090 blocks of 1 query 43.8 and 16.9, 16
+// queries 56.3 and 54.6; 250 blocks of 1 query 9.2 and 10.4, of 64 17.1 and 20.0, 500 of 1
+// 11.2 and 9.8, of 64 27.2 and 30.3.
 int tq_select_chunk(int n_q, int n_kv_heads, int blocks) {
     const long pairs = (long)n_q * n_kv_heads;
     if (blocks <= kFewBlocks || (blocks <= kKeysInLds && pairs >= 128)) return 0;
