@@ -59,3 +59,33 @@ def test_a_step_by_itself_leaves_queries_of_no_sequence_out(nat, oracle):
     for i in (1, 4, 5):
         st.pos[i] = -1
     st.check(out)
+
+
+@pytest.mark.parametrize("length,keep", [(40, 3), (5000, 300)])
+@pytest.mark.parametrize("seq", [-1, 2])
+def test_one_query_of_no_sequence(nat, oracle, length, keep, seq):
+    """Alone in the call, over blocks and behind common tokens: nothing is written."""
+    c = Cache(nat, oracle, length, 8, 2, 64, [length, 5], room=1)
+    st = Step(c, [length], 16, keep, seqs=[0])
+    st.dev["seq"].upload(np.asarray([seq], np.int32))
+    out = st.run()
+    st.pos = [-1]
+    st.check(out)
+    st = Shared(nat, oracle, length, 8, 2, 64, [], behind=[length], order=[], large=False)
+    st.dev["seq"].upload(np.asarray([seq - 1], np.int32) if seq > 0 else np.asarray([seq], np.int32))
+    out = st.run()
+    st.pos = [-1]
+    st.check(out)
+
+
+def test_many_queries_some_of_no_sequence(nat, oracle):
+    """More than are ranked by length, over blocks."""
+    lens = [int(x) for x in np.random.default_rng(3).integers(0, 200, 140)]
+    st = Step(Cache(nat, oracle, 6, 4, 2, 64, lens, room=1), lens, 16, 4, seqs=list(range(140)))
+    seqs = np.arange(140, dtype=np.int32)
+    seqs[::9] = 140 + seqs[::9]
+    seqs[4::9] = -1 - seqs[4::9]
+    st.dev["seq"].upload(seqs)
+    out = st.run()
+    st.pos = [p if 0 <= s < 140 else -1 for p, s in zip(lens, seqs)]
+    st.check(out)
